@@ -24,6 +24,8 @@
  *   nncu_param_* / nncu_grad_*      NCParamList iteration         libnc.h:499-536
  *   nncu_attention_*                the attention sub-graph of
  *                                   trf_eval and its autograd     nncp.c:722-800
+ *   nncu_qk_norm_rope_*, nncu_linear_attention_*, nncu_distill_*
+ *                                   nothing: operators of a student model
  *
  * Layout conventions (all row-major, "row" = one (time, stream) position):
  *   - token ids, targets:  int32 [T][B]  (index t*B + b), exactly the
@@ -393,6 +395,130 @@ int nncu_attention_backward_noalloc(const nncu_attn_shape *s, const void *q, con
                                     const float *w_r, const float *b_r, const void *out,
                                     const float *lse, const void *dout, void *dq, void *dkv,
                                     float *dw_r, float *db_r, void *cuda_stream);
+
+/* ---- the operators of a student model -- no counterpart in the reference.
+ *
+ * What a small, fast model of its own needs that is to take over what the large one knows: queries and keys
+ * that carry their positions, attention over a state of constant size, a loss against the large model's
+ * likeliest symbols.  As for the isolated attention op, tensors are device memory of the CURRENT device, a row is
+ * one (time, stream) position (row = t*B + b), heads are column ranges of a row, and every call queues its
+ * kernels on cuda_stream and returns; nothing is allocated.  Row pitches (ld_*) are in elements, 0 means
+ * that rows lie one behind the other.  dtype_bf16 selects bf16 or fp32 for the activations; gains, states and
+ * losses are fp32.  Results must not overlap inputs but where a call says so.  Two calls that may overlap on the
+ * GPU need workspaces of their own; a captured call holds the addresses that it was given.
+ */
+
+/*
+ * Norm of queries and keys for each head and rotation by position in the same pass, for the attention
+ * ops of this file (nncu_attention_* with w_r NULL, nncu_linear_attention_*):
+ *   x^ = x / sqrt(mean(x^2) + eps) over a head's d_key values,  y = R(pos) (x^ * gain)
+ * R turns pair i of the first d_rot values by pos * rope_base^(-2i / d_rot); values behind them are only
+ * normed.  adjacent: pair i is (2i, 2i + 1), otherwise (i, i + d_rot / 2).
+ *   q [n_rows][n_head*d_key], k [n_rows][n_head_k*d_key] (n_head_k 0: none), gain_q, gain_k [d_key] (NULL: ones),
+ *   pos int32 [n_rows] (may be NULL when d_rot is 0).  A row with pos < 0 is padding: its values are
+ *   not looked at, its results and gradients are zeros.
+ * d_key even, up to NNCU_QK_NORM_DIM_MAX (NNCU_ERR_RANGE beyond); d_rot even, up to d_key.  q_out may be q and
+ * k_out k (same pitch).
+ */
+#define NNCU_QK_NORM_DIM_MAX 256
+typedef struct nncu_qk_norm_shape {
+    int32_t n_rows, n_head, n_head_k, d_key, d_rot;
+    int32_t ld_q, ld_k, ld_q_out, ld_k_out;
+    int32_t adjacent;
+    float eps, rope_base;
+    int32_t dtype_bf16;
+} nncu_qk_norm_shape;
+
+int nncu_qk_norm_rope_forward(const nncu_qk_norm_shape *s, const void *q, const void *k,
+                              const float *gain_q, const float *gain_k, const int32_t *pos,
+                              void *q_out, void *k_out, void *cuda_stream);
+/*
+ * Backward from the same inputs (nothing is saved by the forward pass): dq_out, dk_out with the pitches of
+ * q_out, k_out; dq, dk with those of q, k, and dq may be q or dq_out, dk k or dk_out (same pitch).  dgain_q,
+ * dgain_k [d_key], summed over rows and heads in a fixed order, may be NULL; where one is wanted a
+ * workspace of nncu_qk_norm_rope_workspace bytes is needed (16-byte aligned).
+ */
+int nncu_qk_norm_rope_workspace(const nncu_qk_norm_shape *s, size_t *bytes_out);
+int nncu_qk_norm_rope_backward(const nncu_qk_norm_shape *s, const void *q, const void *k,
+                               const float *gain_q, const float *gain_k, const int32_t *pos,
+                               const void *dq_out, const void *dk_out, void *dq, void *dk,
+                               float *dgain_q, float *dgain_k, void *workspace,
+                               size_t workspace_bytes, void *cuda_stream);
+
+/*
+ * Linear attention with a decay for each head:
+ *   S_t = decay_h S_(t-1) + k_t^T v_t        out_t = scale q_t S_t
+ *   q, k [T*B][H*d_key], v, out [T*B][H*d_value], states fp32 [B][H][d_key][d_value]
+ * decay_host [H] in host memory, each in (0, 1]: constants of the layer, read before the call returns.
+ * len int32 [B] (NULL: seg_len): the tokens of each stream, taken into [0, seg_len]; rows behind a stream's
+ * end are not looked at, out and the gradients are zeros there, and its state is the one behind its last token.
+ * state_in NULL: zeros.  state_out NULL: not wanted; it may be state_in.  One token (seg_len 1) is the
+ * decoder's step, a state carried from call to call.  Steps and whole segments add in another order, so that
+ * their last bits differ: what one codes the other does not decode.
+ * Up to NNCU_LINEAR_ATTN_HEADS_MAX heads of up to NNCU_LINEAR_ATTN_DIM_MAX values (NNCU_ERR_RANGE beyond).  A value
+ * that is not finite reaches rows of its stream from up to 63 tokens before it on.
+ */
+#define NNCU_LINEAR_ATTN_HEADS_MAX 64
+#define NNCU_LINEAR_ATTN_DIM_MAX 128
+typedef struct nncu_linear_attn_shape {
+    int32_t n_streams, n_head, d_key, d_value, seg_len;
+    int32_t ld_q, ld_k, ld_v, ld_out;
+    float scale;
+    int32_t dtype_bf16;
+} nncu_linear_attn_shape;
+
+/* bytes of workspace (16-byte aligned) of the forward or backward call; 0: NULL will do */
+int nncu_linear_attention_workspace(const nncu_linear_attn_shape *s, int backward, size_t *bytes_out);
+int nncu_linear_attention_forward(const nncu_linear_attn_shape *s, const void *q, const void *k,
+                                  const void *v, const float *decay_host, const int32_t *len,
+                                  const float *state_in, void *out, float *state_out,
+                                  void *workspace, size_t workspace_bytes, void *cuda_stream);
+/*
+ * Backward from the same inputs: dout with the pitch of out, dstate_out the gradient of state_out (NULL:
+ * zeros); dq, dk, dv with the pitches of q, k, v, dstate_in that of state_in (NULL: not wanted; it may be
+ * dstate_out).
+ */
+int nncu_linear_attention_backward(const nncu_linear_attn_shape *s, const void *q, const void *k,
+                                   const void *v, const float *decay_host, const int32_t *len,
+                                   const float *state_in, const void *dout,
+                                   const float *dstate_out, void *dq, void *dk, void *dv,
+                                   float *dstate_in, void *workspace, size_t workspace_bytes,
+                                   void *cuda_stream);
+
+/*
+ * A student's loss against a teacher's top logits, mixed with the coded symbol's own:
+ *   q = softmax(top_logits / temperature) over a row's entries
+ *   loss = row_weight [(1 - teacher_share) (-ln p[target])
+ *                      + teacher_share temperature^2 sum_k q_k (ln q_k - ln p_temperature[id_k])]
+ * with p the softmax of the row's logits and p_temperature that of logits / temperature, both over all symbols.
+ *   logits [n_rows][n_symbols], top_ids int32 and top_logits fp32 [n_rows][n_top], targets int32 [n_rows],
+ *   row_weight fp32 [n_rows] (NULL: ones), loss_rows fp32 [n_rows], dlogits like logits (bf16 or fp32 of its own)
+ * Entries whose id is outside [0, n_symbols) are not there (a teacher that sent fewer); a symbol may be
+ * named by several.  A row without entries has no teacher's term, one whose target is outside the alphabet (or
+ * targets NULL) none of its own.  A logit of -inf is a symbol that cannot come.  A row of weight 0, and one
+ * whose logits are all -inf, has loss 0 and gradient 0; the former is not looked at.
+ * n_top up to NNCU_DISTILL_TOP_MAX.  dlogits must not be logits.
+ */
+#define NNCU_DISTILL_TOP_MAX 1024
+typedef struct nncu_distill_shape {
+    int32_t n_rows, n_symbols, n_top;
+    int32_t ld_logits, ld_dlogits;
+    float temperature, teacher_share;
+    int32_t logits_bf16, grad_bf16;
+} nncu_distill_shape;
+
+/* The rows' losses, and lse fp32 [n_rows][2] for the backward call */
+int nncu_distill_forward(const nncu_distill_shape *s, const void *logits, const int32_t *top_ids,
+                         const float *top_logits, const int32_t *targets, const float *row_weight,
+                         float *loss_rows, float *lse, void *cuda_stream);
+/* The gradient of the sum of losses; a gradient that arrives for each loss goes into row_weight */
+int nncu_distill_backward(const nncu_distill_shape *s, const void *logits, const int32_t *top_ids,
+                          const float *top_logits, const int32_t *targets, const float *row_weight,
+                          const float *lse, void *dlogits, void *cuda_stream);
+/* Both in one pass over the logits */
+int nncu_distill_gradient(const nncu_distill_shape *s, const void *logits, const int32_t *top_ids,
+                          const float *top_logits, const int32_t *targets, const float *row_weight,
+                          float *loss_rows, void *dlogits, void *cuda_stream);
 
 /* ---- dense contraction used by every projection (nc_matmul, libnc.h:270-276) ----
  * C[M][N] = A[M][K] * B[N][K]^T (+ bias[N]), bf16 operands, fp32 accumulate,

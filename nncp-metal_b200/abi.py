@@ -7,6 +7,7 @@ FF_RELU, FF_GELU, FF_GEGLU, FF_GATED_SILU = 0, 1, 2, 3
 INIT_UNIFORM, INIT_NORMAL = 0, 1
 GEMM_AUTO, GEMM_SIMT, GEMM_TCGEN05 = 0, 1, 2
 NOALLOC_SCRATCH_FLOATS = 4 << 20
+QK_NORM_DIM_MAX, LINEAR_ATTN_HEADS_MAX, LINEAR_ATTN_DIM_MAX, DISTILL_TOP_MAX = 256, 64, 128, 1024
 OK, ERR_INVALID, ERR_CUDA, ERR_NOMEM, ERR_STATE, ERR_TIMEOUT, ERR_RANGE = range(7)
 
 
@@ -63,6 +64,25 @@ class AttnShape(C.Structure):
         ("attn_len", C.c_int32), ("t0", C.c_int32), ("t1", C.c_int32),
         ("br_scale", C.c_float), ("dtype_bf16", C.c_int32),
     ]
+
+
+class QkNormShape(C.Structure):
+    """struct nncu_qk_norm_shape (include/nncu.h)."""
+    _fields_ = [(n, C.c_int32) for n in ("n_rows", "n_head", "n_head_k", "d_key", "d_rot", "ld_q", "ld_k", "ld_q_out",
+                                         "ld_k_out", "adjacent")] + \
+        [("eps", C.c_float), ("rope_base", C.c_float), ("dtype_bf16", C.c_int32)]
+
+
+class LinearAttnShape(C.Structure):
+    """struct nncu_linear_attn_shape (include/nncu.h)."""
+    _fields_ = [(n, C.c_int32) for n in ("n_streams", "n_head", "d_key", "d_value", "seg_len", "ld_q", "ld_k", "ld_v",
+                                         "ld_out")] + [("scale", C.c_float), ("dtype_bf16", C.c_int32)]
+
+
+class DistillShape(C.Structure):
+    """struct nncu_distill_shape (include/nncu.h)."""
+    _fields_ = [(n, C.c_int32) for n in ("n_rows", "n_symbols", "n_top", "ld_logits", "ld_dlogits")] + \
+        [("temperature", C.c_float), ("teacher_share", C.c_float), ("logits_bf16", C.c_int32), ("grad_bf16", C.c_int32)]
 
 
 class Profile(C.Structure):
@@ -122,6 +142,15 @@ PROTOTYPES = {
     "nncu_attention_backward": (_i, [C.POINTER(AttnShape)] + [_vp] * 12),
     "nncu_attention_backward_noalloc": (_i, [C.POINTER(AttnShape)] + [_vp] * 12),
     "nncu_attention_reduce_tables": (_i, [C.POINTER(AttnShape), _vp, _vp, _vp, _vp, _i, _vp]),
+    "nncu_qk_norm_rope_forward": (_i, [C.POINTER(QkNormShape)] + [_vp] * 8),
+    "nncu_qk_norm_rope_workspace": (_i, [C.POINTER(QkNormShape), C.POINTER(_sz)]),
+    "nncu_qk_norm_rope_backward": (_i, [C.POINTER(QkNormShape)] + [_vp] * 12 + [_sz, _vp]),
+    "nncu_linear_attention_workspace": (_i, [C.POINTER(LinearAttnShape), _i, C.POINTER(_sz)]),
+    "nncu_linear_attention_forward": (_i, [C.POINTER(LinearAttnShape)] + [_vp] * 9 + [_sz, _vp]),
+    "nncu_linear_attention_backward": (_i, [C.POINTER(LinearAttnShape)] + [_vp] * 13 + [_sz, _vp]),
+    "nncu_distill_forward": (_i, [C.POINTER(DistillShape)] + [_vp] * 8),
+    "nncu_distill_backward": (_i, [C.POINTER(DistillShape)] + [_vp] * 8),
+    "nncu_distill_gradient": (_i, [C.POINTER(DistillShape)] + [_vp] * 8),
     "nncu_profile_begin": (_i, [_i]),
     "nncu_profile_end": (_i, [C.POINTER(Profile)]),
     "nncu_gemm_bf16": (_i, [_i, _i, _i, _i, _i, _vp, _i, _vp, _i, _vp, _i, _i, _vp]),
