@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "linear_attention.cuh"
 #include "op_checks.h"
@@ -28,7 +29,7 @@ static int lin_check(const nncu_linear_attn_shape *s)
 static void lin_parts(const nncu_linear_attn_shape *s, int *n_seg, int *seg)
 {
     const long long pairs = (long long)s->n_streams * s->n_head;
-    const int chunk = lin::FC, chunks = ceil_div(s->seg_len, chunk);
+    const int chunk = s->dtype_bf16 ? lin::TC : lin::FC, chunks = ceil_div(s->seg_len, chunk);
     int n = (int)std::min<long long>(std::max<long long>(SMS / pairs, 1), std::max(chunks / 4, 1));
     const int each = ceil_div(chunks, n);
     *seg = each * chunk;
@@ -86,6 +87,46 @@ template <typename T, bool STATES> static int lin_core(const lin::Args &a, cudaS
     return NNCU_OK;
 }
 
+template <int DA, int DC, bool STATES, int TERMS> static int lin_mma_launch(const lin::Args &a, cudaStream_t st)
+{
+    static DeviceOnce once;
+    NNCU_TRY(smem_limit(once, lin::mma_kernel<DA, DC, STATES, TERMS>, lin::MmaSmem<DA, DC>::BYTES));
+    CUDA_TRY(launch_k(lin::mma_kernel<DA, DC, STATES, TERMS>, dim3(a.B * a.H, STATES ? a.n_seg - 1 : a.n_seg), dim3(256),
+                      lin::MmaSmem<DA, DC>::BYTES, st, a));
+    KERNEL_CHECK();
+    return NNCU_OK;
+}
+
+template <int DA, int DC> static int lin_mma_sized(const lin::Args &a, cudaStream_t st)
+{
+    if (a.s_end) {
+        if (a.n_seg > 1)
+            NNCU_TRY((lin_mma_launch<DA, DC, true, 3>(a, st)));
+        return lin_mma_launch<DA, DC, false, 3>(a, st);
+    }
+    if (a.n_seg > 1)
+        NNCU_TRY((lin_mma_launch<DA, DC, true, 2>(a, st)));
+    return lin_mma_launch<DA, DC, false, 2>(a, st);
+}
+
+// head sizes go up to the next of 32, 64 and 128, zeros beyond their own
+static int lin_mma(const lin::Args &a, cudaStream_t st)
+{
+    auto with = [&](auto da) {
+        constexpr int DA = decltype(da)::value;
+        return a.dc <= 32 ? lin_mma_sized<DA, 32>(a, st) : a.dc <= 64 ? lin_mma_sized<DA, 64>(a, st) : lin_mma_sized<DA, 128>(a, st);
+    };
+    return a.da <= 32 ? with(std::integral_constant<int, 32>()) : a.da <= 64 ? with(std::integral_constant<int, 64>())
+                                                                            : with(std::integral_constant<int, 128>());
+}
+
+// rows laid out in 16-byte pieces
+static bool lin_pieces(const lin::Args &a)
+{
+    return a.da % 8 == 0 && a.dc % 8 == 0 && a.lda % 8 == 0 && a.ldb % 8 == 0 && a.ldc % 8 == 0 && a.ldo % 2 == 0 && aligned(a.a, 16) &&
+           aligned(a.b, 16) && aligned(a.c, 16) && aligned(a.o, 4);
+}
+
 // one pass of the form at the head of linear_attention.cuh
 template <typename T> static int lin_run(const lin::Args &a, cudaStream_t st)
 {
@@ -93,6 +134,8 @@ template <typename T> static int lin_run(const lin::Args &a, cudaStream_t st)
         const bool wide = a.dc % 4 == 0 && aligned(a.s0, 16) && aligned(a.s_end, 16);
         return wide ? lin_step<T, 4>(a, st) : lin_step<T, 1>(a, st);
     }
+    if (sizeof(T) == 2 && lin_pieces(a))
+        return lin_mma(a, st);
     if (a.n_seg > 1)
         NNCU_TRY((lin_core<T, true>(a, st)));
     return lin_core<T, false>(a, st);

@@ -245,6 +245,274 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
             to[i] = Ss[i / p.dc * sm.ld_c + i % p.dc];
 }
 
+// ---------------- bf16 on warp-level tensor-core products ----------------
+//
+// A CTA of eight warps goes through one part of one (stream, head) in chunks of 64 tokens.  Warp (r, hc) takes rows
+// 16 r .. 16 r + 15 of a chunk and half hc of the columns of c; of the state it owns the same columns of rows 16 r .. (and
+// 16 (r + 4) .. of 128) in fp32 accumulators.  The results need all of the state: it goes through shared memory in bf16,
+// one rounding, as the pair weights P have one; products of a decayed b with c, which the state adds up, are kept to
+// 24 bits by three bf16 terms of the decayed value, so that the state is an fp32 sum of fp32 products.  The next chunk's
+// tiles are fetched under the present chunk, and one barrier a chunk hands over tiles and state.
+
+constexpr int TC = 64; // tokens in a chunk
+
+template <int DA, int DC> struct MmaSmem {
+    static constexpr int LA = DA + 8, LC = DC + 8;            // pitches: rows four banks on
+    static constexpr int A = 0, B = A + 2 * TC * LA * 2, C = B + 2 * TC * LA * 2, S = C + 2 * TC * LC * 2,
+                         W = S + 2 * DA * LC * 2, BYTES = W + (2 * TC + 8) * 4;
+};
+
+// 64 rows of a matrix as a tile, zeros behind row n and column d
+template <int D>
+__device__ __forceinline__ void tile_load(bf16 *dst, const bf16 *src, long long ldr, int d, const Rows &rows, int u0, int n)
+{
+    constexpr int CPR = D / 8;
+    for (int i = threadIdx.x; i < TC * CPR; i += 256) {
+        const int r = i / CPR, x = i % CPR * 8;
+        const bool ok = r < n && x < d;
+        fa::cp16(dst + r * (D + 8) + x, ok ? src + rows.row(u0 + r) * ldr + x : src, ok);
+    }
+}
+
+// a pair of bf16 values times their weights as three bf16 terms that add up to 24 bits of them
+__device__ __forceinline__ void split3(uint32_t v, float w0, float w1, uint32_t &hi, uint32_t &mid, uint32_t &lo)
+{
+    float x = __uint_as_float(v << 16) * w0, y = __uint_as_float(v & 0xffff0000u) * w1;
+    hi = fa::pack2(x, y);
+    x -= __uint_as_float(hi << 16);
+    y -= __uint_as_float(hi & 0xffff0000u);
+    mid = fa::pack2(x, y);
+    lo = fa::pack2(x - __uint_as_float(mid << 16), y - __uint_as_float(mid & 0xffff0000u));
+}
+
+// TERMS: 3, or 2 where no state is a result (17 bits of a decayed value are more than the rounding behind them keeps)
+template <int DA, int DC, bool STATES, int TERMS>
+__global__ void __launch_bounds__(256) mma_kernel(const __grid_constant__ Args p)
+{
+    using SM = MmaSmem<DA, DC>;
+    constexpr int LA = SM::LA, LC = SM::LC, NT = DC / 16, MT = DA > 64 ? DA / 64 : 1, KS = DA / 16;
+    extern __shared__ __align__(16) unsigned char smb[];
+    bf16 *As = reinterpret_cast<bf16 *>(smb + SM::A), *Bs = reinterpret_cast<bf16 *>(smb + SM::B),
+         *Cs = reinterpret_cast<bf16 *>(smb + SM::C), *Ss = reinterpret_cast<bf16 *>(smb + SM::S);
+    float *wts = reinterpret_cast<float *>(smb + SM::W), *pw16 = wts + 2 * TC; // weights of full and last chunks; l^16m
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
+    // the two warps of a scheduler take rows r and 3 - r: the triangle is dealt evenly
+    const int hc = warp >> 2, r = hc ? 3 - (warp & 3) : warp & 3;
+    const size_t pair = blockIdx.x;
+    const int g = blockIdx.y, b = (int)(pair / p.H), h = (int)(pair % p.H);
+    const float rate = p.rate[h];
+    pdl_trigger();
+    pdl_wait();
+    const Rows rows(p, b);
+    const size_t nn = (size_t)p.da * p.dc;
+    const int begin = g * p.seg, end = min(rows.n, begin + p.seg), total = max(end - begin, 0), chunks = (total + TC - 1) / TC;
+    const bf16 *ga = reinterpret_cast<const bf16 *>(p.a) + (size_t)h * p.da, *gb = reinterpret_cast<const bf16 *>(p.b) + (size_t)h * p.da,
+               *gc = reinterpret_cast<const bf16 *>(p.c) + (size_t)h * p.dc;
+    auto fetch = [&](int k) {
+        const int u0 = begin + k * TC, n = end - u0, buf = k & 1;
+        if (!STATES)
+            tile_load<DA>(As + buf * TC * LA, ga, p.lda, p.da, rows, u0, n);
+        tile_load<DA>(Bs + buf * TC * LA, gb, p.ldb, p.da, rows, u0, n);
+        tile_load<DC>(Cs + buf * TC * LC, gc, p.ldc, p.dc, rows, u0, n);
+        fa::cp_commit();
+    };
+    if (chunks)
+        fetch(0);
+    const int n_last = total - (chunks - 1) * TC;
+    if (tid < TC)
+        wts[tid] = p.s_in * power(rate, TC - 1 - tid + p.e2);
+    else if (tid < 2 * TC)
+        wts[tid] = tid - TC < n_last ? p.s_in * power(rate, n_last - 1 - (tid - TC) + p.e2) : 0.0f;
+    else if (tid < 2 * TC + 4)
+        pw16[tid - 2 * TC] = power(rate, 16 * (tid - 2 * TC));
+
+    // the state: element c of s[m][n] is row 16 (r + 4 m) + gq + 8 (c >> 1), column hc * DC / 2 + 8 n + 2 t + (c & 1)
+    float s[MT][NT][4];
+    const float l_seg = power(rate, p.seg), l_full = power(rate, TC), l_last = power(rate, n_last);
+    const bool has_state = r * 16 < DA; // of 32 rows the warps r = 2, 3 own none
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int x = 16 * (r + 4 * m) + gq + 8 * (c >> 1), y = hc * (DC / 2) + 8 * n + 2 * t + (c & 1);
+                s[m][n][c] = 0.0f;
+                if (x < p.da && y < p.dc) {
+                    if (!STATES)
+                        s[m][n][c] = start_at(p, pair, g, x, y, l_seg);
+                    else if (g == 0) // the state before the first token is kept: s_end may lie where it lies
+                        p.parts[pair * p.n_seg * nn + (size_t)x * p.dc + y] = p.s0 ? state_at(p, p.s0 + pair * nn, x, y) : 0.0f;
+                }
+            }
+    auto publish = [&](int buf) {
+        if (!STATES && has_state)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    bf16 *to = Ss + buf * DA * LC + (16 * (r + 4 * m) + gq) * LC + hc * (DC / 2) + 8 * n + 2 * t;
+                    *reinterpret_cast<uint32_t *>(to) = fa::pack2(s[m][n][0], s[m][n][1]);
+                    *reinterpret_cast<uint32_t *>(to + 8 * LC) = fa::pack2(s[m][n][2], s[m][n][3]);
+                }
+    };
+    publish(0);
+    if (!STATES && p.o)
+        zero_behind<bf16>(p, rows, b, h, g, tid, 256);
+
+    // weights of pairs 16 rows apart and on the diagonal, of this thread's elements of two 8-key groups
+    float apart[2][4], diag[2][4];
+    const float f_a = p.s_state * power(rate, 16 * r + gq + p.e1), f_b = p.s_state * power(rate, 16 * r + gq + 8 + p.e1);
+#pragma unroll
+    for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const int d = gq + 8 * (c >> 1) - 8 * n - 2 * t - (c & 1);
+            apart[n][c] = p.s_pair * power(rate, 16 + d);
+            diag[n][c] = d >= 0 ? p.s_pair * power(rate, d) : 0.0f;
+        }
+
+    for (int k = 0; k < chunks; k++) {
+        const int buf = k & 1, u0 = begin + k * TC, n = min(TC, end - u0);
+        const bool last = k == chunks - 1;
+        fa::cp_wait<0>();
+        __syncthreads(); // this chunk's tiles and state stand; the other buffers are free
+        if (!last)
+            fetch(k + 1);
+        const bf16 *At = As + buf * TC * LA, *Bt = Bs + buf * TC * LA, *Ct = Cs + buf * TC * LC + hc * (DC / 2),
+                   *St = Ss + buf * DA * LC + hc * (DC / 2);
+        float o[NT][4];
+        if (!STATES) {
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    o[x][c] = 0.0f;
+            uint32_t aq[KS][4];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                fa::ldsm4(aq[ks], At + (16 * r + (lane & 15)) * LA + ks * 16 + (lane >> 4) * 8);
+#pragma unroll
+                for (int x = 0; x < NT; x += 2) {
+                    uint32_t f[4];
+                    fa::ldsm4t(f, St + (ks * 16 + (lane & 15)) * LC + x * 8 + (lane >> 4) * 8);
+                    fa::mma(o[x], aq[ks], f[0], f[1]);
+                    fa::mma(o[x + 1], aq[ks], f[2], f[3]);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < NT; x++) {
+                o[x][0] *= f_a; o[x][1] *= f_a;
+                o[x][2] *= f_b; o[x][3] *= f_b;
+            }
+#pragma unroll
+            for (int pc = 0; pc < 4; pc++) {
+                if (pc > r)
+                    break;
+                float w[2][4] = {};
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    uint32_t f[4];
+                    fa::ldsm4(f, Bt + (pc * 16 + (lane & 7) + (lane >> 4) * 8) * LA + ks * 16 + ((lane >> 3) & 1) * 8);
+                    fa::mma(w[0], aq[ks], f[0], f[1]);
+                    fa::mma(w[1], aq[ks], f[2], f[3]);
+                }
+                if (pc == r) {
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+                            w[x][c] = gq + 8 * (c >> 1) >= 8 * x + 2 * t + (c & 1) ? w[x][c] * diag[x][c] : 0.0f;
+                } else {
+                    const float f = pw16[r - pc - 1];
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+                            w[x][c] *= f * apart[x][c];
+                }
+                const uint32_t pf[4] = {fa::pack2(w[0][0], w[0][1]), fa::pack2(w[0][2], w[0][3]), fa::pack2(w[1][0], w[1][1]),
+                                        fa::pack2(w[1][2], w[1][3])};
+#pragma unroll
+                for (int x = 0; x < NT; x += 2) {
+                    uint32_t f[4];
+                    fa::ldsm4t(f, Ct + (pc * 16 + (lane & 15)) * LC + x * 8 + (lane >> 4) * 8);
+                    fa::mma(o[x], pf, f[0], f[1]);
+                    fa::mma(o[x + 1], pf, f[2], f[3]);
+                }
+            }
+            // rows out: a lane's column pairs
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+                const int i = 16 * r + gq + 4 * c;
+                bf16 *to = reinterpret_cast<bf16 *>(p.o) + (i < n ? rows.row(u0 + i) * p.ldo : 0) + (size_t)h * p.dc + hc * (DC / 2) + 2 * t;
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+                    if (i < n && hc * (DC / 2) + 8 * x < p.dc)
+                        *reinterpret_cast<uint32_t *>(to + 8 * x) = fa::pack2(o[x][c], o[x][c + 1]);
+            }
+        }
+        if (last && !STATES && !p.s_end)
+            break;
+        // the state behind the chunk
+        const float l_n = last ? l_last : l_full, *wt = wts + (last ? TC : 0);
+        if (has_state) {
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        s[m][x][c] *= l_n;
+#pragma unroll
+            for (int ks = 0; ks < TC / 16; ks++) {
+                const float2 w0 = *reinterpret_cast<const float2 *>(wt + ks * 16 + 2 * t), w8 = *reinterpret_cast<const float2 *>(wt + ks * 16 + 8 + 2 * t);
+                uint32_t hi[MT][4], mid[MT][4], lo[MT][4];
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    uint32_t f[4];
+                    fa::ldsm4t(f, Bt + (ks * 16 + (lane & 7) + (lane >> 4) * 8) * LA + 16 * (r + 4 * m) + ((lane >> 3) & 1) * 8);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        split3(f[e], e < 2 ? w0.x : w8.x, e < 2 ? w0.y : w8.y, hi[m][e], mid[m][e], lo[m][e]);
+                }
+#pragma unroll
+                for (int x = 0; x < NT; x += 2) {
+                    uint32_t f[4];
+                    fa::ldsm4t(f, Ct + (ks * 16 + (lane & 15)) * LC + x * 8 + (lane >> 4) * 8);
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        fa::mma(s[m][x], hi[m], f[0], f[1]);
+                        fa::mma(s[m][x + 1], hi[m], f[2], f[3]);
+                        fa::mma(s[m][x], mid[m], f[0], f[1]);
+                        fa::mma(s[m][x + 1], mid[m], f[2], f[3]);
+                        if (TERMS > 2) {
+                            fa::mma(s[m][x], lo[m], f[0], f[1]);
+                            fa::mma(s[m][x + 1], lo[m], f[2], f[3]);
+                        }
+                    }
+                }
+            }
+        }
+        if (!last)
+            publish(buf ^ 1);
+    }
+    float *to = STATES ? p.parts + (pair * p.n_seg + g + 1) * nn
+                       : (p.s_end && begin < max(rows.n, 1) && max(rows.n, 1) <= begin + p.seg ? p.s_end + pair * nn : nullptr);
+    if (to && has_state)
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int i = 16 * (r + 4 * m) + gq + 8 * (c >> 1), y = hc * (DC / 2) + 8 * x + 2 * t + (c & 1);
+                    if (i < p.da && y < p.dc)
+                        to[(size_t)i * p.dc + y] = s[m][x][c];
+                }
+}
+
+
 // ---------------- a few tokens: the recurrence itself ----------------
 //
 // A CTA of four warps takes 8 * VEC columns of one (stream, head)'s state into registers, sixteen rows side by side, and
