@@ -467,7 +467,7 @@ typedef struct nncu_linear_attn_shape {
     int32_t dtype_bf16;
 } nncu_linear_attn_shape;
 
-/* bytes of workspace (16-byte aligned) of the forward or backward call; 0: NULL will do */
+/* bytes of workspace (16-byte aligned) that the forward call, or with backward both calls need; 0: NULL will do */
 int nncu_linear_attention_workspace(const nncu_linear_attn_shape *s, int backward, size_t *bytes_out);
 int nncu_linear_attention_forward(const nncu_linear_attn_shape *s, const void *q, const void *k,
                                   const void *v, const float *decay_host, const int32_t *len,

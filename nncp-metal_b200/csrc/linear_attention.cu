@@ -26,124 +26,166 @@ static int lin_check(const nncu_linear_attn_shape *s)
 
 // In how many parts a stream's tokens are cut.  One part is one pass over the tokens; more parts read b and c
 // twice, and pay where one CTA for each (stream, head) would leave most SMs without work.
-static void lin_parts(const nncu_linear_attn_shape *s, int *n_seg, int *seg)
+static void lin_parts(const nncu_linear_attn_shape *s, int roles, int *n_seg, int *seg)
 {
-    const long long pairs = (long long)s->n_streams * s->n_head;
+    const long long ctas = (long long)s->n_streams * s->n_head * roles;
     const int chunk = s->dtype_bf16 ? lin::TC : lin::FC, chunks = ceil_div(s->seg_len, chunk);
-    int n = (int)std::min<long long>(std::max<long long>(SMS / pairs, 1), std::max(chunks / 4, 1));
+    long long want = SMS;
+    if (getenv("LIN_WANT")) want = atoi(getenv("LIN_WANT"));
+    int n = (int)std::min<long long>(std::max<long long>(want / ctas, 1), std::max(chunks / 4, 1));
     const int each = ceil_div(chunks, n);
     *seg = each * chunk;
     *n_seg = ceil_div(chunks, each);
 }
 
-static size_t lin_need(const nncu_linear_attn_shape *s)
+// floats of a state in a workspace: the tensor-core kernel's, head sizes up to the next of 32, 64 and 128 and four
+// groups of 16 rows
+static int lin_slot(const nncu_linear_attn_shape *s)
+{
+    auto up = [](int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; };
+    const int k = up(s->d_key), v = up(s->d_value);
+    return std::max(std::max(k, 64) * v, std::max(v, 64) * k); // [d_key][d_value] and the other way round
+}
+
+static size_t lin_need(const nncu_linear_attn_shape *s, int roles)
 {
     if (s->seg_len <= lin::STEP_TOKENS)
         return 0;
     int n_seg, seg;
-    lin_parts(s, &n_seg, &seg);
-    return n_seg > 1 ? sizeof(float) * (size_t)s->n_streams * s->n_head * n_seg * s->d_key * s->d_value : 0;
+    lin_parts(s, roles, &n_seg, &seg);
+    return n_seg > 1 ? sizeof(float) * (size_t)roles * s->n_streams * s->n_head * n_seg * lin_slot(s) : 0;
 }
 
-static int lin_common(const nncu_linear_attn_shape *s, const float *decay_host, const void *workspace, size_t workspace_bytes)
+static int lin_common(const nncu_linear_attn_shape *s, int roles, const float *decay_host, const void *workspace, size_t workspace_bytes)
 {
     if (!decay_host)
         return nncu_fail(NNCU_ERR_INVALID, "null tensor");
     for (int h = 0; h < s->n_head; h++)
         if (!(decay_host[h] > 0.0f && decay_host[h] <= 1.0f))
             return nncu_fail(NNCU_ERR_INVALID, "linear attention: the decay of head %d is not in (0, 1]", h);
-    if (lin_need(s) > workspace_bytes || (lin_need(s) && (!workspace || !aligned(workspace, 16))))
-        return nncu_fail(NNCU_ERR_INVALID, "linear attention: a workspace of %zu bytes that begins at a multiple of 16 is needed", lin_need(s));
+    const size_t need = lin_need(s, roles);
+    if (need > workspace_bytes || (need && (!workspace || !aligned(workspace, 16))))
+        return nncu_fail(NNCU_ERR_INVALID, "linear attention: a workspace of %zu bytes that begins at a multiple of 16 is needed", need);
     return NNCU_OK;
 }
 
-static lin::Args lin_args(const nncu_linear_attn_shape *s, const float *decay_host, const int32_t *len, void *workspace)
+static lin::Args lin_args(const nncu_linear_attn_shape *s, int roles, const float *decay_host, const int32_t *len, void *workspace)
 {
     lin::Args a;
     memset(&a, 0, sizeof(a));
     a.len = len;
-    a.parts = (float *)workspace;
     a.B = s->n_streams; a.H = s->n_head; a.T = s->seg_len;
-    lin_parts(s, &a.n_seg, &a.seg);
+    lin_parts(s, roles, &a.n_seg, &a.seg);
+    a.slot = lin_slot(s);
+    for (int i = 0; i < roles; i++)
+        a.role[i].parts = (float *)workspace + (size_t)i * a.B * a.H * a.n_seg * a.slot;
     for (int h = 0; h < s->n_head; h++)
         a.rate[h] = (float)log2((double)decay_host[h]);
     return a;
 }
 
-template <typename T, int VEC> static int lin_step(const lin::Args &a, cudaStream_t st)
+template <typename T, int VEC> static int lin_step(const lin::Args &a, int roles, int dc, cudaStream_t st)
 {
-    CUDA_TRY(launch_k(lin::step_kernel<T, VEC>, dim3(a.B * a.H, ceil_div(a.dc, 8 * VEC)), dim3(128), 0, st, a));
+    CUDA_TRY(launch_k(lin::step_kernel<T, VEC>, dim3(a.B * a.H, ceil_div(dc, 8 * VEC), roles), dim3(128), 0, st, a));
     KERNEL_CHECK();
     return NNCU_OK;
 }
 
-template <typename T, bool STATES> static int lin_core(const lin::Args &a, cudaStream_t st)
+template <typename T, bool STATES> static int lin_core(const lin::Args &a, int roles, cudaStream_t st)
 {
     static DeviceOnce once;
     NNCU_TRY(smem_limit(once, lin::core_kernel<T, STATES>, 4 * lin::CoreSmem(lin::DIM_MAX, lin::DIM_MAX).floats));
-    CUDA_TRY(launch_k(lin::core_kernel<T, STATES>, dim3(a.B * a.H, STATES ? a.n_seg - 1 : a.n_seg), dim3(256),
-                      4 * lin::CoreSmem(a.da, a.dc).floats, st, a));
+    int floats = 0;
+    for (int i = 0; i < roles; i++)
+        floats = std::max(floats, lin::CoreSmem(a.role[i].da, a.role[i].dc).floats);
+    CUDA_TRY(launch_k(lin::core_kernel<T, STATES>, dim3(a.B * a.H, STATES ? a.n_seg - 1 : a.n_seg, roles), dim3(256), 4 * floats, st, a));
     KERNEL_CHECK();
     return NNCU_OK;
 }
 
-template <int DA, int DC, bool STATES, int TERMS> static int lin_mma_launch(const lin::Args &a, cudaStream_t st)
+template <int DA, int DC, bool STATES> static int lin_mma_launch(const lin::MmaArgs &m, int roles, cudaStream_t st)
 {
     static DeviceOnce once;
-    NNCU_TRY(smem_limit(once, lin::mma_kernel<DA, DC, STATES, TERMS>, lin::MmaSmem<DA, DC>::BYTES));
-    CUDA_TRY(launch_k(lin::mma_kernel<DA, DC, STATES, TERMS>, dim3(a.B * a.H, STATES ? a.n_seg - 1 : a.n_seg), dim3(256),
-                      lin::MmaSmem<DA, DC>::BYTES, st, a));
+    NNCU_TRY(smem_limit(once, lin::mma_kernel<DA, DC, STATES>, lin::MmaSmem<DA, DC>::BYTES));
+    CUDA_TRY(launch_k(lin::mma_kernel<DA, DC, STATES>, dim3(m.p.B * m.p.H, STATES ? m.p.n_seg - 1 : m.p.n_seg, roles), dim3(4 * DC),
+                      lin::MmaSmem<DA, DC>::BYTES, st, m));
     KERNEL_CHECK();
     return NNCU_OK;
 }
 
-template <int DA, int DC> static int lin_mma_sized(const lin::Args &a, cudaStream_t st)
+// 64 tokens x `cols` values of one head of rows [T*B][ld]
+static int lin_map(const lin::Args &a, const void *rows, long long ld, int d, int cols, CUtensorMap *out)
 {
-    if (a.s_end) {
-        if (a.n_seg > 1)
-            NNCU_TRY((lin_mma_launch<DA, DC, true, 3>(a, st)));
-        return lin_mma_launch<DA, DC, false, 3>(a, st);
+    tc::EncodeTiledFn fn = tc::encode_fn();
+    if (!fn)
+        return nncu_fail(NNCU_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)a.H, (cuuint64_t)a.B, (cuuint64_t)a.T};
+    const cuuint64_t strides[3] = {(cuuint64_t)d * 2, (cuuint64_t)ld * 2, (cuuint64_t)ld * 2 * a.B};
+    const cuuint32_t box[4] = {(cuuint32_t)std::min(cols, 64), 1, 1, lin::TC}, each[4] = {1, 1, 1, 1};
+    const CUresult rc = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(rows), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? NNCU_OK : nncu_fail(NNCU_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)rc);
+}
+
+template <int DA, int DC> static int lin_mma_sized(const lin::Args &a, int roles, cudaStream_t st)
+{
+    lin::MmaArgs m;
+    m.p = a;
+    for (int i = 0; i < roles; i++) {
+        const lin::Role &q = a.role[i];
+        NNCU_TRY(lin_map(a, q.a, q.lda, q.da, DA, &m.map[i][0]));
+        NNCU_TRY(lin_map(a, q.b, q.ldb, q.da, DA, &m.map[i][1]));
+        NNCU_TRY(lin_map(a, q.c, q.ldc, q.dc, DC, &m.map[i][2]));
     }
     if (a.n_seg > 1)
-        NNCU_TRY((lin_mma_launch<DA, DC, true, 2>(a, st)));
-    return lin_mma_launch<DA, DC, false, 2>(a, st);
+        NNCU_TRY((lin_mma_launch<DA, DC, true>(m, roles, st)));
+    return lin_mma_launch<DA, DC, false>(m, roles, st);
 }
 
 // head sizes go up to the next of 32, 64 and 128, zeros beyond their own
-static int lin_mma(const lin::Args &a, cudaStream_t st)
+static int lin_mma(const lin::Args &a, int roles, cudaStream_t st)
 {
-    auto with = [&](auto da) {
-        constexpr int DA = decltype(da)::value;
-        return a.dc <= 32 ? lin_mma_sized<DA, 32>(a, st) : a.dc <= 64 ? lin_mma_sized<DA, 64>(a, st) : lin_mma_sized<DA, 128>(a, st);
+    const int dc = a.role[0].dc, da = a.role[0].da;
+    auto with = [&](auto size) {
+        constexpr int DA = decltype(size)::value;
+        return dc <= 32 ? lin_mma_sized<DA, 32>(a, roles, st) : dc <= 64 ? lin_mma_sized<DA, 64>(a, roles, st) : lin_mma_sized<DA, 128>(a, roles, st);
     };
-    return a.da <= 32 ? with(std::integral_constant<int, 32>()) : a.da <= 64 ? with(std::integral_constant<int, 64>())
-                                                                            : with(std::integral_constant<int, 128>());
+    return da <= 32 ? with(std::integral_constant<int, 32>()) : da <= 64 ? with(std::integral_constant<int, 64>())
+                                                                         : with(std::integral_constant<int, 128>());
 }
 
-// rows laid out in 16-byte pieces
-static bool lin_pieces(const lin::Args &a)
+// rows laid out in 16-byte pieces, and pitches that a tensor map takes
+static bool lin_pieces(const lin::Role &q, long long B)
 {
-    return a.da % 8 == 0 && a.dc % 8 == 0 && a.lda % 8 == 0 && a.ldb % 8 == 0 && a.ldc % 8 == 0 && a.ldo % 2 == 0 && aligned(a.a, 16) &&
-           aligned(a.b, 16) && aligned(a.c, 16) && aligned(a.o, 4);
+    for (long long ld : {q.lda, q.ldb, q.ldc, q.ldo})
+        if (ld % 8 != 0 || ld * B * 2 >= 1ll << 40)
+            return false;
+    return q.da % 8 == 0 && q.dc % 8 == 0 && aligned(q.a, 16) && aligned(q.b, 16) && aligned(q.c, 16) && aligned(q.o, 16) && aligned(q.s0, 8) &&
+           aligned(q.s_end, 8);
 }
 
-// one pass of the form at the head of linear_attention.cuh
-template <typename T> static int lin_run(const lin::Args &a, cudaStream_t st)
+// Roles of the same head sizes, side by side in one launch, in the form at the head of linear_attention.cuh
+template <typename T> static int lin_run(const lin::Args &a, int roles, cudaStream_t st)
 {
-    if (a.T <= lin::STEP_TOKENS) {
-        const bool wide = a.dc % 4 == 0 && aligned(a.s0, 16) && aligned(a.s_end, 16);
-        return wide ? lin_step<T, 4>(a, st) : lin_step<T, 1>(a, st);
+    bool pieces = sizeof(T) == 2, wide = true;
+    for (int i = 0; i < roles; i++) {
+        const lin::Role &q = a.role[i];
+        pieces = pieces && lin_pieces(q, a.B);
+        wide = wide && q.dc % 4 == 0 && aligned(q.s0, 16) && aligned(q.s_end, 16);
     }
-    if (sizeof(T) == 2 && lin_pieces(a))
-        return lin_mma(a, st);
+    if (a.T <= lin::STEP_TOKENS)
+        return wide ? lin_step<T, 4>(a, roles, a.role[0].dc, st) : lin_step<T, 1>(a, roles, a.role[0].dc, st);
+    if (pieces)
+        return lin_mma(a, roles, st);
     if (a.n_seg > 1)
-        NNCU_TRY((lin_core<T, true>(a, st)));
-    return lin_core<T, false>(a, st);
+        NNCU_TRY((lin_core<T, true>(a, roles, st)));
+    return lin_core<T, false>(a, roles, st);
 }
 
-static int lin_any(const nncu_linear_attn_shape *s, const lin::Args &a, cudaStream_t st)
+static int lin_any(const nncu_linear_attn_shape *s, const lin::Args &a, int roles, cudaStream_t st)
 {
-    return s->dtype_bf16 ? lin_run<bf16>(a, st) : lin_run<float>(a, st);
+    return s->dtype_bf16 ? lin_run<bf16>(a, roles, st) : lin_run<float>(a, roles, st);
 }
 
 extern "C" {
@@ -153,8 +195,7 @@ int nncu_linear_attention_workspace(const nncu_linear_attn_shape *s, int backwar
     NNCU_TRY(lin_check(s));
     if (!bytes_out)
         return nncu_fail(NNCU_ERR_INVALID, "null argument");
-    (void)backward;
-    *bytes_out = lin_need(s);
+    *bytes_out = std::max(lin_need(s, 1), backward ? lin_need(s, 3) : 0);
     return NNCU_OK;
 }
 
@@ -165,13 +206,14 @@ int nncu_linear_attention_forward(const nncu_linear_attn_shape *s, const void *q
     NNCU_TRY(lin_check(s));
     if (!q || !k || !v || !out)
         return nncu_fail(NNCU_ERR_INVALID, "null tensor");
-    NNCU_TRY(lin_common(s, decay_host, workspace, workspace_bytes));
+    NNCU_TRY(lin_common(s, 1, decay_host, workspace, workspace_bytes));
     if (out == q || out == k || out == v)
         return nncu_fail(NNCU_ERR_INVALID, "linear attention: the result cannot go over q, k or v");
     NNCU_TRY(elements_aligned({q, k, v, out}, s->dtype_bf16 ? 2 : 4));
     NNCU_TRY(elements_aligned({len, state_in, state_out}, 4));
-    NNCU_TRY(on_device({q, k, v, len, state_in, out, state_out, lin_need(s) ? workspace : nullptr}));
-    lin::Args a = lin_args(s, decay_host, len, workspace);
+    NNCU_TRY(on_device({q, k, v, len, state_in, out, state_out, lin_need(s, 1) ? workspace : nullptr}));
+    lin::Args args = lin_args(s, 1, decay_host, len, workspace);
+    lin::Role &a = args.role[0];
     const long long wk = (long long)s->n_head * s->d_key, wv = (long long)s->n_head * s->d_value;
     a.a = q; a.b = k; a.c = v; a.o = out;
     a.lda = s->ld_q ? s->ld_q : wk; a.ldb = s->ld_k ? s->ld_k : wk; a.ldc = s->ld_v ? s->ld_v : wv; a.ldo = s->ld_out ? s->ld_out : wv;
@@ -181,7 +223,7 @@ int nncu_linear_attention_forward(const nncu_linear_attn_shape *s, const void *q
     a.s_state = a.s_pair = s->scale;
     a.s_in = 1.0f;
     ChainScope chain;
-    return lin_any(s, a, (cudaStream_t)cuda_stream);
+    return lin_any(s, args, 1, (cudaStream_t)cuda_stream);
 }
 
 int nncu_linear_attention_backward(const nncu_linear_attn_shape *s, const void *q, const void *k, const void *v, const float *decay_host,
@@ -191,40 +233,39 @@ int nncu_linear_attention_backward(const nncu_linear_attn_shape *s, const void *
     NNCU_TRY(lin_check(s));
     if (!q || !k || !v || !dout || !dq || !dk || !dv)
         return nncu_fail(NNCU_ERR_INVALID, "null tensor");
-    NNCU_TRY(lin_common(s, decay_host, workspace, workspace_bytes));
+    NNCU_TRY(lin_common(s, 3, decay_host, workspace, workspace_bytes));
     for (const void *to : {dq, dk, dv})
         if (to == q || to == k || to == v || to == dout || (to == dq) + (to == dk) + (to == dv) > 1)
             return nncu_fail(NNCU_ERR_INVALID, "linear attention: a gradient needs a place of its own");
     NNCU_TRY(elements_aligned({q, k, v, dout, dq, dk, dv}, s->dtype_bf16 ? 2 : 4));
     NNCU_TRY(elements_aligned({len, state_in, dstate_out, dstate_in}, 4));
-    NNCU_TRY(on_device({q, k, v, len, state_in, dout, dstate_out, dq, dk, dv, dstate_in, lin_need(s) ? workspace : nullptr}));
+    NNCU_TRY(on_device({q, k, v, len, state_in, dout, dstate_out, dq, dk, dv, dstate_in, lin_need(s, 3) ? workspace : nullptr}));
     const long long wk = (long long)s->n_head * s->d_key, wv = (long long)s->n_head * s->d_value;
     const long long lq = s->ld_q ? s->ld_q : wk, lk = s->ld_k ? s->ld_k : wk, lv = s->ld_v ? s->ld_v : wv, lo = s->ld_out ? s->ld_out : wv;
     ChainScope chain;
     cudaStream_t st = (cudaStream_t)cuda_stream;
-    const lin::Args base = lin_args(s, decay_host, len, workspace);
-    lin::Args a = base;
-    a.a = dout; a.lda = lo; a.b = v; a.ldb = lv; a.c = k; a.ldc = lk; a.o = dq; a.ldo = lq;
-    a.da = s->d_value; a.dc = s->d_key;
-    a.s0 = state_in; a.s0_t = 1;
-    a.e1 = 1;
-    a.s_state = a.s_pair = s->scale;
-    a.s_in = 1.0f;
-    NNCU_TRY(lin_any(s, a, st));
-    a = base;
-    a.reverse = 1;
-    a.e2 = 1;
-    a.s_state = 1.0f;
-    a.s_pair = a.s_in = s->scale;
-    a.s0 = dstate_out;
-    lin::Args d = a;
-    a.a = v; a.lda = lv; a.b = dout; a.ldb = lo; a.c = q; a.ldc = lq; a.o = dk; a.ldo = lk;
-    a.da = s->d_value; a.dc = s->d_key; a.s0_t = 1;
-    NNCU_TRY(lin_any(s, a, st));
-    // last: dstate_in may lie where dstate_out lies
-    d.a = k; d.lda = lk; d.b = q; d.ldb = lq; d.c = dout; d.ldc = lo; d.o = dv; d.ldo = lv;
-    d.da = s->d_key; d.dc = s->d_value; d.s_end = dstate_in;
-    return lin_any(s, d, st);
+    lin::Args all = lin_args(s, 3, decay_host, len, workspace);
+    lin::Role &rq = all.role[0], &rk = all.role[1], &rv = all.role[2];
+    rq.a = dout; rq.lda = lo; rq.b = v; rq.ldb = lv; rq.c = k; rq.ldc = lk; rq.o = dq; rq.ldo = lq;
+    rk.a = v; rk.lda = lv; rk.b = dout; rk.ldb = lo; rk.c = q; rk.ldc = lq; rk.o = dk; rk.ldo = lk;
+    rv.a = k; rv.lda = lk; rv.b = q; rv.ldb = lq; rv.c = dout; rv.ldc = lo; rv.o = dv; rv.ldo = lv;
+    rq.da = rk.da = s->d_value; rq.dc = rk.dc = s->d_key; rv.da = s->d_key; rv.dc = s->d_value;
+    rq.s0 = state_in; rk.s0 = rv.s0 = dstate_out;
+    rq.s0_t = rk.s0_t = 1;
+    rv.s_end = dstate_in;
+    rq.e1 = rk.e2 = rv.e2 = 1;
+    rk.reverse = rv.reverse = 1;
+    rq.s_state = rq.s_pair = rk.s_pair = rv.s_pair = rk.s_in = rv.s_in = s->scale;
+    rq.s_in = rk.s_state = rv.s_state = 1.0f;
+    // one launch for all three, or dv behind the others: where its head sizes are other than theirs, and where
+    // dstate_in lies over the dstate_out that they read
+    const float *from = dstate_out, *to = dstate_in;
+    const size_t states = (size_t)s->n_streams * wk * s->d_value;
+    if (s->d_key == s->d_value && !(from && to && from < to + states && to < from + states))
+        return lin_any(s, all, 3, st);
+    NNCU_TRY(lin_any(s, all, 2, st));
+    all.role[0] = rv;
+    return lin_any(s, all, 1, st);
 }
 
 } // extern "C"

@@ -20,6 +20,7 @@
 //
 // with e1 = 1, e2 = 0 in the sequence's order and e1 = 0, e2 = 1 in the reverse one.
 #pragma once
+#include "gemm_tc.cuh"
 #include "warp_mma.cuh"
 
 namespace lin {
@@ -27,19 +28,25 @@ namespace lin {
 constexpr int HEADS_MAX = NNCU_LINEAR_ATTN_HEADS_MAX;
 constexpr int DIM_MAX = NNCU_LINEAR_ATTN_DIM_MAX;
 
-struct Args {
+// one set of rows and its state
+struct Role {
     const void *a, *b, *c;
-    void *o;             // NULL: states only
+    void *o;
     const float *s0;     // state before the first token, [B][H][da][dc] or, where s0_t, [B][H][dc][da]; NULL: zeros
     float *s_end;        // state behind the last token, [B][H][da][dc]; NULL: not wanted
-    float *parts;        // [B*H][n_seg][da*dc]: slot 0 the state before the first token, slot g what part g - 1 adds up to
-    const int32_t *len;  // tokens of each stream; NULL: T
+    float *parts;        // [B*H][n_seg][slot]: slot 0 the state before the first token, slot g what part g - 1 adds up to
     long long lda, ldb, ldc, ldo; // elements from row to row
-    int B, H, T, da, dc;
-    int reverse, s0_t, e1, e2;
+    int da, dc, reverse, s0_t, e1, e2;
     float s_state, s_pair, s_in;
+};
+
+struct Args {
+    Role role[3];        // blockIdx.z says which
+    const int32_t *len;  // tokens of each stream; NULL: T
+    int B, H, T;
     int n_seg;           // parts a stream's tokens are cut into
     int seg;             // tokens in a part
+    int slot;            // floats of a state in parts
     float rate[HEADS_MAX]; // log2 of each head's decay
 };
 
@@ -50,42 +57,35 @@ __device__ __forceinline__ float power(float rate, int n) { return exp2f(rate * 
 struct Rows {
     long long first, step; // rows
     int n;
-    __device__ __forceinline__ Rows(const Args &p, int b)
+    __device__ __forceinline__ Rows(const Args &p, const Role &q, int b)
     {
         n = p.len ? min(max(p.len[b], 0), p.T) : p.T;
-        step = p.reverse ? -(long long)p.B : p.B;
-        first = (p.reverse ? (long long)(n - 1) * p.B : 0) + b;
+        step = q.reverse ? -(long long)p.B : p.B;
+        first = (q.reverse ? (long long)(n - 1) * p.B : 0) + b;
     }
     __device__ __forceinline__ long long row(int u) const { return first + step * u; }
 };
 
-// rows of the result behind a stream's end are zeros: those of them that part g is to write
+// rows of the result behind a stream's end are zeros: those of them that part g is to write, a warp a row
 template <typename T>
-__device__ __forceinline__ void zero_behind(const Args &p, const Rows &rows, int b, int h, int g, int tid, int nthr)
+__device__ __forceinline__ void zero_behind(const Args &p, const Role &q, const Rows &rows, int b, int h, int g, int warp, int warps, int lane)
 {
-    const int lo = max(rows.n, g * p.seg), hi = g == p.n_seg - 1 ? p.T : min(p.T, (g + 1) * p.seg);
-    T *o = reinterpret_cast<T *>(p.o) + (size_t)h * p.dc;
-    for (long long i = tid; i < (long long)(hi - lo) * p.dc; i += nthr)
-        o[((long long)(lo + i / p.dc) * p.B + b) * p.ldo + i % p.dc] = from_f<T>(0.0f);
+    const int hi = g == p.n_seg - 1 ? p.T : min(p.T, (g + 1) * p.seg);
+    for (int t = max(rows.n, g * p.seg) + warp; t < hi; t += warps) {
+        T *o = reinterpret_cast<T *>(q.o) + ((long long)t * p.B + b) * q.ldo + (size_t)h * q.dc;
+        for (int i = lane; i < q.dc; i += 32)
+            o[i] = from_f<T>(0.0f);
+    }
 }
 
-__device__ __forceinline__ float state_at(const Args &p, const float *s, int i, int c)
+__device__ __forceinline__ float state_at(const Role &q, const float *s, int i, int c)
 {
-    return p.s0_t ? s[(size_t)c * p.da + i] : s[(size_t)i * p.dc + c];
+    return q.s0_t ? s[(size_t)c * q.da + i] : s[(size_t)i * q.dc + c];
 }
 
-// Element (i, c) of the state that part g begins with, from the sums of the parts before it
-__device__ __forceinline__ float start_at(const Args &p, size_t pair, int g, int i, int c, float l_seg)
-{
-    const size_t nn = (size_t)p.da * p.dc;
-    if (p.n_seg == 1)
-        return p.s0 ? state_at(p, p.s0 + pair * nn, i, c) : 0.0f;
-    const float *at = p.parts + pair * p.n_seg * nn + (size_t)i * p.dc + c;
-    float s = at[0];
-    for (int k = 1; k <= g; k++)
-        s = fmaf(l_seg, s, at[k * nn]);
-    return s;
-}
+// Whether the last token of a stream of n is in part g: the state behind it is the stream's.  A stream without tokens
+// ends in part 0.
+__device__ __forceinline__ bool ends_in(const Args &p, int n, int g) { return g * p.seg < max(n, 1) && max(n, 1) <= g * p.seg + p.seg; }
 
 // ---------------- CUDA cores: fp32, and bf16 whose rows are not laid out in 16-byte pieces ----------------
 //
@@ -121,7 +121,8 @@ template <typename T, bool STATES>
 __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args p)
 {
     extern __shared__ __align__(16) float smf[];
-    const CoreSmem sm(p.da, p.dc);
+    const Role &q = p.role[blockIdx.z];
+    const CoreSmem sm(q.da, q.dc);
     float *As = smf, *Bs = smf + sm.b, *Cs = smf + sm.c, *Ss = smf + sm.s, *Ps = smf + sm.p, *pw = smf + sm.w, *wt = pw + FC + 2;
     const int tid = threadIdx.x;
     const size_t pair = blockIdx.x;
@@ -129,8 +130,8 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
     const float rate = p.rate[h];
     pdl_trigger();
     pdl_wait();
-    const Rows rows(p, b);
-    const size_t nn = (size_t)p.da * p.dc;
+    const Rows rows(p, q, b);
+    const size_t nn = (size_t)q.da * q.dc;
     const int begin = g * p.seg, end = min(rows.n, begin + p.seg);
     const float l_seg = power(rate, p.seg);
     for (int i = tid; i < FC + 2; i += 256)
@@ -138,26 +139,30 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
     for (int i = tid; i < sm.da4 * sm.dc4; i += 256) {
         const int x = i / sm.dc4, y = i % sm.dc4;
         float s = 0.0f;
-        if (x < p.da && y < p.dc) {
-            if (!STATES)
-                s = start_at(p, pair, g, x, y, l_seg);
-            else if (g == 0) { // the state before the first token is kept: s_end may lie where it lies
-                p.parts[pair * p.n_seg * nn + (size_t)x * p.dc + y] = p.s0 ? state_at(p, p.s0 + pair * nn, x, y) : 0.0f;
+        if (x < q.da && y < q.dc) {
+            float *part = q.parts + pair * p.n_seg * p.slot + (size_t)x * q.dc + y;
+            const float first = q.s0 && (p.n_seg == 1 || (STATES && g == 0)) ? state_at(q, q.s0 + pair * nn, x, y) : 0.0f;
+            if (STATES && g == 0) // the state before the first token is kept: s_end may lie where it lies
+                *part = first;
+            if (!STATES) {
+                s = p.n_seg == 1 ? first : part[0];
+                for (int k = 1; k <= g; k++)
+                    s = fmaf(l_seg, s, part[(size_t)k * p.slot]);
             }
         }
         Ss[x * sm.ld_c + y] = s;
     }
-    if (!STATES && p.o)
-        zero_behind<T>(p, rows, b, h, g, tid, 256);
+    if (!STATES)
+        zero_behind<T>(p, q, rows, b, h, g, tid >> 5, 8, tid & 31);
     for (int u0 = begin; u0 < end; u0 += FC) {
         const int n = min(FC, end - u0);
         __syncthreads();
         if (!STATES)
-            core_load<T>(As, sm.ld_a, sm.da4, p.da, p.a, p.lda, h, rows, u0, n);
-        core_load<T>(Bs, sm.ld_a, sm.da4, p.da, p.b, p.ldb, h, rows, u0, n);
-        core_load<T>(Cs, sm.ld_c, sm.dc4, p.dc, p.c, p.ldc, h, rows, u0, n);
+            core_load<T>(As, sm.ld_a, sm.da4, q.da, q.a, q.lda, h, rows, u0, n);
+        core_load<T>(Bs, sm.ld_a, sm.da4, q.da, q.b, q.ldb, h, rows, u0, n);
+        core_load<T>(Cs, sm.ld_c, sm.dc4, q.dc, q.c, q.ldc, h, rows, u0, n);
         for (int i = tid; i < FC; i += 256)
-            wt[i] = i < n ? p.s_in * pw[n - 1 - i + p.e2] : 0.0f;
+            wt[i] = i < n ? q.s_in * pw[n - 1 - i + q.e2] : 0.0f;
         __syncthreads();
         if (!STATES) {
             for (int k = 0; k < FC * FC / 256; k++) {
@@ -168,7 +173,7 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
                         const float4 u = *reinterpret_cast<const float4 *>(As + i * sm.ld_a + x), v = *reinterpret_cast<const float4 *>(Bs + j * sm.ld_a + x);
                         s = fmaf(u.x, v.x, fmaf(u.y, v.y, fmaf(u.z, v.z, fmaf(u.w, v.w, s))));
                     }
-                    s *= p.s_pair * pw[i - j];
+                    s *= q.s_pair * pw[i - j];
                 }
                 Ps[i * (FC + 1) + j] = s;
             }
@@ -176,7 +181,7 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
             for (int it = tid; it < FC / 4 * (sm.dc4 / 4); it += 256) {
                 const int i0 = it / (sm.dc4 / 4) * 4, c0 = it % (sm.dc4 / 4) * 4;
                 float acc[4][4] = {};
-                for (int x = 0; x < p.da; x++) {
+                for (int x = 0; x < q.da; x++) {
                     const float4 s = *reinterpret_cast<const float4 *>(Ss + x * sm.ld_c + c0);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
@@ -187,7 +192,7 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float f = p.s_state * pw[i0 + r + p.e1];
+                    const float f = q.s_state * pw[i0 + r + q.e1];
 #pragma unroll
                     for (int c = 0; c < 4; c++)
                         acc[r][c] *= f;
@@ -204,10 +209,10 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     if (i0 + r < n) {
-                        T *o = reinterpret_cast<T *>(p.o) + rows.row(u0 + i0 + r) * p.ldo + (size_t)h * p.dc + c0;
+                        T *o = reinterpret_cast<T *>(q.o) + rows.row(u0 + i0 + r) * q.ldo + (size_t)h * q.dc + c0;
 #pragma unroll
                         for (int c = 0; c < 4; c++)
-                            if (c0 + c < p.dc)
+                            if (c0 + c < q.dc)
                                 o[c] = from_f<T>(acc[r][c]);
                     }
             }
@@ -237,42 +242,65 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
         }
     }
     __syncthreads();
-    // behind the last token; a stream without tokens ends in part 0
-    float *to = STATES ? p.parts + (pair * p.n_seg + g + 1) * nn
-                       : (p.s_end && begin < max(rows.n, 1) && max(rows.n, 1) <= begin + p.seg ? p.s_end + pair * nn : nullptr);
+    float *to = STATES ? q.parts + (pair * p.n_seg + g + 1) * p.slot : (q.s_end && ends_in(p, rows.n, g) ? q.s_end + pair * nn : nullptr);
     if (to)
-        for (int i = tid; i < p.da * p.dc; i += 256)
-            to[i] = Ss[i / p.dc * sm.ld_c + i % p.dc];
+        for (int i = tid; i < q.da * q.dc; i += 256)
+            to[i] = Ss[i / q.dc * sm.ld_c + i % q.dc];
 }
 
 // ---------------- bf16 on warp-level tensor-core products ----------------
 //
-// A CTA of eight warps goes through one part of one (stream, head) in chunks of 64 tokens.  Warp (r, hc) takes rows
-// 16 r .. 16 r + 15 of a chunk and half hc of the columns of c; of the state it owns the same columns of rows 16 r .. (and
-// 16 (r + 4) .. of 128) in fp32 accumulators.  The results need all of the state: it goes through shared memory in bf16,
-// one rounding, as the pair weights P have one; products of a decayed b with c, which the state adds up, are kept to
-// 24 bits by three bf16 terms of the decayed value, so that the state is an fp32 sum of fp32 products.  The next chunk's
-// tiles are fetched under the present chunk, and one barrier a chunk hands over tiles and state.
+// A CTA of 4 CG warps goes through one part of one (stream, head) in chunks of 64 tokens.  Warp (r, cg) takes rows
+// 16 r .. 16 r + 15 of a chunk and 32 columns of c, the cg-th; of the state it owns the same columns of rows 16 r ..
+// (and 16 (r + 4) .. of 128) in fp32 accumulators.  The results need all of the state: it goes through shared memory in
+// bf16, one rounding, as the pair weights P have one; products of a decayed b with c, which the state adds up, are kept to
+// 24 bits by three bf16 terms of the decayed value, so that the state is an fp32 sum of fp32 products.
+//
+// Tiles come by TMA, 64 tokens x 64 (32) values of a head a copy, from a map of (value, head, stream, token): what lies beyond
+// a head's values or the sequence arrives as zeros.  One thread asks for the next chunk's under the present chunk (copies
+// of 16 bytes by all threads took 2000 of a chunk's 4600 cycles, 128 pairs of head size 64); one barrier a chunk hands over
+// tiles and state.  In the reverse order a chunk's row i is the tile's row 63 - i.
 
 constexpr int TC = 64; // tokens in a chunk
 
-template <int DA, int DC> struct MmaSmem {
-    static constexpr int LA = DA + 8, LC = DC + 8;            // pitches: rows four banks on
-    static constexpr int A = 0, B = A + 2 * TC * LA * 2, C = B + 2 * TC * LA * 2, S = C + 2 * TC * LC * 2,
-                         W = S + 2 * DA * LC * 2, BYTES = W + (2 * TC + 8) * 4;
+struct __align__(64) MmaArgs {
+    CUtensorMap map[3][3]; // of a, b, c of each role
+    Args p;
 };
 
-// 64 rows of a matrix as a tile, zeros behind row n and column d
-template <int D>
-__device__ __forceinline__ void tile_load(bf16 *dst, const bf16 *src, long long ldr, int d, const Rows &rows, int u0, int n)
+template <int DA, int DC> struct MmaSmem {
+    static constexpr int TA = TC * DA * 2, TB = TC * DC * 2, LC = DC + 8; // tiles; pitch of the state, rows four banks on
+    static constexpr int A = 0, B = A + 2 * TA, C = B + 2 * TA, S = C + 2 * TB, W = S + 2 * DA * LC * 2, BAR = W + (2 * TC + 8) * 4,
+                         BYTES = BAR + 16 + 1024; // the tiles begin at a multiple of 1024
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int h, int b, int t)
 {
-    constexpr int CPR = D / 8;
-    for (int i = threadIdx.x; i < TC * CPR; i += 256) {
-        const int r = i / CPR, x = i % CPR * 8;
-        const bool ok = r < n && x < d;
-        fa::cp16(dst + r * (D + 8) + x, ok ? src + rows.row(u0 + r) * ldr + x : src, ok);
-    }
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(h), "r"(b), "r"(t)
+                 : "memory");
 }
+__device__ __forceinline__ void ldsm4_at(uint32_t (&r)[4], uint32_t at)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void ldsm4t_at(uint32_t (&r)[4], uint32_t at)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at));
+}
+// Byte offset of 16-byte piece c of row r in a tile of D values a row: blocks of 64 columns, rows of 128 bytes, piece c at
+// c ^ (r % 8); with 32 columns rows of 64 bytes and piece c at c ^ (r / 2 % 4).  Flipping bits 1 and 2 of c flips bits 5
+// and 6 of the offset; 16 rows on, the pieces lie in the same order.
+template <int D> __device__ __forceinline__ uint32_t tile_at(int r, int c)
+{
+    if constexpr (D == 32)
+        return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+    else
+        return (uint32_t)((c >> 3) * (TC * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+template <int D> struct Rows16 { static constexpr int BYTES = D == 32 ? 16 * 64 : 16 * 128; };
 
 // a pair of bf16 values times their weights as three bf16 terms that add up to 24 bits of them
 __device__ __forceinline__ void split3(uint32_t v, float w0, float w1, uint32_t &hi, uint32_t &mid, uint32_t &lo)
@@ -285,104 +313,166 @@ __device__ __forceinline__ void split3(uint32_t v, float w0, float w1, uint32_t 
     lo = fa::pack2(x - __uint_as_float(mid << 16), y - __uint_as_float(mid & 0xffff0000u));
 }
 
-// TERMS: 3, or 2 where no state is a result (17 bits of a decayed value are more than the rounding behind them keeps)
-template <int DA, int DC, bool STATES, int TERMS>
-__global__ void __launch_bounds__(256) mma_kernel(const __grid_constant__ Args p)
+template <int DA, int DC, bool STATES>
+__global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kernel(const __grid_constant__ MmaArgs args)
 {
     using SM = MmaSmem<DA, DC>;
-    constexpr int LA = SM::LA, LC = SM::LC, NT = DC / 16, MT = DA > 64 ? DA / 64 : 1, KS = DA / 16;
-    extern __shared__ __align__(16) unsigned char smb[];
-    bf16 *As = reinterpret_cast<bf16 *>(smb + SM::A), *Bs = reinterpret_cast<bf16 *>(smb + SM::B),
-         *Cs = reinterpret_cast<bf16 *>(smb + SM::C), *Ss = reinterpret_cast<bf16 *>(smb + SM::S);
-    float *wts = reinterpret_cast<float *>(smb + SM::W), *pw16 = wts + 2 * TC; // weights of full and last chunks; l^16m
+    constexpr int LC = SM::LC, NT = 4, MT = DA > 64 ? DA / 64 : 1, KS = DA / 16, THR = 4 * DC;
+    extern __shared__ __align__(16) unsigned char smraw[];
+    __shared__ int abort_s, flag;
+    unsigned char *sm = smraw + ((1024u - (fa::smem_addr(smraw) & 1023u)) & 1023u);
+    const uint32_t base = fa::smem_addr(sm), bar = base + SM::BAR;
+    bf16 *Ss = reinterpret_cast<bf16 *>(sm + SM::S);
+    float *wts = reinterpret_cast<float *>(sm + SM::W), *pw16 = wts + 2 * TC; // weights of full and last chunks; l^16m
+    const Args &p = args.p;
+    const Role &q = p.role[blockIdx.z];
+    const CUtensorMap *maps = args.map[blockIdx.z];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
-    // the two warps of a scheduler take rows r and 3 - r: the triangle is dealt evenly
-    const int hc = warp >> 2, r = hc ? 3 - (warp & 3) : warp & 3;
+    // a scheduler's warps take rows r and 3 - r in turn: the triangle is dealt evenly
+    const int cg = warp >> 2, r = cg & 1 ? 3 - (warp & 3) : warp & 3;
     const size_t pair = blockIdx.x;
     const int g = blockIdx.y, b = (int)(pair / p.H), h = (int)(pair % p.H);
     const float rate = p.rate[h];
-    pdl_trigger();
-    pdl_wait();
-    const Rows rows(p, b);
-    const size_t nn = (size_t)p.da * p.dc;
+    if (tid == 0) {
+        abort_s = 0;
+        tc::mbar_init(bar, 1);
+        tc::mbar_init(bar + 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_wait(); // no early trigger: successors resident beside these CTAs cost more than their launch
+    const Rows rows(p, q, b);
+    const size_t nn = (size_t)q.da * q.dc;
     const int begin = g * p.seg, end = min(rows.n, begin + p.seg), total = max(end - begin, 0), chunks = (total + TC - 1) / TC;
-    const bf16 *ga = reinterpret_cast<const bf16 *>(p.a) + (size_t)h * p.da, *gb = reinterpret_cast<const bf16 *>(p.b) + (size_t)h * p.da,
-               *gc = reinterpret_cast<const bf16 *>(p.c) + (size_t)h * p.dc;
+    bool ok = true; // this thread's waits; behind one that ran out results are NaN and nothing more is asked for
     auto fetch = [&](int k) {
-        const int u0 = begin + k * TC, n = end - u0, buf = k & 1;
-        if (!STATES)
-            tile_load<DA>(As + buf * TC * LA, ga, p.lda, p.da, rows, u0, n);
-        tile_load<DA>(Bs + buf * TC * LA, gb, p.ldb, p.da, rows, u0, n);
-        tile_load<DC>(Cs + buf * TC * LC, gc, p.ldc, p.dc, rows, u0, n);
-        fa::cp_commit();
+        if (tid == 0 && ok) {
+            const int u0 = begin + k * TC, buf = k & 1, t0 = q.reverse ? rows.n - TC - u0 : u0;
+            const uint32_t full = bar + 8 * buf;
+            tc::mbar_expect_tx(full, (STATES ? 1 : 2) * SM::TA + SM::TB);
+#pragma unroll
+            for (int x = 0; x < DA; x += 64) {
+                if (!STATES)
+                    tma_load_4d(base + SM::A + buf * SM::TA + x * TC * 2, &maps[0], full, x, h, b, t0);
+                tma_load_4d(base + SM::B + buf * SM::TA + x * TC * 2, &maps[1], full, x, h, b, t0);
+            }
+#pragma unroll
+            for (int x = 0; x < DC; x += 64)
+                tma_load_4d(base + SM::C + buf * SM::TB + x * TC * 2, &maps[2], full, x, h, b, t0);
+        }
     };
     if (chunks)
         fetch(0);
-    const int n_last = total - (chunks - 1) * TC;
-    if (tid < TC)
-        wts[tid] = p.s_in * power(rate, TC - 1 - tid + p.e2);
-    else if (tid < 2 * TC)
-        wts[tid] = tid - TC < n_last ? p.s_in * power(rate, n_last - 1 - (tid - TC) + p.e2) : 0.0f;
-    else if (tid < 2 * TC + 4)
-        pw16[tid - 2 * TC] = power(rate, 16 * (tid - 2 * TC));
 
-    // the state: element c of s[m][n] is row 16 (r + 4 m) + gq + 8 (c >> 1), column hc * DC / 2 + 8 n + 2 t + (c & 1)
+    // the state: element c of s[m][n] is row 16 (r + 4 m) + gq + 8 (c >> 1), column 32 cg + 8 n + 2 t + (c & 1); in
+    // parts it lies as the threads hold it
     float s[MT][NT][4];
-    const float l_seg = power(rate, p.seg), l_full = power(rate, TC), l_last = power(rate, n_last);
     const bool has_state = r * 16 < DA; // of 32 rows the warps r = 2, 3 own none
+    const bool first = p.n_seg == 1 || (STATES && g == 0);
+    float4 *part = reinterpret_cast<float4 *>(q.parts + pair * p.n_seg * p.slot) + tid;
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int x = 16 * (r + 4 * m) + gq + 8 * (c >> 1), y = hc * (DC / 2) + 8 * n + 2 * t + (c & 1);
-                s[m][n][c] = 0.0f;
-                if (x < p.da && y < p.dc) {
-                    if (!STATES)
-                        s[m][n][c] = start_at(p, pair, g, x, y, l_seg);
-                    else if (g == 0) // the state before the first token is kept: s_end may lie where it lies
-                        p.parts[pair * p.n_seg * nn + (size_t)x * p.dc + y] = p.s0 ? state_at(p, p.s0 + pair * nn, x, y) : 0.0f;
+            for (int c = 0; c < 4; c += 2) {
+                const int x = 16 * (r + 4 * m) + gq + 4 * c, y = 32 * cg + 8 * n + 2 * t;
+                float2 f = make_float2(0.0f, 0.0f);
+                if (first && q.s0 && x < q.da && y < q.dc) {
+                    const float *from = q.s0 + pair * nn;
+                    f = q.s0_t ? make_float2(from[y * q.da + x], from[(y + 1) * q.da + x])
+                               : *reinterpret_cast<const float2 *>(from + x * q.dc + y);
                 }
+                s[m][n][c] = f.x;
+                s[m][n][c + 1] = f.y;
             }
+    const int n_last = total - (chunks - 1) * TC;
+    const float l_seg = power(rate, p.seg), l_full = power(rate, TC), l_last = power(rate, n_last);
+    if (tid < TC) {
+        wts[tid] = q.s_in * power(rate, TC - 1 - tid + q.e2);
+        wts[tid + TC] = tid < n_last ? q.s_in * power(rate, n_last - 1 - tid + q.e2) : 0.0f;
+    } else if (tid < TC + 4) {
+        pw16[tid - TC] = power(rate, 16 * (tid - TC));
+    }
+    // weights of pairs on the diagonal and 16 rows from it, of this thread's elements of two 8-key groups: row - key is
+    // d + 8 j with j = (c >> 1) - n from -1 to 1, less c & 1
+    float apart[3][2], diag[3][2], f_a = 0.0f, f_b = 0.0f;
+    if (!STATES) {
+        f_a = q.s_state * power(rate, 16 * r + gq + q.e1);
+        f_b = q.s_state * power(rate, 16 * r + gq + 8 + q.e1);
+#pragma unroll
+        for (int j = 0; j < 3; j++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int d = gq - 2 * t - c + 8 * (j - 1);
+                apart[j][c] = q.s_pair * power(rate, 16 + d);
+                diag[j][c] = q.s_pair * power(rate, max(d, 0));
+            }
+    }
+    // fragments of the tiles: this lane's rows of sixteen, in the chunk's order
+    auto row_of = [&](int i) { return q.reverse ? TC - 1 - i : i; };
+    const int step_a = (q.reverse ? -1 : 1) * Rows16<DA>::BYTES, step_c = (q.reverse ? -1 : 1) * Rows16<DC>::BYTES;
+    const int l15 = lane & 15, lrow = (lane & 7) + (lane >> 4) * 8, lhi = lane >> 4, lmid = (lane >> 3) & 1;
+    const uint32_t a_at = base + SM::A + tile_at<DA>(row_of(16 * r + l15), lhi);          // rows r of a, values 16 ks: ^ ks << 5
+    const uint32_t b_at = base + SM::B + tile_at<DA>(row_of(lrow), lmid);                  // rows 0 .. 15 of b, the same
+    const uint32_t bt_at = base + SM::B + tile_at<DA>(row_of(lrow), 2 * r % (DA / 8) + lmid); // transposed: values 16 r
+    const uint32_t c_at = base + SM::C + tile_at<DC>(row_of(l15), 4 * cg + lhi);           // transposed: rows 0 .. 15 of c
+    const uint32_t s_at = base + SM::S + (l15 * LC + 32 * cg + lhi * 8) * 2;
+    if (p.n_seg > 1) {
+        if (STATES) {
+            if (g == 0) // the state before the first token is kept: s_end may lie where it lies
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        part[(m * NT + n) * THR] = make_float4(s[m][n][0], s[m][n][1], s[m][n][2], s[m][n][3]);
+                        s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.0f;
+                    }
+        } else {
+#pragma unroll 1
+            for (int k = 0; k <= g; k++, part += p.slot / 4)
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const float4 f = part[(m * NT + n) * THR];
+                        s[m][n][0] = fmaf(l_seg, s[m][n][0], f.x); s[m][n][1] = fmaf(l_seg, s[m][n][1], f.y);
+                        s[m][n][2] = fmaf(l_seg, s[m][n][2], f.z); s[m][n][3] = fmaf(l_seg, s[m][n][3], f.w);
+                    }
+        }
+    }
     auto publish = [&](int buf) {
         if (!STATES && has_state)
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    bf16 *to = Ss + buf * DA * LC + (16 * (r + 4 * m) + gq) * LC + hc * (DC / 2) + 8 * n + 2 * t;
+                    bf16 *to = Ss + buf * DA * LC + (16 * (r + 4 * m) + gq) * LC + 32 * cg + 8 * n + 2 * t;
                     *reinterpret_cast<uint32_t *>(to) = fa::pack2(s[m][n][0], s[m][n][1]);
                     *reinterpret_cast<uint32_t *>(to + 8 * LC) = fa::pack2(s[m][n][2], s[m][n][3]);
                 }
     };
     publish(0);
-    if (!STATES && p.o)
-        zero_behind<bf16>(p, rows, b, h, g, tid, 256);
-
-    // weights of pairs 16 rows apart and on the diagonal, of this thread's elements of two 8-key groups
-    float apart[2][4], diag[2][4];
-    const float f_a = p.s_state * power(rate, 16 * r + gq + p.e1), f_b = p.s_state * power(rate, 16 * r + gq + 8 + p.e1);
-#pragma unroll
-    for (int n = 0; n < 2; n++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const int d = gq + 8 * (c >> 1) - 8 * n - 2 * t - (c & 1);
-            apart[n][c] = p.s_pair * power(rate, 16 + d);
-            diag[n][c] = d >= 0 ? p.s_pair * power(rate, d) : 0.0f;
-        }
+    if (!STATES)
+        zero_behind<bf16>(p, q, rows, b, h, g, warp, THR / 32, lane);
 
     for (int k = 0; k < chunks; k++) {
         const int buf = k & 1, u0 = begin + k * TC, n = min(TC, end - u0);
         const bool last = k == chunks - 1;
-        fa::cp_wait<0>();
+        ok = ok && tc::mbar_wait(bar + 8 * buf, (k >> 1) & 1, &abort_s, &flag, 81);
+        if (n < TC && p.len && !q.reverse) // rows behind the stream's end hold anything: the tile's are zeros
+            for (int i = tid; i < (TC - n) * (DA / 8 + DC / 8); i += THR) {
+                const int row = n + i / (DA / 8 + DC / 8), x = i % (DA / 8 + DC / 8);
+                unsigned char *to = sm + (x < DA / 8 ? SM::B + buf * SM::TA + tile_at<DA>(row, x) : SM::C + buf * SM::TB + tile_at<DC>(row, x - DA / 8));
+                *reinterpret_cast<uint4 *>(to) = make_uint4(0u, 0u, 0u, 0u);
+            }
         __syncthreads(); // this chunk's tiles and state stand; the other buffers are free
         if (!last)
             fetch(k + 1);
-        const bf16 *At = As + buf * TC * LA, *Bt = Bs + buf * TC * LA, *Ct = Cs + buf * TC * LC + hc * (DC / 2),
-                   *St = Ss + buf * DA * LC + hc * (DC / 2);
-        float o[NT][4];
+        const uint32_t At = a_at + buf * SM::TA, Bt = b_at + buf * SM::TA, Tt = bt_at + buf * SM::TA, Ct = c_at + buf * SM::TB,
+                       St = s_at + buf * DA * LC * 2;
         if (!STATES) {
+            float o[NT][4];
 #pragma unroll
             for (int x = 0; x < NT; x++)
 #pragma unroll
@@ -391,11 +481,11 @@ __global__ void __launch_bounds__(256) mma_kernel(const __grid_constant__ Args p
             uint32_t aq[KS][4];
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                fa::ldsm4(aq[ks], At + (16 * r + (lane & 15)) * LA + ks * 16 + (lane >> 4) * 8);
+                ldsm4_at(aq[ks], (At ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128));
 #pragma unroll
                 for (int x = 0; x < NT; x += 2) {
                     uint32_t f[4];
-                    fa::ldsm4t(f, St + (ks * 16 + (lane & 15)) * LC + x * 8 + (lane >> 4) * 8);
+                    ldsm4t_at(f, St + (ks * 16 * LC + x * 8) * 2);
                     fa::mma(o[x], aq[ks], f[0], f[1]);
                     fa::mma(o[x + 1], aq[ks], f[2], f[3]);
                 }
@@ -413,7 +503,7 @@ __global__ void __launch_bounds__(256) mma_kernel(const __grid_constant__ Args p
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     uint32_t f[4];
-                    fa::ldsm4(f, Bt + (pc * 16 + (lane & 7) + (lane >> 4) * 8) * LA + ks * 16 + ((lane >> 3) & 1) * 8);
+                    ldsm4_at(f, ((Bt ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128)) + pc * step_a);
                     fa::mma(w[0], aq[ks], f[0], f[1]);
                     fa::mma(w[1], aq[ks], f[2], f[3]);
                 }
@@ -422,40 +512,49 @@ __global__ void __launch_bounds__(256) mma_kernel(const __grid_constant__ Args p
                     for (int x = 0; x < 2; x++)
 #pragma unroll
                         for (int c = 0; c < 4; c++)
-                            w[x][c] = gq + 8 * (c >> 1) >= 8 * x + 2 * t + (c & 1) ? w[x][c] * diag[x][c] : 0.0f;
+                            w[x][c] = gq + 8 * (c >> 1) >= 8 * x + 2 * t + (c & 1) ? w[x][c] * diag[(c >> 1) - x + 1][c & 1] : 0.0f;
                 } else {
                     const float f = pw16[r - pc - 1];
 #pragma unroll
                     for (int x = 0; x < 2; x++)
 #pragma unroll
                         for (int c = 0; c < 4; c++)
-                            w[x][c] *= f * apart[x][c];
+                            w[x][c] *= f * apart[(c >> 1) - x + 1][c & 1];
                 }
                 const uint32_t pf[4] = {fa::pack2(w[0][0], w[0][1]), fa::pack2(w[0][2], w[0][3]), fa::pack2(w[1][0], w[1][1]),
                                         fa::pack2(w[1][2], w[1][3])};
 #pragma unroll
                 for (int x = 0; x < NT; x += 2) {
                     uint32_t f[4];
-                    fa::ldsm4t(f, Ct + (pc * 16 + (lane & 15)) * LC + x * 8 + (lane >> 4) * 8);
+                    ldsm4t_at(f, (Ct ^ (x << 4)) + pc * step_c);
                     fa::mma(o[x], pf, f[0], f[1]);
                     fa::mma(o[x + 1], pf, f[2], f[3]);
                 }
             }
-            // rows out: a lane's column pairs
+            if (!ok)
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+                    o[x][0] = o[x][1] = o[x][2] = o[x][3] = NAN;
+            // rows out: a quad's 32 columns in four pieces of 16 bytes
 #pragma unroll
             for (int c = 0; c < 4; c += 2) {
                 const int i = 16 * r + gq + 4 * c;
-                bf16 *to = reinterpret_cast<bf16 *>(p.o) + (i < n ? rows.row(u0 + i) * p.ldo : 0) + (size_t)h * p.dc + hc * (DC / 2) + 2 * t;
+                bf16 *to = reinterpret_cast<bf16 *>(q.o) + (i < n ? rows.row(u0 + i) * q.ldo : 0) + (size_t)h * q.dc + 32 * cg;
+                uint32_t v[4];
 #pragma unroll
                 for (int x = 0; x < NT; x++)
-                    if (i < n && hc * (DC / 2) + 8 * x < p.dc)
-                        *reinterpret_cast<uint32_t *>(to + 8 * x) = fa::pack2(o[x][c], o[x][c + 1]);
+                    v[x] = fa::pack2(o[x][c], o[x][c + 1]);
+                fa::quad_transpose(v, t);
+                if (i < n && 32 * cg + 8 * t < q.dc)
+                    *reinterpret_cast<uint4 *>(to + 8 * t) = make_uint4(v[0], v[1], v[2], v[3]);
             }
         }
-        if (last && !STATES && !p.s_end)
+        if (last && !STATES && !q.s_end)
             break;
         // the state behind the chunk
         const float l_n = last ? l_last : l_full, *wt = wts + (last ? TC : 0);
+        // the third term where a state is a result; 17 bits are more than the roundings behind them keep
+        const bool third = q.s_end != nullptr;
         if (has_state) {
 #pragma unroll
             for (int m = 0; m < MT; m++)
@@ -471,7 +570,7 @@ __global__ void __launch_bounds__(256) mma_kernel(const __grid_constant__ Args p
 #pragma unroll
                 for (int m = 0; m < MT; m++) {
                     uint32_t f[4];
-                    fa::ldsm4t(f, Bt + (ks * 16 + (lane & 7) + (lane >> 4) * 8) * LA + 16 * (r + 4 * m) + ((lane >> 3) & 1) * 8);
+                    ldsm4t_at(f, Tt + m * (TC * 128) + ks * step_a);
 #pragma unroll
                     for (int e = 0; e < 4; e++)
                         split3(f[e], e < 2 ? w0.x : w8.x, e < 2 ? w0.y : w8.y, hi[m][e], mid[m][e], lo[m][e]);
@@ -479,14 +578,14 @@ __global__ void __launch_bounds__(256) mma_kernel(const __grid_constant__ Args p
 #pragma unroll
                 for (int x = 0; x < NT; x += 2) {
                     uint32_t f[4];
-                    fa::ldsm4t(f, Ct + (ks * 16 + (lane & 15)) * LC + x * 8 + (lane >> 4) * 8);
+                    ldsm4t_at(f, (Ct ^ (x << 4)) + ks * step_c);
 #pragma unroll
                     for (int m = 0; m < MT; m++) {
                         fa::mma(s[m][x], hi[m], f[0], f[1]);
                         fa::mma(s[m][x + 1], hi[m], f[2], f[3]);
                         fa::mma(s[m][x], mid[m], f[0], f[1]);
                         fa::mma(s[m][x + 1], mid[m], f[2], f[3]);
-                        if (TERMS > 2) {
+                        if (third) {
                             fa::mma(s[m][x], lo[m], f[0], f[1]);
                             fa::mma(s[m][x + 1], lo[m], f[2], f[3]);
                         }
@@ -497,21 +596,36 @@ __global__ void __launch_bounds__(256) mma_kernel(const __grid_constant__ Args p
         if (!last)
             publish(buf ^ 1);
     }
-    float *to = STATES ? p.parts + (pair * p.n_seg + g + 1) * nn
-                       : (p.s_end && begin < max(rows.n, 1) && max(rows.n, 1) <= begin + p.seg ? p.s_end + pair * nn : nullptr);
-    if (to && has_state)
+    if (!ok) {
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+                s[m][x][0] = s[m][x][1] = s[m][x][2] = s[m][x][3] = NAN;
+        for (int x = 0; x < 2; x++) // copies in flight may land before the CTA leaves
+            tc::mbar_wait(bar + 8 * x, 0, &abort_s, &flag, 81, tc::DRAIN_TRIES);
+    }
+    if (STATES) {
+        part += (size_t)(g + 1) * (p.slot / 4);
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+                part[(m * NT + x) * THR] = make_float4(s[m][x][0], s[m][x][1], s[m][x][2], s[m][x][3]);
+    } else if (q.s_end && has_state && ends_in(p, rows.n, g)) {
+        float *to = q.s_end + pair * nn;
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
             for (int x = 0; x < NT; x++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const int i = 16 * (r + 4 * m) + gq + 8 * (c >> 1), y = hc * (DC / 2) + 8 * x + 2 * t + (c & 1);
-                    if (i < p.da && y < p.dc)
-                        to[(size_t)i * p.dc + y] = s[m][x][c];
+                for (int c = 0; c < 4; c += 2) {
+                    const int i = 16 * (r + 4 * m) + gq + 4 * c, y = 32 * cg + 8 * x + 2 * t;
+                    if (i < q.da && y < q.dc)
+                        *reinterpret_cast<float2 *>(to + i * q.dc + y) = make_float2(s[m][x][c], s[m][x][c + 1]);
                 }
+    }
 }
-
 
 // ---------------- a few tokens: the recurrence itself ----------------
 //
@@ -526,14 +640,15 @@ __global__ void __launch_bounds__(128) step_kernel(const __grid_constant__ Args 
 {
     constexpr int COLS = 8 * VEC, MOST = DIM_MAX / 16;
     __shared__ float As[STEP_TOKENS][DIM_MAX], Bs[STEP_TOKENS][DIM_MAX], Cs[STEP_TOKENS][COLS], red[STEP_TOKENS][4][COLS];
+    const Role &q = p.role[blockIdx.z];
     const int tid = threadIdx.x, cg = tid & 7, rl = tid >> 3;
     const size_t pair = blockIdx.x;
     const int b = (int)(pair / p.H), h = (int)(pair % p.H), c0 = blockIdx.y * COLS;
     const float l = exp2f(p.rate[h]);
     pdl_trigger();
     pdl_wait();
-    const Rows rows(p, b);
-    const size_t nn = (size_t)p.da * p.dc;
+    const Rows rows(p, q, b);
+    const size_t nn = (size_t)q.da * q.dc;
     float s[MOST][VEC];
 #pragma unroll
     for (int k = 0; k < MOST; k++) {
@@ -541,31 +656,31 @@ __global__ void __launch_bounds__(128) step_kernel(const __grid_constant__ Args 
 #pragma unroll
         for (int v = 0; v < VEC; v++)
             s[k][v] = 0.0f;
-        if (p.s0 && x < p.da && c < p.dc) {
-            const float *s0 = p.s0 + pair * nn;
-            if (VEC == 4 && !p.s0_t) {
-                const float4 f = *reinterpret_cast<const float4 *>(s0 + (size_t)x * p.dc + c);
+        if (q.s0 && x < q.da && c < q.dc) {
+            const float *s0 = q.s0 + pair * nn;
+            if (VEC == 4 && !q.s0_t) {
+                const float4 f = *reinterpret_cast<const float4 *>(s0 + (size_t)x * q.dc + c);
                 s[k][0] = f.x; s[k][1 % VEC] = f.y; s[k][2 % VEC] = f.z; s[k][3 % VEC] = f.w;
             } else {
 #pragma unroll
                 for (int v = 0; v < VEC; v++)
-                    s[k][v] = state_at(p, s0, x, c + v);
+                    s[k][v] = state_at(q, s0, x, c + v);
             }
         }
     }
-    const T *a = reinterpret_cast<const T *>(p.a) + (size_t)h * p.da, *bb = reinterpret_cast<const T *>(p.b) + (size_t)h * p.da,
-            *cc = reinterpret_cast<const T *>(p.c) + (size_t)h * p.dc;
+    const T *a = reinterpret_cast<const T *>(q.a) + (size_t)h * q.da, *bb = reinterpret_cast<const T *>(q.b) + (size_t)h * q.da,
+            *cc = reinterpret_cast<const T *>(q.c) + (size_t)h * q.dc;
     for (int u = 0; u < rows.n; u++) {
         const long long row = rows.row(u);
-        if (tid < p.da) {
-            As[u][tid] = to_f(a[row * p.lda + tid]);
-            Bs[u][tid] = p.s_in * to_f(bb[row * p.ldb + tid]);
+        if (tid < q.da) {
+            As[u][tid] = to_f(a[row * q.lda + tid]);
+            Bs[u][tid] = q.s_in * to_f(bb[row * q.ldb + tid]);
         }
         if (tid < COLS)
-            Cs[u][tid] = c0 + tid < p.dc ? to_f(cc[row * p.ldc + c0 + tid]) : 0.0f;
+            Cs[u][tid] = c0 + tid < q.dc ? to_f(cc[row * q.ldc + c0 + tid]) : 0.0f;
     }
     __syncthreads();
-    const float before = p.e1 ? l : 1.0f, behind = p.e2 ? l : 1.0f, s_out = p.s_state;
+    const float before = q.e1 ? l : 1.0f, behind = q.e2 ? l : 1.0f, s_out = q.s_state;
     for (int u = 0; u < rows.n; u++) {
         float acc[VEC], cv[VEC];
 #pragma unroll
@@ -576,7 +691,7 @@ __global__ void __launch_bounds__(128) step_kernel(const __grid_constant__ Args 
 #pragma unroll
         for (int k = 0; k < MOST; k++) {
             const int x = rl + 16 * k;
-            if (x < p.da) {
+            if (x < q.da) {
                 const float av = As[u][x], bv = Bs[u][x];
 #pragma unroll
                 for (int v = 0; v < VEC; v++) {
@@ -594,12 +709,12 @@ __global__ void __launch_bounds__(128) step_kernel(const __grid_constant__ Args 
                 red[u][tid >> 5][cg * VEC + v] = acc[v];
         }
     }
-    if (p.s_end) {
+    if (q.s_end) {
 #pragma unroll
         for (int k = 0; k < MOST; k++) {
             const int x = rl + 16 * k, c = c0 + cg * VEC;
-            if (x < p.da && c < p.dc) {
-                float *to = p.s_end + pair * nn + (size_t)x * p.dc + c;
+            if (x < q.da && c < q.dc) {
+                float *to = q.s_end + pair * nn + (size_t)x * q.dc + c;
                 if (VEC == 4)
                     *reinterpret_cast<float4 *>(to) = make_float4(s[k][0], s[k][1 % VEC], s[k][2 % VEC], s[k][3 % VEC]);
                 else
@@ -608,16 +723,16 @@ __global__ void __launch_bounds__(128) step_kernel(const __grid_constant__ Args 
         }
     }
     __syncthreads();
-    if (p.o) {
-        T *o = reinterpret_cast<T *>(p.o) + (size_t)h * p.dc;
+    {
+        T *o = reinterpret_cast<T *>(q.o) + (size_t)h * q.dc;
         for (int i = tid; i < p.T * COLS; i += 128) {
             const int u = i / COLS, x = i % COLS;
-            if (c0 + x >= p.dc)
+            if (c0 + x >= q.dc)
                 continue;
             if (u < rows.n)
-                o[rows.row(u) * p.ldo + c0 + x] = from_f<T>(s_out * (red[u][0][x] + red[u][1][x] + red[u][2][x] + red[u][3][x]));
+                o[rows.row(u) * q.ldo + c0 + x] = from_f<T>(s_out * (red[u][0][x] + red[u][1][x] + red[u][2][x] + red[u][3][x]));
             else // behind the stream's end
-                o[((long long)u * p.B + b) * p.ldo + c0 + x] = from_f<T>(0.0f);
+                o[((long long)u * p.B + b) * q.ldo + c0 + x] = from_f<T>(0.0f);
         }
     }
 }
