@@ -417,10 +417,11 @@ int nncu_attention_backward_noalloc(const nncu_attn_shape *s, const void *q, con
  *   q [n_rows][n_head*d_key], k [n_rows][n_head_k*d_key] (n_head_k 0: none), gain_q, gain_k [d_key] (NULL: ones),
  *   pos int32 [n_rows] (may be NULL when d_rot is 0).  A row with pos < 0 is padding: its values are
  *   not looked at, its results and gradients are zeros.
- * d_key even, up to NNCU_QK_NORM_DIM_MAX (NNCU_ERR_RANGE beyond); d_rot even, up to d_key.  q_out may be q and
- * k_out k (same pitch).
+ * d_key even, up to NNCU_QK_NORM_DIM_MAX, up to NNCU_QK_NORM_HEADS_MAX heads (NNCU_ERR_RANGE beyond); d_rot even,
+ * up to d_key.  q_out may be q and k_out k (same pitch).
  */
 #define NNCU_QK_NORM_DIM_MAX 256
+#define NNCU_QK_NORM_HEADS_MAX 1024
 typedef struct nncu_qk_norm_shape {
     int32_t n_rows, n_head, n_head_k, d_key, d_rot;
     int32_t ld_q, ld_k, ld_q_out, ld_k_out;

@@ -7,7 +7,8 @@ FF_RELU, FF_GELU, FF_GEGLU, FF_GATED_SILU = 0, 1, 2, 3
 INIT_UNIFORM, INIT_NORMAL = 0, 1
 GEMM_AUTO, GEMM_SIMT, GEMM_TCGEN05 = 0, 1, 2
 NOALLOC_SCRATCH_FLOATS = 4 << 20
-QK_NORM_DIM_MAX, LINEAR_ATTN_HEADS_MAX, LINEAR_ATTN_DIM_MAX, DISTILL_TOP_MAX = 256, 64, 128, 1024
+QK_NORM_DIM_MAX, QK_NORM_HEADS_MAX, DISTILL_TOP_MAX = 256, 1024, 1024
+LINEAR_ATTN_DIM_MAX, LINEAR_ATTN_HEADS_MAX = 128, 64
 OK, ERR_INVALID, ERR_CUDA, ERR_NOMEM, ERR_STATE, ERR_TIMEOUT, ERR_RANGE = range(7)
 
 

@@ -19,36 +19,48 @@ static int distill_check(const nncu_distill_shape *s)
     return NNCU_OK;
 }
 
-template <typename TZ, typename TG, int WHAT, int THR, int VEC, int PER> static int distill_launch(const distill::Args &a, cudaStream_t st)
+template <typename TZ, typename TG, int WHAT, int THR, int PER, bool TWO> static int distill_launch(const distill::Args &a, cudaStream_t st)
 {
-    CUDA_TRY(launch_k(distill::kernel<TZ, TG, WHAT, THR, VEC, PER>, dim3(a.N), dim3(THR), sizeof(float) * 2 * (size_t)a.K, st, a));
+    CUDA_TRY(launch_k(distill::kernel<TZ, TG, WHAT, THR, PER, TWO>, dim3(a.N), dim3(THR), sizeof(float) * 3 * (size_t)a.K4, st, a));
     KERNEL_CHECK();
     return NNCU_OK;
 }
 
-// Short rows take a CTA of four warps, long ones of sixteen; a thread holds 32 logits at most.
-template <typename TZ, typename TG, int WHAT, int VEC> static int distill_sized(const distill::Args &a, cudaStream_t st)
+// Rows of up to 1024 logits take a CTA of four warps, up to 4096 one of eight, longer ones sixteen; a thread holds 32
+// logits at most.  The gradient from sums that stand needs a logit only once.
+template <typename TZ, typename TG, int WHAT, bool TWO> static int distill_sized(const distill::Args &a, cudaStream_t st)
 {
-    const int groups = ceil_div(a.V, VEC), most = 32 / VEC;
-    if (groups <= 128 * most) {
-        const int per = ceil_div(groups, 128);
-        if (per <= most / 4)
-            return distill_launch<TZ, TG, WHAT, 128, VEC, most / 4>(a, st);
-        return per <= most / 2 ? distill_launch<TZ, TG, WHAT, 128, VEC, most / 2>(a, st) : distill_launch<TZ, TG, WHAT, 128, VEC, most>(a, st);
+    const bool begins = a.ldz % 4 == 0 && aligned(a.z, 4 * sizeof(TZ)); // every row with a group
+    const int groups = begins ? ceil_div(a.V, 4) : (a.V + 6) / 4;
+    if constexpr (WHAT == distill::GRAD) {
+        return groups <= 512 ? distill_launch<TZ, TG, WHAT, 128, 0, TWO>(a, st) : distill_launch<TZ, TG, WHAT, 256, 0, TWO>(a, st);
+    } else {
+        if (groups <= 128)
+            return distill_launch<TZ, TG, WHAT, 128, 1, TWO>(a, st);
+        if (groups <= 256)
+            return distill_launch<TZ, TG, WHAT, 128, 2, TWO>(a, st);
+        if (groups <= 512)
+            return distill_launch<TZ, TG, WHAT, 256, 2, TWO>(a, st);
+        if (groups <= 1024)
+            return distill_launch<TZ, TG, WHAT, 256, 4, TWO>(a, st);
+        switch (ceil_div(groups, 512)) {
+        case 3: return distill_launch<TZ, TG, WHAT, 512, 3, TWO>(a, st);
+        case 4: return distill_launch<TZ, TG, WHAT, 512, 4, TWO>(a, st);
+        case 5: return distill_launch<TZ, TG, WHAT, 512, 5, TWO>(a, st);
+        case 6: return distill_launch<TZ, TG, WHAT, 512, 6, TWO>(a, st);
+        case 7: return distill_launch<TZ, TG, WHAT, 512, 7, TWO>(a, st);
+        case 8: return distill_launch<TZ, TG, WHAT, 512, 8, TWO>(a, st);
+        default: return distill_launch<TZ, TG, WHAT, 512, 0, TWO>(a, st);
+        }
     }
-    if (groups <= 512 * most) {
-        const int per = ceil_div(groups, 512);
-        if (per <= most / 2)
-            return distill_launch<TZ, TG, WHAT, 512, VEC, most / 2>(a, st);
-        return distill_launch<TZ, TG, WHAT, 512, VEC, most>(a, st);
-    }
-    return distill_launch<TZ, TG, WHAT, 512, VEC, 0>(a, st);
 }
 
 template <typename TZ, typename TG, int WHAT> static int distill_run(const distill::Args &a, cudaStream_t st)
 {
-    const bool wide = a.ldz % 4 == 0 && aligned(a.z, 4 * sizeof(TZ)) && (!(WHAT & distill::GRAD) || (a.lddz % 4 == 0 && aligned(a.dz, 4 * sizeof(TG))));
-    return wide ? distill_sized<TZ, TG, WHAT, 4>(a, st) : distill_sized<TZ, TG, WHAT, 1>(a, st);
+    if constexpr (WHAT != distill::GRAD)
+        if (!a.power)
+            return distill_sized<TZ, TG, WHAT, true>(a, st);
+    return distill_sized<TZ, TG, WHAT, false>(a, st);
 }
 
 template <int WHAT>
@@ -72,7 +84,11 @@ static int distill_any(const nncu_distill_shape *s, const void *logits, const in
     a.ldz = s->ld_logits ? s->ld_logits : s->n_symbols;
     a.lddz = s->ld_dlogits ? s->ld_dlogits : s->n_symbols;
     a.N = s->n_rows; a.V = s->n_symbols; a.K = s->n_top;
-    a.share = s->teacher_share; a.tau = s->temperature; a.inv_tau = 1.0f / s->temperature;
+    a.K4 = (s->n_top + 3) & ~3;
+    a.share = s->teacher_share;
+    a.tau = a.share == 0.0f ? 1.0f : s->temperature; // of a term that is not there
+    a.inv_tau = 1.0f / a.tau;
+    a.power = a.share == 1.0f ? 1 : a.tau <= 4.0f && a.tau == floorf(a.tau) ? (int)a.tau : 0; // of p too
     ChainScope chain;
     cudaStream_t st = (cudaStream_t)cuda_stream;
     if (!(WHAT & distill::GRAD))

@@ -13,28 +13,28 @@ static int qk_check(const nncu_qk_norm_shape *s)
     if (!s || s->n_rows < 1 || s->n_head < 1 || s->n_head_k < 0 || s->d_key < 2 || (s->d_key & 1) || s->d_rot < 0 ||
         (s->d_rot & 1) || s->d_rot > s->d_key || !(s->eps >= 0.0f) || !isfinite(s->eps) || (s->d_rot && !(s->rope_base > 0.0f && isfinite(s->rope_base))))
         return nncu_fail(NNCU_ERR_INVALID, "qk norm: bad shape");
-    if (s->d_key > NNCU_QK_NORM_DIM_MAX)
-        return nncu_fail(NNCU_ERR_RANGE, "qk norm: d_key %d is more than %d", s->d_key, NNCU_QK_NORM_DIM_MAX);
+    if (s->d_key > NNCU_QK_NORM_DIM_MAX || s->n_head > NNCU_QK_NORM_HEADS_MAX || s->n_head_k > NNCU_QK_NORM_HEADS_MAX)
+        return nncu_fail(NNCU_ERR_RANGE, "qk norm: d_key over %d or more than %d heads", NNCU_QK_NORM_DIM_MAX, NNCU_QK_NORM_HEADS_MAX);
     const long long wq = (long long)s->n_head * s->d_key, wk = (long long)s->n_head_k * s->d_key;
     if ((s->ld_q && s->ld_q < wq) || (s->ld_q_out && s->ld_q_out < wq) || (s->ld_k && s->ld_k < wk) || (s->ld_k_out && s->ld_k_out < wk))
         return nncu_fail(NNCU_ERR_INVALID, "qk norm: a row pitch is less than the row");
-    if (wq > INT_MAX / 64 || wk > INT_MAX / 64)
-        return nncu_fail(NNCU_ERR_RANGE, "qk norm: rows too wide");
     return NNCU_OK;
 }
 
-// rows that a CTA takes at a time: enough for its warps, few enough for a CTA on every SM
+// Rows that a CTA takes at a time: heads for its eight warps at least (a lane holds eight pairs or so), and eight where
+// that leaves two CTAs an SM.
 static int qk_rows_per(const nncu_qk_norm_shape *s)
 {
-    int n = 8;
-    while (n > 1 && ceil_div(s->n_rows, n) < 2 * SMS)
-        n /= 2;
+    const int heads = s->n_head + s->n_head_k, per_warp = std::max(1, 32 * 16 / s->d_key);
+    int n = 1;
+    while (n < 8 && (n * heads < 8 * per_warp || ceil_div(s->n_rows, 2 * n) >= 2 * SMS))
+        n *= 2;
     return n;
 }
 static int qk_blocks(const nncu_qk_norm_shape *s, bool back)
 {
     const int blocks = ceil_div(s->n_rows, qk_rows_per(s));
-    return back ? std::min(blocks, 4 * SMS) : blocks;
+    return back ? std::min(blocks, 2 * SMS) : blocks; // each leaves a partial sum of dgain
 }
 
 static qkn::Args qk_args(const nncu_qk_norm_shape *s, const void *q, const void *k, const float *gain_q, const float *gain_k, const int32_t *pos)
@@ -50,6 +50,8 @@ static qkn::Args qk_args(const nncu_qk_norm_shape *s, const void *q, const void 
     a.heads[0] = s->n_head; a.heads[1] = s->n_head_k;
     a.N = s->n_rows; a.d = s->d_key; a.rot = s->d_rot; a.adjacent = s->adjacent != 0; a.eps = s->eps;
     a.rows_per = qk_rows_per(s);
+    for (int i = 0; i < 2; i++)
+        a.inverse[i] = a.heads[i] > 1 ? (uint32_t)(((1ull << 32) + a.heads[i] - 1) / a.heads[i]) : 0;
     for (int i = 0; i < s->d_rot / 2; i++)
         a.turns[i] = pow((double)s->rope_base, -2.0 * i / s->d_rot) / 6.283185307179586476925;
     return a;
@@ -60,7 +62,7 @@ template <typename T, int W, int NG, bool BACK> static int qk_launch(const nncu_
     a.lanes = 1;
     while (a.lanes * W * NG < a.d / 2)
         a.lanes *= 2;
-    const size_t smem = sizeof(float) * ((size_t)a.rows_per * a.rot + (BACK ? 8 * a.d : 0));
+    const size_t smem = sizeof(float) * ((size_t)a.rows_per * a.rot + (BACK ? 10 : 2) * a.d);
     CUDA_TRY(launch_k(qkn::kernel<T, W, NG, BACK>, dim3(qk_blocks(s, BACK)), dim3(256), smem, st, a));
     KERNEL_CHECK();
     return NNCU_OK;
@@ -141,7 +143,7 @@ int nncu_qk_norm_rope_backward(const nncu_qk_norm_shape *s, const void *q, const
     cudaStream_t st = (cudaStream_t)cuda_stream;
     NNCU_TRY((s->dtype_bf16 ? qk_any<bf16, true>(s, a, st) : qk_any<float, true>(s, a, st)));
     if (gains) {
-        CUDA_TRY(launch_k(qkn::gain_kernel, dim3(ceil_div(2 * s->d_key, 32)), dim3(256), 0, st, (const float *)a.part, qk_blocks(s, true), s->d_key,
+        CUDA_TRY(launch_k(qkn::gain_kernel, dim3(ceil_div(2 * s->d_key, 8)), dim3(256), 0, st, (const float *)a.part, qk_blocks(s, true), s->d_key,
                           dgain_q, dgain_k));
         KERNEL_CHECK();
     }

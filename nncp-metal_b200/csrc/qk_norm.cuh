@@ -25,48 +25,35 @@ struct Args {
     float *part;         // [grid][2][d] partial sums of dgain
     long long ldx[2], ldy[2];
     int heads[2];
+    uint32_t inverse[2]; // ceil(2^32 / heads); 0 for one head
     int N, d, rot, adjacent, lanes, rows_per; // lanes: of a head (a power of two)
     float eps;
     double turns[DIM_MAX / 2]; // of pair i from one position to the next
 };
 
-template <typename T, int W> __device__ __forceinline__ void take(float (&v)[W], const T *p)
+// W values as they lie in memory
+template <int BYTES> struct Raw;
+template <> struct Raw<16> { typedef uint4 type; };
+template <> struct Raw<8> { typedef uint2 type; };
+template <> struct Raw<4> { typedef uint32_t type; };
+template <> struct Raw<2> { typedef uint16_t type; };
+template <typename T, int W> using raw_t = typename Raw<sizeof(T) * W>::type;
+
+template <typename T, int W> __device__ __forceinline__ void take(float (&v)[W], const raw_t<T, W> &u)
 {
+    const T *p = reinterpret_cast<const T *>(&u);
 #pragma unroll
     for (int i = 0; i < W; i++)
         v[i] = to_f(p[i]);
 }
-template <typename T, int W> __device__ __forceinline__ void load(float (&v)[W], const T *p)
+template <typename T, int W> __device__ __forceinline__ raw_t<T, W> put(const float (&v)[W])
 {
-    if constexpr (sizeof(T) * W == 16) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
-        take<T, W>(v, reinterpret_cast<const T *>(&u));
-    } else if constexpr (sizeof(T) * W == 8) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(p);
-        take<T, W>(v, reinterpret_cast<const T *>(&u));
-    } else if constexpr (sizeof(T) * W == 4) {
-        const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
-        take<T, W>(v, reinterpret_cast<const T *>(&u));
-    } else {
-        take<T, W>(v, p);
-    }
-}
-template <typename T, int W> __device__ __forceinline__ void store(T *p, const float (&v)[W])
-{
-    struct __align__(16) { T t[W]; } o;
+    raw_t<T, W> u;
+    T *p = reinterpret_cast<T *>(&u);
 #pragma unroll
     for (int i = 0; i < W; i++)
-        o.t[i] = from_f<T>(v[i]);
-    if constexpr (sizeof(T) * W == 16)
-        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(&o);
-    else if constexpr (sizeof(T) * W == 8)
-        *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(&o);
-    else if constexpr (sizeof(T) * W == 4)
-        *reinterpret_cast<uint32_t *>(p) = *reinterpret_cast<const uint32_t *>(&o);
-    else
-#pragma unroll
-        for (int i = 0; i < W; i++)
-            p[i] = o.t[i];
+        p[i] = from_f<T>(v[i]);
+    return u;
 }
 
 // Where a lane's pairs p0 .. p0 + W - 1 lie in a head's row: two runs of W values.  Pairs behind the rotated ones are
@@ -107,26 +94,31 @@ template <int W> __device__ __forceinline__ void turn(float (&x)[2][W], const fl
     }
 }
 
-// cosines and sines of rows r0 .. r0 + n - 1: [n][rot / 2]
-__device__ __forceinline__ void angles(const Args &a, float2 *cs, int r0, int n, int tid, int nthr)
+// Cosines and sines of rows r0 .. r0 + n - 1, [n][rot / 2], and which of them are no padding
+__device__ __forceinline__ void angles(const Args &a, float2 *cs, int *live, int r0, int n, int tid)
 {
     const int half = a.rot / 2;
-    for (int i = tid; i < n * half; i += nthr) {
+    for (int i = tid; i < n * half; i += 256) {
         const double t = (double)a.pos[r0 + i / half] * a.turns[i % half];
         float s, c;
         sincospif((float)(2.0 * (t - rint(t))), &s, &c);
         cs[i] = make_float2(c, s);
     }
+    if (tid < n)
+        live[tid] = !a.pos || a.pos[r0 + tid] >= 0;
 }
 
-// A lane has NG groups of W pairs, a group's neighbours in the neighbouring lanes
+// A warp takes 32 / lanes heads of neighbouring places at a time, queries of the CTA's rows and then keys; the
+// next ones are on their way while it computes, the first while the angles are taken.  A lane has NG groups of W pairs,
+// a group's neighbours in the neighbouring lanes.
 template <typename T, int W, int NG, bool BACK>
-__global__ void __launch_bounds__(256) kernel(const __grid_constant__ Args a)
+__global__ void __launch_bounds__(256, BACK ? 2 : 3) kernel(const __grid_constant__ Args a)
 {
     extern __shared__ __align__(16) float sh[];
+    __shared__ int live[8];
     float2 *cs = reinterpret_cast<float2 *>(sh);
-    float *red = sh + a.rows_per * a.rot; // backward: [8 warps][d]
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.lanes, per_warp = 32 / G;
+    float *gains = sh + a.rows_per * a.rot, *red = gains + 2 * a.d; // backward: red [8 warps][d]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.lanes, per_warp = 32 / G, sub = lane / G;
     const int half = a.rot / 2;
     int p0[NG], lo[NG], hi[NG];
     bool mine[NG];
@@ -139,105 +131,132 @@ __global__ void __launch_bounds__(256) kernel(const __grid_constant__ Args a)
         hi[g] = at.hi;
     }
     const float inv_d = 1.0f / (float)a.d;
-    pdl_trigger();
     pdl_wait();
+    for (int i = tid; i < 2 * a.d; i += 256) {
+        const float *from = a.gain[i >= a.d];
+        gains[i] = from ? from[i >= a.d ? i - a.d : i] : 1.0f;
+    }
     float acc[BACK ? 2 : 1][NG][2][W] = {};
+    struct Item {
+        raw_t<T, W> x[NG][2], dy[BACK ? NG : 1][2];
+        long long at; // where the result goes
+        int r, what;
+        bool real;
+    };
     for (int r0 = blockIdx.x * a.rows_per; r0 < a.N; r0 += gridDim.x * a.rows_per) {
         const int n = min(a.rows_per, a.N - r0);
-        if (half) {
-            __syncthreads();
-            angles(a, cs, r0, n, tid, 256);
-            __syncthreads();
-        }
+        const int rounds_q = (n * a.heads[0] + per_warp - 1) / per_warp, rounds = rounds_q + (n * a.heads[1] + per_warp - 1) / per_warp;
+        auto fetch = [&](int round) {
+            Item it;
+            it.what = round >= rounds_q;
+            const int H = a.heads[it.what], i = (round - (it.what ? rounds_q : 0)) * per_warp + sub;
+            it.real = i < n * H;
+            it.r = it.real ? (H == 1 ? i : (int)__umulhi((uint32_t)i, a.inverse[it.what])) : 0;
+            const long long row = r0 + it.r, col = (long long)(it.real ? i - it.r * H : 0) * a.d;
+            const T *px = reinterpret_cast<const T *>(a.x[it.what]) + row * a.ldx[it.what] + col;
+            const T *pd = reinterpret_cast<const T *>(a.dy[it.what]) + row * a.ldy[it.what] + col;
+            it.at = row * (BACK ? a.ldx[it.what] : a.ldy[it.what]) + col;
 #pragma unroll
-        for (int what = 0; what < 2; what++) {
-            const int H = a.heads[what];
-            float gain[NG][2][W];
+            for (int g = 0; g < NG; g++) {
+                it.x[g][0] = it.x[g][1] = raw_t<T, W>();
+                if (BACK)
+                    it.dy[BACK ? g : 0][0] = it.dy[BACK ? g : 0][1] = raw_t<T, W>();
+                if (it.real && mine[g]) {
+                    it.x[g][0] = *reinterpret_cast<const raw_t<T, W> *>(px + lo[g]);
+                    it.x[g][1] = *reinterpret_cast<const raw_t<T, W> *>(px + hi[g]);
+                    if (BACK) {
+                        it.dy[BACK ? g : 0][0] = *reinterpret_cast<const raw_t<T, W> *>(pd + lo[g]);
+                        it.dy[BACK ? g : 0][1] = *reinterpret_cast<const raw_t<T, W> *>(pd + hi[g]);
+                    }
+                }
+            }
+            return it;
+        };
+        Item next = {};
+        if (warp < rounds)
+            next = fetch(warp);
+        __syncthreads();
+        angles(a, cs, live, r0, n, tid);
+        __syncthreads();
+#pragma unroll 1
+        for (int round = warp; round < rounds; round += 8) { // all lanes of a warp go through every round (shuffles)
+            const Item it = next;
+            if (round + 8 < rounds)
+                next = fetch(round + 8);
+            const bool alive = it.real && live[it.r];
+            const float *gain = gains + it.what * a.d;
+            const float2 *turns = cs + it.r * half;
+            float x[NG][2][W], u[NG][2][W];
+            float sq = 0.0f;
 #pragma unroll
             for (int g = 0; g < NG; g++)
 #pragma unroll
-                for (int j = 0; j < 2; j++)
+                for (int j = 0; j < 2; j++) {
+                    take<T, W>(x[g][j], it.x[g][j]);
+                    if (BACK)
+                        take<T, W>(u[g][j], it.dy[BACK ? g : 0][j]);
+                    if (!alive) // padding: zeros, whatever lies there
+#pragma unroll
+                        for (int k = 0; k < W; k++)
+                            x[g][j][k] = u[g][j][k] = 0.0f;
 #pragma unroll
                     for (int k = 0; k < W; k++)
-                        gain[g][j][k] = a.gain[what] && mine[g] ? a.gain[what][(j ? hi[g] : lo[g]) + k] : 1.0f;
-            // a warp's heads are neighbours; all its lanes go through every round (shuffles)
-            for (int i0 = warp * per_warp; i0 < n * H; i0 += 8 * per_warp) {
-                const int i = i0 + lane / G, r = i < n * H ? i / H : 0, h = i < n * H ? i % H : 0;
-                const long long row = r0 + r;
-                const bool real = i < n * H, live = real && (!a.pos || a.pos[row] >= 0);
-                const T *px = reinterpret_cast<const T *>(a.x[what]) + row * a.ldx[what] + (size_t)h * a.d;
-                const T *pd = reinterpret_cast<const T *>(a.dy[what]) + row * a.ldy[what] + (size_t)h * a.d;
-                float x[NG][2][W] = {}, u[NG][2][W] = {};
-                float sq = 0.0f;
-#pragma unroll
-                for (int g = 0; g < NG; g++)
-                    if (live && mine[g]) {
-                        load<T, W>(x[g][0], px + lo[g]);
-                        load<T, W>(x[g][1], px + hi[g]);
-                        if (BACK) {
-                            load<T, W>(u[g][0], pd + lo[g]);
-                            load<T, W>(u[g][1], pd + hi[g]);
-                        }
-                    }
-#pragma unroll
-                for (int g = 0; g < NG; g++)
-#pragma unroll
-                    for (int k = 0; k < W; k++)
-                        sq += x[g][0][k] * x[g][0][k] + x[g][1][k] * x[g][1][k];
-                for (int o = G / 2; o > 0; o >>= 1)
-                    sq += __shfl_xor_sync(0xffffffffu, sq, o);
-                const float rs = rsqrtf(sq * inv_d + a.eps);
-                if (!BACK) {
-#pragma unroll
-                    for (int g = 0; g < NG; g++) {
-#pragma unroll
-                        for (int j = 0; j < 2; j++)
-#pragma unroll
-                            for (int k = 0; k < W; k++)
-                                u[g][j][k] = x[g][j][k] * rs * gain[g][j][k];
-                        if (p0[g] < half)
-                            turn<W>(u[g], cs + r * half + p0[g], a.adjacent, 1.0f);
-                    }
-                } else {
-                    float dot = 0.0f;
-#pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        if (p0[g] < half)
-                            turn<W>(u[g], cs + r * half + p0[g], a.adjacent, -1.0f);
-#pragma unroll
-                        for (int j = 0; j < 2; j++)
-#pragma unroll
-                            for (int k = 0; k < W; k++) {
-                                x[g][j][k] *= rs;
-                                acc[what][g][j][k] += u[g][j][k] * x[g][j][k];
-                                u[g][j][k] *= gain[g][j][k];
-                                dot += u[g][j][k] * x[g][j][k];
-                            }
-                    }
-                    for (int o = G / 2; o > 0; o >>= 1)
-                        dot += __shfl_xor_sync(0xffffffffu, dot, o);
-                    dot *= inv_d;
-#pragma unroll
-                    for (int g = 0; g < NG; g++)
-#pragma unroll
-                        for (int j = 0; j < 2; j++)
-#pragma unroll
-                            for (int k = 0; k < W; k++)
-                                u[g][j][k] = rs * (u[g][j][k] - x[g][j][k] * dot);
+                        sq += x[g][j][k] * x[g][j][k];
                 }
-                // padding: x and u are zeros, and so are the results (eps may be 0)
-                T *py = reinterpret_cast<T *>(a.y[what]) + row * (BACK ? a.ldx[what] : a.ldy[what]) + (size_t)h * a.d;
+            for (int o = G / 2; o > 0; o >>= 1)
+                sq += __shfl_xor_sync(0xffffffffu, sq, o);
+            const float rs = alive ? rsqrtf(sq * inv_d + a.eps) : 0.0f;
+            if (!BACK) {
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    if (!mine[g])
+                        continue;
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int k = 0; k < W; k++)
+                            u[g][j][k] = x[g][j][k] * rs * gain[(j ? hi[g] : lo[g]) + k];
+                    if (p0[g] < half)
+                        turn<W>(u[g], turns + p0[g], a.adjacent, 1.0f);
+                }
+            } else {
+                float dot = 0.0f;
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    if (!mine[g])
+                        continue;
+                    if (p0[g] < half)
+                        turn<W>(u[g], turns + p0[g], a.adjacent, -1.0f);
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int k = 0; k < W; k++) {
+                            x[g][j][k] *= rs;
+                            const float ux = u[g][j][k] * x[g][j][k];
+                            acc[0][g][j][k] += it.what ? 0.0f : ux;
+                            acc[BACK ? 1 : 0][g][j][k] += it.what ? ux : 0.0f;
+                            u[g][j][k] *= gain[(j ? hi[g] : lo[g]) + k];
+                            dot += u[g][j][k] * x[g][j][k];
+                        }
+                }
+                for (int o = G / 2; o > 0; o >>= 1)
+                    dot += __shfl_xor_sync(0xffffffffu, dot, o);
+                dot *= inv_d;
 #pragma unroll
                 for (int g = 0; g < NG; g++)
-                    if (real && mine[g]) {
-                        if (!live)
 #pragma unroll
-                            for (int k = 0; k < W; k++)
-                                u[g][0][k] = u[g][1][k] = 0.0f;
-                        store<T, W>(py + lo[g], u[g][0]);
-                        store<T, W>(py + hi[g], u[g][1]);
-                    }
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int k = 0; k < W; k++)
+                            u[g][j][k] = rs * (u[g][j][k] - x[g][j][k] * dot);
             }
+            T *py = reinterpret_cast<T *>(a.y[it.what]) + it.at;
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+                if (it.real && mine[g]) {
+                    *reinterpret_cast<raw_t<T, W> *>(py + lo[g]) = alive ? put<T, W>(u[g][0]) : raw_t<T, W>();
+                    *reinterpret_cast<raw_t<T, W> *>(py + hi[g]) = alive ? put<T, W>(u[g][1]) : raw_t<T, W>();
+                }
         }
     }
     if (BACK && a.part) {
@@ -268,27 +287,29 @@ __global__ void __launch_bounds__(256) kernel(const __grid_constant__ Args a)
     }
 }
 
-// dgain of queries and keys: the CTAs' sums, eight strands in a fixed order
+// dgain of queries and keys: the CTAs' sums, eight columns a CTA, 32 strands in a fixed order
 __global__ void __launch_bounds__(256) gain_kernel(const float *__restrict__ part, int n_parts, int d, float *dgain_q, float *dgain_k)
 {
-    __shared__ float red[8][32];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5;
-    pdl_trigger();
+    __shared__ float red[32][9];
+    const int x = threadIdx.x & 7, strand = threadIdx.x >> 3, col = blockIdx.x * 8 + x;
     pdl_wait();
-    float s = 0.0f;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (col < 2 * d)
-        for (int i = strand; i < n_parts; i += 8)
-            s += part[(size_t)i * 2 * d + col];
-    red[strand][threadIdx.x & 31] = s;
+        for (int i = strand; i < n_parts; i += 128)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i + 32 * k < n_parts)
+                    s[k] += part[(size_t)(i + 32 * k) * 2 * d + col];
+    red[strand][x] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
     if (strand == 0 && col < 2 * d) {
-        s = red[0][threadIdx.x];
+        float sum = 0.0f;
 #pragma unroll
-        for (int k = 1; k < 8; k++)
-            s += red[k][threadIdx.x];
+        for (int k = 0; k < 32; k++)
+            sum += red[k][x];
         float *to = col < d ? dgain_q : dgain_k;
         if (to)
-            to[col < d ? col : col - d] = s;
+            to[col < d ? col : col - d] = sum;
     }
 }
 
