@@ -19,48 +19,38 @@ static int distill_check(const nncu_distill_shape *s)
     return NNCU_OK;
 }
 
-template <typename TZ, typename TG, int WHAT, int THR, int PER, bool TWO> static int distill_launch(const distill::Args &a, cudaStream_t st)
+// An SM takes as many CTAs as rows fit its shared memory, each with a place or, where eight fit twice, more: one loads
+// while others compute (rows of 16384 fp32 logits, 2048 of them, loss and gradient: three CTAs of one place 55 us, one CTA of
+// three places 78).  Some 1024 threads an SM share them.
+template <typename TZ, typename TG, int WHAT, int HARD> static int distill_launch(distill::Args &a, cudaStream_t st)
 {
-    CUDA_TRY(launch_k(distill::kernel<TZ, TG, WHAT, THR, PER, TWO>, dim3(a.N), dim3(THR), sizeof(float) * 3 * (size_t)a.K4, st, a));
+    const int entries = 2 * 3 * 4 * a.K4, fixed = entries + 4 * distill::PLACES + 2048; // static arrays and what a CTA costs
+    const long long row = (((long long)a.V * sizeof(TZ)) + 31) & ~15ll;
+    if (row + fixed > SMEM_MOST) {
+        a.slots = a.slot_bytes = 0;
+        CUDA_TRY(launch_k(distill::kernel<TZ, TG, WHAT, HARD, false>, dim3(a.N), dim3(distill::THREADS_MAX), (size_t)entries, st, a));
+        KERNEL_CHECK();
+        return NNCU_OK;
+    }
+    a.slot_bytes = (int)row;
+    const int ctas = std::min(a.V <= 2048 ? 16 : 8, SMEM_MOST / (a.slot_bytes + fixed));
+    int threads = 64;
+    while (threads < distill::THREADS_MAX && 2 * threads * ctas <= 1024)
+        threads *= 2;
+    a.slots = std::max(1, std::min(distill::SLOTS_MAX, (SMEM_MOST / ctas - fixed) / a.slot_bytes));
+    static DeviceOnce once;
+    NNCU_TRY(smem_limit(once, distill::kernel<TZ, TG, WHAT, HARD, true>, SMEM_MOST - 4 * distill::PLACES - 1024));
+    CUDA_TRY(launch_k(distill::kernel<TZ, TG, WHAT, HARD, true>, dim3(std::min(a.N, ctas * SMS)), dim3(threads), (size_t)a.slots * a.slot_bytes + entries,
+                      st, a));
     KERNEL_CHECK();
     return NNCU_OK;
 }
 
-// Rows of up to 1024 logits take a CTA of four warps, up to 4096 one of eight, longer ones sixteen; a thread holds 32
-// logits at most.  The gradient from sums that stand needs a logit only once.
-template <typename TZ, typename TG, int WHAT, bool TWO> static int distill_sized(const distill::Args &a, cudaStream_t st)
+template <typename TZ, typename TG, int WHAT> static int distill_run(distill::Args &a, cudaStream_t st)
 {
-    const bool begins = a.ldz % 4 == 0 && aligned(a.z, 4 * sizeof(TZ)); // every row with a group
-    const int groups = begins ? ceil_div(a.V, 4) : (a.V + 6) / 4;
-    if constexpr (WHAT == distill::GRAD) {
-        return groups <= 512 ? distill_launch<TZ, TG, WHAT, 128, 0, TWO>(a, st) : distill_launch<TZ, TG, WHAT, 256, 0, TWO>(a, st);
-    } else {
-        if (groups <= 128)
-            return distill_launch<TZ, TG, WHAT, 128, 1, TWO>(a, st);
-        if (groups <= 256)
-            return distill_launch<TZ, TG, WHAT, 128, 2, TWO>(a, st);
-        if (groups <= 512)
-            return distill_launch<TZ, TG, WHAT, 256, 2, TWO>(a, st);
-        if (groups <= 1024)
-            return distill_launch<TZ, TG, WHAT, 256, 4, TWO>(a, st);
-        switch (ceil_div(groups, 512)) {
-        case 3: return distill_launch<TZ, TG, WHAT, 512, 3, TWO>(a, st);
-        case 4: return distill_launch<TZ, TG, WHAT, 512, 4, TWO>(a, st);
-        case 5: return distill_launch<TZ, TG, WHAT, 512, 5, TWO>(a, st);
-        case 6: return distill_launch<TZ, TG, WHAT, 512, 6, TWO>(a, st);
-        case 7: return distill_launch<TZ, TG, WHAT, 512, 7, TWO>(a, st);
-        case 8: return distill_launch<TZ, TG, WHAT, 512, 8, TWO>(a, st);
-        default: return distill_launch<TZ, TG, WHAT, 512, 0, TWO>(a, st);
-        }
-    }
-}
-
-template <typename TZ, typename TG, int WHAT> static int distill_run(const distill::Args &a, cudaStream_t st)
-{
-    if constexpr (WHAT != distill::GRAD)
-        if (!a.power)
-            return distill_sized<TZ, TG, WHAT, true>(a, st);
-    return distill_sized<TZ, TG, WHAT, false>(a, st);
+    if (a.tau == 1.0f || a.share == 1.0f) // p is p_tau, or not there
+        return distill_launch<TZ, TG, WHAT, distill::SAME>(a, st);
+    return a.tau == 2.0f ? distill_launch<TZ, TG, WHAT, distill::SQUARE>(a, st) : distill_launch<TZ, TG, WHAT, distill::APART>(a, st);
 }
 
 template <int WHAT>
@@ -84,11 +74,10 @@ static int distill_any(const nncu_distill_shape *s, const void *logits, const in
     a.ldz = s->ld_logits ? s->ld_logits : s->n_symbols;
     a.lddz = s->ld_dlogits ? s->ld_dlogits : s->n_symbols;
     a.N = s->n_rows; a.V = s->n_symbols; a.K = s->n_top;
-    a.K4 = (s->n_top + 3) & ~3;
+    a.K4 = (s->n_top + 1 + 3) & ~3;
     a.share = s->teacher_share;
     a.tau = a.share == 0.0f ? 1.0f : s->temperature; // of a term that is not there
     a.inv_tau = 1.0f / a.tau;
-    a.power = a.share == 1.0f ? 1 : a.tau <= 4.0f && a.tau == floorf(a.tau) ? (int)a.tau : 0; // of p too
     ChainScope chain;
     cudaStream_t st = (cudaStream_t)cuda_stream;
     if (!(WHAT & distill::GRAD))

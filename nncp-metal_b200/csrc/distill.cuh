@@ -4,23 +4,32 @@
 //   L = w [(1 - share) (lse(z) - z_target) + share tau^2 sum_k q_k (ln q_k - ln p_tau(id_k))]
 //   dL/dz = w [(1 - share) (p - 1_target) + share tau (p_tau - sum_k q_k 1_{id_k})]
 //
-// Bound by HBM: the logits once in, the gradient once out.  A row of up to 16384 logits lies in the registers of one
-// CTA from the first read to the gradient; longer rows are read again.  With d = z - max,
-// T1 = sum_k e_k (top_k - maxtop - d_k) / tau and e_k = exp((top_k - maxtop) / tau) the teacher's term is
-// T1 / sum e - ln sum e + ln sum exp(d / tau): two reductions over a row, one of maxima and one of sums.
+// With u = z log2(e) / tau - R for a whole number R next to the row's largest (so that no rounding of a shift is in
+// every term), e = 2^u and l = sum e:  p_tau = e / l,  ln p_tau = u ln 2 - ln l,  and with e_k = exp((top_k - maxtop) / tau)
+// the teacher's term is sum_k e_k ((top_k - maxtop) / tau - u_k ln 2) / sum e_k - ln sum e_k + ln l.  Two reductions over a
+// row, one of maxima and one of sums.
 //
-// Exponentials are what an SM has least of: sixteen a cycle, and two a logit and pass take half of the time that HBM
-// needs.  At a temperature of 1, 2, 3 or 4 exp(d) is that power of exp(d / tau): one exponential a logit and one register
-// for it from the sums to the gradient, and two rows of 16384 to an SM instead of one.
+// Bound by HBM: the logits once in, the gradient once out.  A CTA stays and takes every gridDim.x-th row; the rows behind come
+// by bulk copy into `slots` places in shared memory while one is gone through three times there: maximum, sums,
+// gradient.  (A row that is loaded, reduced twice and stored in turn leaves HBM idle most of the time: 2048 rows of 16384
+// logits, loss and gradient, took 69 us with a row in the registers of a CTA.)  What of a row does not lie in whole
+// 16-byte pieces, at its two ends, is a thread's each.
+//
+// Exponentials are what an SM has least of, sixteen a cycle.  Where tau is 1 or 2, or one of the terms is not there, p
+// is 2^u or its square over their sum: one exponential a logit and pass instead of two.
 //
 // The gradient is written dense first; the few entries that the target and the teacher name are computed again whole and
 // written over it, so that each value is rounded once.
 #pragma once
+#include "gemm_tc.cuh"
 #include "warp_mma.cuh"
 
 namespace distill {
 
 constexpr int TOP_MAX = NNCU_DISTILL_TOP_MAX;
+constexpr int THREADS_MAX = 512, SLOTS_MAX = 4;
+constexpr int PLACES = 1024; // by which entries that name the same symbol are found
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Args {
     const void *z;
@@ -32,256 +41,355 @@ struct Args {
     float *lse;             // [N][2]: of z and of z / tau
     void *dz;
     long long ldz, lddz;
-    int N, V, K, K4;        // K4: K up to the next multiple of four
-    int power;              // exp(d) is this power of exp(d / tau); 0: neither 1 to 4
+    int N, V, K, K4;        // K4: entries and the target, up to a multiple of four
+    int slots, slot_bytes;
     float share, tau, inv_tau;
 };
 
 enum { LOSS = 1, GRAD = 2 }; // what a launch gives; GRAD alone takes the sums from lse
+// how p follows from e: itself, its square, or an exponential of its own
+enum { SAME = 1, SQUARE = 2, APART = 0 };
 
-// block-wide reductions of a few values at once; every thread gets the results
-template <int THR, int N_, bool MAX> __device__ __forceinline__ void reduce(float (&v)[N_], float *red)
+__device__ __forceinline__ float ex2(float x)
 {
-    constexpr int WARPS = THR / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// block-wide reductions of a few values at once behind one barrier; every thread gets the results
+template <int N_, bool MAX> __device__ __forceinline__ void reduce(float (&v)[N_], float *red)
+{
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < N_; i++)
         v[i] = MAX ? warp_max(v[i]) : warp_sum(v[i]);
-    __syncthreads(); // red may still be read
     if (lane == 0)
 #pragma unroll
         for (int i = 0; i < N_; i++)
-            red[i * WARPS + warp] = v[i];
+            red[i * 16 + warp] = v[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N_; i++) {
-        float s = red[i * WARPS + lane % WARPS];
+    for (int i = 0; i < N_; i++)
+        v[i] = red[i * 16 + (lane & (warps - 1))]; // warps: a power of two, 16 at most
+    for (int o = warps / 2; o > 0; o >>= 1)
 #pragma unroll
-        for (int o = WARPS / 2; o > 0; o >>= 1) {
-            const float u = __shfl_xor_sync(0xffffffffu, s, o);
-            s = MAX ? fmaxf(s, u) : s + u;
+        for (int i = 0; i < N_; i++) {
+            const float u = __shfl_xor_sync(0xffffffffu, v[i], o);
+            v[i] = MAX ? fmaxf(v[i], u) : v[i] + u;
         }
-        v[i] = s;
-    }
 }
 
-template <typename T> __device__ __forceinline__ float4 load4(const T *p)
+template <typename T> __device__ __forceinline__ void load4(float (&v)[4], const T *p)
 {
-    if constexpr (sizeof(T) == 4)
-        return *reinterpret_cast<const float4 *>(p);
-    const uint2 u = *reinterpret_cast<const uint2 *>(p);
-    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+    if constexpr (sizeof(T) == 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(p);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+        const uint2 u = *reinterpret_cast<const uint2 *>(p);
+        v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
+        v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
+    }
 }
-template <typename T> __device__ __forceinline__ void store4(T *p, float4 v)
+template <typename T> __device__ __forceinline__ void store4(T *p, const float (&v)[4])
 {
     if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<float4 *>(p) = v;
+        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
     else
-        *reinterpret_cast<uint2 *>(p) = make_uint2(fa::pack2(v.x, v.y), fa::pack2(v.z, v.w));
+        *reinterpret_cast<uint2 *>(p) = make_uint2(fa::pack2(v[0], v[1]), fa::pack2(v[2], v[3]));
 }
 
-// exp(d) from exp(d / tau)
-__device__ __forceinline__ float to_power(float e, int power)
-{
-    const float e2 = e * e;
-    return power == 1 ? e : power == 2 ? e2 : power == 3 ? e2 * e : e2 * e2;
-}
+// A CTA's entries of one row: the teacher's, and behind them the target, whose e is 0
+struct Entries {
+    int32_t *id;
+    float *e, *z;
+};
 
-// PER groups of four logits a thread; PER = 0: a row of any length, read again for each use.  TWO: exp(d) and
-// exp(d / tau) are apart.  Groups begin at multiples of four elements in memory, `shift` logits before the row's first where
-// that lies between: whole groups go in one access, the row's ends one by one.
-template <typename TZ, typename TG, int WHAT, int THR, int PER, bool TWO>
-__global__ void __launch_bounds__(THR, PER > 0 && !TWO && (WHAT & LOSS) ? 1024 / THR : 1) kernel(const __grid_constant__ Args a)
+// RING: rows through shared memory; otherwise rows too long for it are read from global memory each time, one to a CTA.
+//
+// Two barriers a row.  What one row leaves for behind a barrier -- the named entries over its dense gradient, its place in the
+// ring for the next copy -- is done behind the first one of the next row; entries and partial sums lie in two
+// places that rows take in turn.
+template <typename TZ, typename TG, int WHAT, int HARD, bool RING>
+__global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__ Args a)
 {
-    constexpr bool KEEP = PER > 0;
-    constexpr int E = KEEP ? PER : 1;
-    extern __shared__ __align__(16) float sh[]; // of the teacher's entries: symbols, e, the student's logits
-    __shared__ float red[4 * THR / 32];
-    int32_t *sid = reinterpret_cast<int32_t *>(sh);
-    float *se = sh + a.K4, *sz = se + a.K4;
-    const int tid = threadIdx.x, V = a.V, K = a.K;
-    const long long r = blockIdx.x;
-    pdl_wait();
-    const TZ *z = reinterpret_cast<const TZ *>(a.z) + r * a.ldz;
-    TG *dz = reinterpret_cast<TG *>(a.dz) + r * a.lddz;
-    const int shift = (int)(reinterpret_cast<uintptr_t>(z) / sizeof(TZ) % 4);
-    auto each = [&](auto f) { // f(slot, first logit)
-        if constexpr (KEEP) {
-#pragma unroll
-            for (int k = 0; k < PER; k++)
-                f(k, (k * THR + tid) * 4 - shift);
-        } else {
-#pragma unroll 4
-            for (int i = tid * 4 - shift; i < V; i += THR * 4)
-                f(0, i);
-        }
-    };
-    float x[E][4], y[TWO ? E : 1][4];
-    auto read = [&](float (&v)[4], int i) {
-        if (i >= 0 && i + 4 <= V) {
-            const float4 f = load4<TZ>(z + i);
-            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-        } else {
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-                v[c] = i + c >= 0 && i + c < V ? to_f(z[i + c]) : -INFINITY;
-        }
-    };
-    if constexpr (KEEP)
-        each([&](int k, int i) { read(x[k], i); });
-    const float w = a.weight ? a.weight[r] : 1.0f;
-    const int target = a.targets ? a.targets[r] : -1;
-    const bool known = target >= 0 && target < V;
-    // the teacher's entries
-    float most[2] = {-INFINITY, -INFINITY};
-    for (int k = tid; k < a.K4; k += THR) {
-        const int id = k < K ? a.ids[r * K + k] : -1;
-        const bool there = id >= 0 && id < V;
-        sid[k] = there ? id : -1;
-        se[k] = there ? a.top[r * K + k] : -INFINITY;
-        sz[k] = there ? to_f(z[id]) : 0.0f;
-        most[1] = fmaxf(most[1], se[k]);
+    extern __shared__ __align__(128) unsigned char ring[]; // rows, then twice the entries: symbols, e, the student's logits
+    __shared__ float red[2][6 * 16];
+    __shared__ __align__(8) uint64_t bars[SLOTS_MAX];
+    __shared__ int abort_s, flag;
+    __shared__ __align__(4) uint16_t last[PLACES], many[PLACES]; // of the entries of a place: one of them; the row in which it had several
+    const int tid = threadIdx.x, thr = blockDim.x, V = a.V, K = a.K;
+    const uint32_t bar0 = fa::smem_addr(bars), ring0 = fa::smem_addr(ring);
+    if (RING && tid == 0) {
+        abort_s = 0;
+        for (int i = 0; i < a.slots; i++)
+            tc::mbar_init(bar0 + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const float z_target = known ? to_f(z[target]) : 0.0f;
-    auto nothing = [&]() { // a row without weight, or whose mask leaves no symbol
-        if (WHAT & LOSS) {
-            if (tid == 0) {
+    for (int i = tid; i < PLACES / 2; i += thr)
+        reinterpret_cast<uint32_t *>(many)[i] = 0xffffffffu;
+    __syncthreads();
+    pdl_wait();
+    bool ok = true; // this thread's waits; behind one that ran out results are NaN and nothing more is asked for
+    // the whole pieces of row r: logits [lo, hi)
+    auto pieces = [&](const TZ *z, int &lo, int &hi) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(z);
+        lo = min(V, (int)(-at & 15) / (int)sizeof(TZ));
+        hi = max(lo, V - (int)((at + (size_t)V * sizeof(TZ)) & 15) / (int)sizeof(TZ));
+    };
+    auto fetch = [&](int slot, long long r) {
+        if (RING && tid == 0 && ok && r < a.N) {
+            const TZ *z = reinterpret_cast<const TZ *>(a.z) + r * a.ldz;
+            int lo, hi;
+            pieces(z, lo, hi);
+            const uint32_t bytes = (uint32_t)(hi - lo) * sizeof(TZ), bar = bar0 + 8 * slot;
+            tc::mbar_expect_tx(bar, bytes);
+            if (bytes)
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring0 + slot * a.slot_bytes),
+                             "l"(z + lo), "r"(bytes), "r"(bar)
+                             : "memory");
+        }
+    };
+    // what a row needs beside its logits, one row ahead
+    struct Side {
+        float w, top, lse, lse_tau;
+        int target, id;
+    };
+    auto side = [&](long long r) {
+        Side s;
+        s.w = a.weight ? a.weight[r] : 1.0f;
+        s.target = a.targets ? a.targets[r] : -1;
+        s.id = tid < K ? a.ids[r * K + tid] : -1;
+        s.top = tid < K ? a.top[r * K + tid] : 0.0f;
+        if constexpr (!(WHAT & LOSS)) {
+            s.lse = a.lse[2 * r];
+            s.lse_tau = a.lse[2 * r + 1];
+        }
+        return s;
+    };
+    const float scale = LOG2E * a.inv_tau;
+    const bool defer = K + 1 <= 2 * thr; // a thread keeps two entries at most
+    long long r = blockIdx.x;
+    for (int i = 0; i < a.slots; i++)
+        fetch(i, r + (long long)i * gridDim.x);
+    Side next = side(r);
+    int slot = 0, phase = 0, turn = 0;
+    TG *late[2] = {nullptr, nullptr}; // entries of the row before, to be written behind a barrier
+    float late_value[2];
+    uint16_t round = 0;
+    for (; r < a.N; r += gridDim.x, turn ^= 1, round++) {
+        const Side now = next;
+        if (r + gridDim.x < a.N)
+            next = side(r + gridDim.x);
+        const TZ *z = reinterpret_cast<const TZ *>(a.z) + r * a.ldz;
+        TG *dz = reinterpret_cast<TG *>(a.dz) + r * a.lddz;
+        int lo, hi;
+        pieces(z, lo, hi);
+        const TZ *row = RING ? reinterpret_cast<const TZ *>(ring + slot * a.slot_bytes) : z + lo; // logit lo + i at row[i]
+        const int pieces4 = (hi - lo) / 4, edge = tid < lo ? tid : tid < lo + V - hi ? hi + tid - lo : -1; // a logit at one of the ends
+        const float z_edge = edge >= 0 ? to_f(z[edge]) : -INFINITY;
+        if (RING)
+            ok = ok && tc::mbar_wait(bar0 + 8 * slot, phase, &abort_s, &flag, 82);
+        const float w = now.w;
+        const bool known = now.target >= 0 && now.target < V;
+        Entries en;
+        en.id = reinterpret_cast<int32_t *>(ring + a.slots * a.slot_bytes) + turn * 3 * a.K4;
+        en.e = reinterpret_cast<float *>(en.id) + a.K4;
+        en.z = en.e + a.K4;
+        float most[2] = {z_edge, -INFINITY};
+#pragma unroll 1
+        for (int k = tid; k < a.K4; k += thr) {
+            const int id = k == K ? now.target : k > K ? -1 : k < thr ? now.id : a.ids[r * K + k];
+            const bool there = id >= 0 && id < V;
+            const float top = there && k < K ? (k < thr ? now.top : a.top[r * K + k]) : -INFINITY;
+            en.id[k] = there ? id : -1;
+            if ((WHAT & GRAD) && there)
+                last[(unsigned)id % PLACES] = (uint16_t)k;
+            en.e[k] = top;
+            en.z[k] = !there ? 0.0f : to_f(RING && id >= lo && id < hi ? row[id - lo] : z[id]);
+            most[1] = fmaxf(most[1], top);
+        }
+        if constexpr (WHAT & LOSS) {
+#pragma unroll 4
+            for (int i = tid; i < pieces4; i += thr) {
+                float v[4];
+                load4<TZ>(v, row + 4 * i);
+                most[0] = fmaxf(fmaxf(most[0], fmaxf(v[0], v[1])), fmaxf(v[2], v[3]));
+            }
+        }
+        reduce<2, true>(most, red[turn]);
+        // behind the barrier: what the row before has left
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if ((WHAT & GRAD) && late[i])
+                *late[i] = from_f<TG>(late_value[i]);
+            late[i] = nullptr;
+        }
+        if (a.slots > 1 && r != blockIdx.x)
+            fetch(slot ? slot - 1 : a.slots - 1, r + (long long)(a.slots - 1) * gridDim.x);
+        const float m = (WHAT & LOSS) ? most[0] : now.lse_tau * a.tau, mq = most[1];
+        const bool none = w == 0.0f || ((WHAT & LOSS) ? most[0] : now.lse) == -INFINITY; // no weight, or a mask that leaves no symbol
+        if (none) {
+            if ((WHAT & LOSS) && tid == 0) {
                 a.loss[r] = 0.0f;
                 if (a.lse)
                     a.lse[2 * r] = a.lse[2 * r + 1] = -INFINITY;
             }
-        }
-        if (WHAT & GRAD)
-            for (int i = tid; i < V; i += THR)
-                dz[i] = from_f<TG>(0.0f);
-    };
-    if (w == 0.0f) {
-        nothing();
-        return;
-    }
-    float lse = 0.0f, lse_tau = 0.0f, m = 0.0f, inv_l = 0.0f, inv_l_tau = 0.0f;
-    if constexpr (WHAT & LOSS)
-        each([&](int k, int i) {
-            if constexpr (!KEEP)
-                read(x[k], i);
-            most[0] = fmaxf(fmaxf(fmaxf(most[0], x[k][0]), fmaxf(x[k][1], x[k][2])), x[k][3]);
-        });
-    reduce<THR, 2, true>(most, red);
-    const float mq = most[1];
-    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f}; // of exp(d), of exp(d / tau), of e, T1
-    if constexpr (WHAT & LOSS) {
-        m = most[0];
-        if (m == -INFINITY) {
-            nothing();
-            return;
-        }
-        const float f = 1.4426950408889634f * a.inv_tau, from = -m * f;
-        each([&](int k, int i) {
-            if constexpr (!KEEP)
-                read(x[k], i);
+            if constexpr (WHAT & GRAD)
+                for (int i = tid; i < V; i += thr)
+                    dz[i] = from_f<TG>(0.0f);
+        } else {
+            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f}; // of what p is over, of e, of e_k, the teacher's
+            const float shift = rintf(m * scale), shift1 = rintf(m * LOG2E);
+            auto soft = [&](float v) { return ex2(fmaf(v, scale, -shift)); };
+            auto hard = [&](float v, float e) { return HARD == SAME ? e : HARD == SQUARE ? e * e : ex2(fmaf(v, LOG2E, -shift1)); };
+            if constexpr (WHAT & LOSS) {
+#pragma unroll 4
+                for (int i = tid; i < pieces4; i += thr) {
+                    float v[4];
+                    load4<TZ>(v, row + 4 * i);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const float e = exp2f(fmaf(x[k][c], f, from));
-                if constexpr (TWO) {
-                    x[k][c] = __expf(x[k][c] - m);
-                    y[k][c] = e;
-                    sums[0] += x[k][c];
-                } else {
-                    x[k][c] = e;
-                    sums[0] += to_power(e, a.power);
+                    for (int c = 0; c < 4; c++) {
+                        const float e = soft(v[c]);
+                        sums[1] += e;
+                        if constexpr (HARD != SAME)
+                            sums[0] += hard(v[c], e);
+                    }
                 }
+                const float e = soft(z_edge);
                 sums[1] += e;
+                if constexpr (HARD != SAME)
+                    sums[0] += hard(z_edge, e);
             }
-        });
-    }
-    for (int k = tid; k < a.K4; k += THR) {
-        const float d = se[k] - mq, e = sid[k] >= 0 ? expf(d * a.inv_tau) : 0.0f;
-        if (e > 0.0f) {
-            sums[2] += e;
-            if constexpr (WHAT & LOSS)
-                sums[3] += e * (d - (sz[k] - m)) * a.inv_tau;
-        }
-        se[k] = e > 0.0f ? e : 0.0f;
-    }
-    reduce<THR, 4, false>(sums, red); // its barriers also let the entries be read by all
-    pdl_trigger();
-    const bool taught = sums[2] > 0.0f;
-    if constexpr (WHAT & LOSS) {
-        inv_l = 1.0f / sums[0];
-        inv_l_tau = 1.0f / sums[1];
-        if (tid == 0) {
-            float loss = 0.0f;
-            if (known && a.share != 1.0f)
-                loss += (1.0f - a.share) * (logf(sums[0]) - (z_target - m));
-            if (taught && a.share != 0.0f)
-                loss += a.share * a.tau * a.tau * (sums[3] / sums[2] + logf(sums[1] / sums[2]));
-            a.loss[r] = w * loss;
-            if (a.lse) {
-                a.lse[2 * r] = m + logf(sums[0]);
-                a.lse[2 * r + 1] = m * a.inv_tau + logf(sums[1]);
+#pragma unroll 1
+            for (int k = tid; k < a.K4; k += thr) {
+                const float d = (en.e[k] - mq) * a.inv_tau, e = k < K && en.id[k] >= 0 ? expf(d) : 0.0f;
+                if (e > 0.0f) {
+                    sums[2] += e;
+                    if constexpr (WHAT & LOSS)
+                        sums[3] += e * (d - fmaf(en.z[k], scale, -shift) * LN2);
+                }
+                en.e[k] = e > 0.0f ? e : 0.0f;
+                if ((WHAT & GRAD) && en.id[k] >= 0 && last[(unsigned)en.id[k] % PLACES] != k)
+                    many[(unsigned)en.id[k] % PLACES] = round;
+            }
+            reduce<4, false>(sums, red[turn] + 2 * 16); // its barrier also lets the entries be read by all
+            if constexpr (HARD == SAME)
+                sums[0] = sums[1];
+            if (!ok)
+                sums[0] = sums[1] = sums[2] = sums[3] = NAN;
+            const bool taught = !(sums[2] <= 0.0f);
+            if ((WHAT & LOSS) && tid == thr - 1) {
+                // log2 of e's whole part of p, for the target and for the sum
+                const float whole = HARD == APART ? shift1 : HARD * shift;
+                float loss = 0.0f;
+                if (known && a.share != 1.0f)
+                    loss += (1.0f - a.share) * (logf(sums[0]) - fmaf(en.z[K], HARD == APART ? LOG2E : HARD * scale, -whole) * LN2);
+                if (taught && a.share != 0.0f)
+                    loss += a.share * a.tau * a.tau * (sums[3] / sums[2] + logf(sums[1] / sums[2]));
+                a.loss[r] = w * loss;
+                if (a.lse) {
+                    a.lse[2 * r] = fmaf(whole, LN2, logf(sums[0]));
+                    a.lse[2 * r + 1] = fmaf(shift, LN2, logf(sums[1]));
+                }
+            }
+            if constexpr (WHAT & GRAD) {
+                const float f = known ? w * (1.0f - a.share) : 0.0f, f_tau = taught ? w * a.share * a.tau : 0.0f;
+                float g, g_tau; // of what p is over, of e
+                if constexpr (WHAT & LOSS) {
+                    g = __fdividef(f, sums[0]);
+                    g_tau = __fdividef(f_tau, sums[1]);
+                } else {
+                    g = f * ex2(fmaf(-now.lse, LOG2E, HARD == APART ? shift1 : HARD * shift));
+                    g_tau = f_tau * ex2(fmaf(-now.lse_tau, LOG2E, shift));
+                }
+                const float inv_e = taught ? __fdividef(f_tau, sums[2]) : 0.0f;
+                auto both = [&](float v) {
+                    const float e = soft(v);
+                    return HARD == SAME ? (g + g_tau) * e : HARD == SQUARE ? e * fmaf(g, e, g_tau) : fmaf(g, hard(v, e), g_tau * e);
+                };
+                // The gradient of the symbol of entry k: f less at the target, and inv_e times the sum of e over all entries that
+                // name it.  The first of them writes.  Entries alone in their place are alone.
+                auto named = [&](int k, TG *&to, float &value) {
+                    const int id = k <= K ? en.id[k] : -1;
+                    to = nullptr;
+                    if (id < 0)
+                        return;
+                    float off = en.e[k];
+                    bool first = true;
+                    if (many[(unsigned)id % PLACES] == round) {
+                        off = 0.0f;
+#pragma unroll 1
+                        for (int j = 0; j < a.K4; j += 4) {
+                            const int4 like = *reinterpret_cast<const int4 *>(en.id + j);
+                            if (like.x == id || like.y == id || like.z == id || like.w == id)
+                                for (int i = j; i < j + 4; i++)
+                                    if (en.id[i] == id) {
+                                        off += en.e[i];
+                                        first = first && i >= k;
+                                    }
+                        }
+                    }
+                    if (first) {
+                        to = dz + id;
+                        value = both(en.z[k]) - (id == now.target ? f : 0.0f) - off * inv_e;
+                    }
+                };
+                if (defer) {
+                    if (tid <= K)
+                        named(tid, late[0], late_value[0]);
+                    if (tid + thr <= K)
+                        named(tid + thr, late[1], late_value[1]);
+                }
+                TG *to = dz + lo;
+                if (reinterpret_cast<uintptr_t>(to) % (4 * sizeof(TG)) == 0) {
+#pragma unroll 4
+                    for (int i = tid; i < pieces4; i += thr) {
+                        float v[4];
+                        load4<TZ>(v, row + 4 * i);
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+                            v[c] = both(v[c]);
+                        store4<TG>(to + 4 * i, v);
+                    }
+                } else {
+#pragma unroll 4
+                    for (int i = tid; i < hi - lo; i += thr)
+                        to[i] = from_f<TG>(both(to_f(row[i])));
+                }
+                if (edge >= 0)
+                    dz[edge] = from_f<TG>(both(z_edge));
+                if (!defer) {
+                    __syncthreads();
+                    for (int k = tid; k <= K; k += thr) {
+                        TG *at;
+                        float value;
+                        named(k, at, value);
+                        if (at)
+                            *at = from_f<TG>(value);
+                    }
+                }
             }
         }
-    } else {
-        lse = a.lse[2 * r];
-        lse_tau = a.lse[2 * r + 1];
-        if (lse == -INFINITY) {
-            nothing();
-            return;
+        if (a.slots == 1) { // no place for a row ahead
+            __syncthreads();
+            fetch(0, r + gridDim.x);
+        }
+        if (++slot >= a.slots) {
+            slot = 0;
+            phase ^= 1;
         }
     }
     if constexpr (WHAT & GRAD) {
-        const float f = known ? w * (1.0f - a.share) : 0.0f, f_tau = taught ? w * a.share * a.tau : 0.0f;
-        const float g = f * inv_l, g_tau = f_tau * inv_l_tau;
-        // f p + f_tau p_tau of one logit
-        auto both = [&](float zv) {
-            if constexpr (WHAT & LOSS)
-                return g * __expf(zv - m) + g_tau * __expf((zv - m) * a.inv_tau);
-            else
-                return f * __expf(zv - lse) + f_tau * __expf(zv * a.inv_tau - lse_tau);
-        };
-        const bool whole = reinterpret_cast<uintptr_t>(dz) / sizeof(TG) % 4 == shift; // the groups are groups there too
-        each([&](int k, int i) {
-            float o[4];
-            if constexpr (KEEP && (WHAT & LOSS)) {
+        __syncthreads();
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    o[c] = TWO ? g * x[k][c] + g_tau * y[TWO ? k : 0][c] : g * to_power(x[k][c], a.power) + g_tau * x[k][c];
-            } else {
-                float v[4];
-                read(v, i);
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    o[c] = both(v[c]);
-            }
-            if (whole && i >= 0 && i + 4 <= V)
-                store4<TG>(dz + i, make_float4(o[0], o[1], o[2], o[3]));
-            else
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (i + c >= 0 && i + c < V)
-                        dz[i + c] = from_f<TG>(o[c]);
-        });
-        __syncthreads(); // the named entries go over the dense ones
-        const float inv_e = taught ? f_tau / sums[2] : 0.0f;
-        for (int k = tid; k <= K; k += THR) {
-            const int id = k < K ? sid[k] : (known ? target : -1);
-            if (id < 0)
-                continue;
-            float off = 0.0f; // of all entries that name this symbol; the first of them writes
-            bool first = true;
-            for (int j = 0; j < a.K4; j += 4) {
-                const int4 s = *reinterpret_cast<const int4 *>(sid + j);
-                const float4 e = *reinterpret_cast<const float4 *>(se + j);
-                off += s.x == id ? e.x : 0.0f;
-                off += s.y == id ? e.y : 0.0f;
-                off += s.z == id ? e.z : 0.0f;
-                off += s.w == id ? e.w : 0.0f;
-                first = first && !((s.x == id && j < k) || (s.y == id && j + 1 < k) || (s.z == id && j + 2 < k) || (s.w == id && j + 3 < k));
-            }
-            if (first)
-                dz[id] = from_f<TG>(both(k < K ? sz[k] : z_target) - (id == target ? f : 0.0f) - off * inv_e);
-        }
+        for (int i = 0; i < 2; i++)
+            if (late[i])
+                *late[i] = from_f<TG>(late_value[i]);
     }
+    if (!ok) // copies in flight may land before the CTA leaves
+        for (int i = 0; i < a.slots; i++)
+            tc::mbar_wait(bar0 + 8 * i, phase, &abort_s, &flag, 82, tc::DRAIN_TRIES);
 }
 
 } // namespace distill
