@@ -30,9 +30,7 @@ static void lin_parts(const nncu_linear_attn_shape *s, int roles, int *n_seg, in
 {
     const long long ctas = (long long)s->n_streams * s->n_head * roles;
     const int chunk = s->dtype_bf16 ? lin::TC : lin::FC, chunks = ceil_div(s->seg_len, chunk);
-    long long want = SMS;
-    if (getenv("LIN_WANT")) want = atoi(getenv("LIN_WANT"));
-    int n = (int)std::min<long long>(std::max<long long>(want / ctas, 1), std::max(chunks / 4, 1));
+    const int n = (int)std::min<long long>(std::max<long long>(SMS / ctas, 1), std::max(chunks / 4, 1));
     const int each = ceil_div(chunks, n);
     *seg = each * chunk;
     *n_seg = ceil_div(chunks, each);

@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
 // 16 r .. 16 r + 15 of a chunk and 32 columns of c, the cg-th; of the state it owns the same columns of rows 16 r ..
 // (and 16 (r + 4) .. of 128) in fp32 accumulators.  The results need all of the state: it goes through shared memory in
 // bf16, one rounding, as the pair weights P have one; products of a decayed b with c, which the state adds up, are kept to
-// 24 bits by three bf16 terms of the decayed value, so that the state is an fp32 sum of fp32 products.
+// 24 bits by three bf16 terms of the decayed value, so that the state is an fp32 sum of fp32 products.  Pair weights and
+// terms are the same for the CG warps of the same rows: each computes every CG-th and they meet at a barrier of their own.
 //
 // Tiles come by TMA, 64 tokens x 64 (32) values of a head a copy, from a map of (value, head, stream, token): what lies beyond
 // a head's values or the sequence arrives as zeros.  One thread asks for the next chunk's under the present chunk (copies
@@ -270,8 +271,10 @@ struct __align__(64) MmaArgs {
 
 template <int DA, int DC> struct MmaSmem {
     static constexpr int TA = TC * DA * 2, TB = TC * DC * 2, LC = DC + 8; // tiles; pitch of the state, rows four banks on
-    static constexpr int A = 0, B = A + 2 * TA, C = B + 2 * TA, S = C + 2 * TB, W = S + 2 * DA * LC * 2, BAR = W + (2 * TC + 8) * 4,
-                         BYTES = BAR + 16 + 1024; // the tiles begin at a multiple of 1024
+    static constexpr int MT = DA > 64 ? DA / 64 : 1;
+    static constexpr int XP = 4 * 4 * 512, XS = 4 * 4 * MT * 3 * 512; // what warps of the same rows hand one another
+    static constexpr int A = 0, B = A + 2 * TA, C = B + 2 * TA, S = C + 2 * TB, P = S + 2 * DA * LC * 2, SP = P + XP, W = SP + XS,
+                         BAR = W + (2 * TC + 8) * 4, BYTES = BAR + 16 + 1024; // the tiles begin at a multiple of 1024
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int h, int b, int t)
@@ -317,7 +320,7 @@ template <int DA, int DC, bool STATES>
 __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kernel(const __grid_constant__ MmaArgs args)
 {
     using SM = MmaSmem<DA, DC>;
-    constexpr int LC = SM::LC, NT = 4, MT = DA > 64 ? DA / 64 : 1, KS = DA / 16, THR = 4 * DC;
+    constexpr int LC = SM::LC, NT = 4, MT = SM::MT, KS = DA / 16, THR = 4 * DC, CG = DC / 32;
     extern __shared__ __align__(16) unsigned char smraw[];
     __shared__ int abort_s, flag;
     unsigned char *sm = smraw + ((1024u - (fa::smem_addr(smraw) & 1023u)) & 1023u);
@@ -418,6 +421,8 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     const uint32_t bt_at = base + SM::B + tile_at<DA>(row_of(lrow), 2 * r % (DA / 8) + lmid); // transposed: values 16 r
     const uint32_t c_at = base + SM::C + tile_at<DC>(row_of(l15), 4 * cg + lhi);           // transposed: rows 0 .. 15 of c
     const uint32_t s_at = base + SM::S + (l15 * LC + 32 * cg + lhi * 8) * 2;
+    uint4 *pairs = reinterpret_cast<uint4 *>(sm + SM::P) + r * 4 * 32 + lane;                  // fragments of this warp's rows
+    uint4 *terms = reinterpret_cast<uint4 *>(sm + SM::SP) + r * 4 * MT * 3 * 32 + lane;
     if (p.n_seg > 1) {
         if (STATES) {
             if (g == 0) // the state before the first token is kept: s_end may lie where it lies
@@ -471,32 +476,18 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             fetch(k + 1);
         const uint32_t At = a_at + buf * SM::TA, Bt = b_at + buf * SM::TA, Tt = bt_at + buf * SM::TA, Ct = c_at + buf * SM::TB,
                        St = s_at + buf * DA * LC * 2;
+        const bool carries = has_state && (STATES || !last || q.s_end); // the state behind the chunk is of use
+        const float *wt = wts + (last ? TC : 0);
+        float o[NT][4];
         if (!STATES) {
-            float o[NT][4];
-#pragma unroll
-            for (int x = 0; x < NT; x++)
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    o[x][c] = 0.0f;
+            // pair weights of every CG-th sixteen keys, for all warps of these rows
             uint32_t aq[KS][4];
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
+            for (int ks = 0; ks < KS; ks++)
                 ldsm4_at(aq[ks], (At ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128));
 #pragma unroll
-                for (int x = 0; x < NT; x += 2) {
-                    uint32_t f[4];
-                    ldsm4t_at(f, St + (ks * 16 * LC + x * 8) * 2);
-                    fa::mma(o[x], aq[ks], f[0], f[1]);
-                    fa::mma(o[x + 1], aq[ks], f[2], f[3]);
-                }
-            }
-#pragma unroll
-            for (int x = 0; x < NT; x++) {
-                o[x][0] *= f_a; o[x][1] *= f_a;
-                o[x][2] *= f_b; o[x][3] *= f_b;
-            }
-#pragma unroll
-            for (int pc = 0; pc < 4; pc++) {
+            for (int i = 0; i < 4 / CG; i++) {
+                const int pc = cg + i * CG;
                 if (pc > r)
                     break;
                 float w[2][4] = {};
@@ -521,16 +512,92 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                         for (int c = 0; c < 4; c++)
                             w[x][c] *= f * apart[(c >> 1) - x + 1][c & 1];
                 }
-                const uint32_t pf[4] = {fa::pack2(w[0][0], w[0][1]), fa::pack2(w[0][2], w[0][3]), fa::pack2(w[1][0], w[1][1]),
-                                        fa::pack2(w[1][2], w[1][3])};
+                pairs[pc * 32] = make_uint4(fa::pack2(w[0][0], w[0][1]), fa::pack2(w[0][2], w[0][3]), fa::pack2(w[1][0], w[1][1]),
+                                            fa::pack2(w[1][2], w[1][3]));
+            }
+            // what the state gives
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    o[x][c] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                 for (int x = 0; x < NT; x += 2) {
                     uint32_t f[4];
-                    ldsm4t_at(f, (Ct ^ (x << 4)) + pc * step_c);
-                    fa::mma(o[x], pf, f[0], f[1]);
-                    fa::mma(o[x + 1], pf, f[2], f[3]);
+                    ldsm4t_at(f, St + (ks * 16 * LC + x * 8) * 2);
+                    fa::mma(o[x], aq[ks], f[0], f[1]);
+                    fa::mma(o[x + 1], aq[ks], f[2], f[3]);
+                }
+#pragma unroll
+            for (int x = 0; x < NT; x++) {
+                o[x][0] *= f_a; o[x][1] *= f_a;
+                o[x][2] *= f_b; o[x][3] *= f_b;
+            }
+        }
+        // decayed values of every CG-th sixteen tokens, in three terms
+        if (carries) {
+#pragma unroll
+            for (int i = 0; i < 4 / CG; i++) {
+                const int ks = cg + i * CG;
+                const float2 w0 = *reinterpret_cast<const float2 *>(wt + ks * 16 + 2 * t), w8 = *reinterpret_cast<const float2 *>(wt + ks * 16 + 8 + 2 * t);
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    uint32_t f[4], hi[4], mid[4], lo[4];
+                    ldsm4t_at(f, Tt + m * (TC * 128) + ks * step_a);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        split3(f[e], e < 2 ? w0.x : w8.x, e < 2 ? w0.y : w8.y, hi[e], mid[e], lo[e]);
+                    uint4 *to = terms + (ks * MT + m) * 96;
+                    to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    to[32] = make_uint4(mid[0], mid[1], mid[2], mid[3]);
+                    to[64] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
+            const float l_n = last ? l_last : l_full;
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        s[m][x][c] *= l_n;
+        }
+        if constexpr (CG > 1)
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + r), "n"(32 * CG) : "memory"); // the warps of these rows
+        else
+            __syncwarp();
+        // the third term where a state is a result; 17 bits are more than the roundings behind them keep
+        const bool third = q.s_end != nullptr;
+#pragma unroll
+        for (int ks = 0; ks < TC / 16; ks++) {
+            uint32_t f[NT / 2][4];
+#pragma unroll
+            for (int x = 0; x < NT; x += 2)
+                ldsm4t_at(f[x / 2], (Ct ^ (x << 4)) + ks * step_c);
+            if (!STATES && ks <= r) {
+                const uint4 u = pairs[ks * 32];
+                const uint32_t pf[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+                    fa::mma(o[x], pf, f[x / 2][x % 2 * 2], f[x / 2][x % 2 * 2 + 1]);
+            }
+            if (carries) {
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int term = 0; term < 3; term++)
+                        if (term < 2 || third) {
+                            const uint4 u = terms[(ks * MT + m) * 96 + term * 32];
+                            const uint32_t bf[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int x = 0; x < NT; x++)
+                                fa::mma(s[m][x], bf, f[x / 2][x % 2 * 2], f[x / 2][x % 2 * 2 + 1]);
+                        }
+            }
+        }
+        if (!STATES) {
             if (!ok)
 #pragma unroll
                 for (int x = 0; x < NT; x++)
@@ -547,50 +614,6 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                 fa::quad_transpose(v, t);
                 if (i < n && 32 * cg + 8 * t < q.dc)
                     *reinterpret_cast<uint4 *>(to + 8 * t) = make_uint4(v[0], v[1], v[2], v[3]);
-            }
-        }
-        if (last && !STATES && !q.s_end)
-            break;
-        // the state behind the chunk
-        const float l_n = last ? l_last : l_full, *wt = wts + (last ? TC : 0);
-        // the third term where a state is a result; 17 bits are more than the roundings behind them keep
-        const bool third = q.s_end != nullptr;
-        if (has_state) {
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int x = 0; x < NT; x++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        s[m][x][c] *= l_n;
-#pragma unroll
-            for (int ks = 0; ks < TC / 16; ks++) {
-                const float2 w0 = *reinterpret_cast<const float2 *>(wt + ks * 16 + 2 * t), w8 = *reinterpret_cast<const float2 *>(wt + ks * 16 + 8 + 2 * t);
-                uint32_t hi[MT][4], mid[MT][4], lo[MT][4];
-#pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    uint32_t f[4];
-                    ldsm4t_at(f, Tt + m * (TC * 128) + ks * step_a);
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        split3(f[e], e < 2 ? w0.x : w8.x, e < 2 ? w0.y : w8.y, hi[m][e], mid[m][e], lo[m][e]);
-                }
-#pragma unroll
-                for (int x = 0; x < NT; x += 2) {
-                    uint32_t f[4];
-                    ldsm4t_at(f, (Ct ^ (x << 4)) + ks * step_c);
-#pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        fa::mma(s[m][x], hi[m], f[0], f[1]);
-                        fa::mma(s[m][x + 1], hi[m], f[2], f[3]);
-                        fa::mma(s[m][x], mid[m], f[0], f[1]);
-                        fa::mma(s[m][x + 1], mid[m], f[2], f[3]);
-                        if (third) {
-                            fa::mma(s[m][x], lo[m], f[0], f[1]);
-                            fa::mma(s[m][x + 1], lo[m], f[2], f[3]);
-                        }
-                    }
-                }
             }
         }
         if (!last)
