@@ -101,11 +101,11 @@ template <typename T, bool STATES> static int lin_core(const lin::Args &a, int r
     return NNCU_OK;
 }
 
-template <int DA, int DC, bool STATES> static int lin_mma_launch(const lin::MmaArgs &m, int roles, cudaStream_t st)
+template <int DA, int DC, bool STATES, bool TMA> static int lin_mma_launch(const lin::MmaArgs &m, int roles, cudaStream_t st)
 {
     static DeviceOnce once;
-    NNCU_TRY(smem_limit(once, lin::mma_kernel<DA, DC, STATES>, lin::MmaSmem<DA, DC>::BYTES));
-    CUDA_TRY(launch_k(lin::mma_kernel<DA, DC, STATES>, dim3(m.p.B * m.p.H, STATES ? m.p.n_seg - 1 : m.p.n_seg, roles), dim3(4 * DC),
+    NNCU_TRY(smem_limit(once, lin::mma_kernel<DA, DC, STATES, TMA>, lin::MmaSmem<DA, DC>::BYTES));
+    CUDA_TRY(launch_k(lin::mma_kernel<DA, DC, STATES, TMA>, dim3(m.p.B * m.p.H, STATES ? m.p.n_seg - 1 : m.p.n_seg, roles), dim3(4 * DC),
                       lin::MmaSmem<DA, DC>::BYTES, st, m));
     KERNEL_CHECK();
     return NNCU_OK;
@@ -130,6 +130,8 @@ template <int DA, int DC> static int lin_mma_sized(const lin::Args &a, int roles
 {
     lin::MmaArgs m;
     m.p = a;
+    if (a.T <= lin::TC)
+        return lin_mma_launch<DA, DC, false, false>(m, roles, st);
     for (int i = 0; i < roles; i++) {
         const lin::Role &q = a.role[i];
         NNCU_TRY(lin_map(a, q.a, q.lda, q.da, DA, &m.map[i][0]));
@@ -137,8 +139,8 @@ template <int DA, int DC> static int lin_mma_sized(const lin::Args &a, int roles
         NNCU_TRY(lin_map(a, q.c, q.ldc, q.dc, DC, &m.map[i][2]));
     }
     if (a.n_seg > 1)
-        NNCU_TRY((lin_mma_launch<DA, DC, true>(m, roles, st)));
-    return lin_mma_launch<DA, DC, false>(m, roles, st);
+        NNCU_TRY((lin_mma_launch<DA, DC, true, true>(m, roles, st)));
+    return lin_mma_launch<DA, DC, false, true>(m, roles, st);
 }
 
 // head sizes go up to the next of 32, 64 and 128, zeros beyond their own
@@ -243,7 +245,8 @@ int nncu_linear_attention_backward(const nncu_linear_attn_shape *s, const void *
     ChainScope chain;
     cudaStream_t st = (cudaStream_t)cuda_stream;
     lin::Args all = lin_args(s, 3, decay_host, len, workspace);
-    lin::Role &rq = all.role[0], &rk = all.role[1], &rv = all.role[2];
+    // the longest first: dv carries the third term
+    lin::Role &rv = all.role[0], &rq = all.role[1], &rk = all.role[2];
     rq.a = dout; rq.lda = lo; rq.b = v; rq.ldb = lv; rq.c = k; rq.ldc = lk; rq.o = dq; rq.ldo = lq;
     rk.a = v; rk.lda = lv; rk.b = dout; rk.ldb = lo; rk.c = q; rk.ldc = lq; rk.o = dk; rk.ldo = lk;
     rv.a = k; rv.lda = lk; rv.b = q; rv.ldb = lq; rv.c = dout; rv.ldc = lo; rv.o = dv; rv.ldo = lv;
@@ -261,8 +264,10 @@ int nncu_linear_attention_backward(const nncu_linear_attn_shape *s, const void *
     const size_t states = (size_t)s->n_streams * wk * s->d_value;
     if (s->d_key == s->d_value && !(from && to && from < to + states && to < from + states))
         return lin_any(s, all, 3, st);
-    NNCU_TRY(lin_any(s, all, 2, st));
-    all.role[0] = rv;
+    lin::Args two = all;
+    two.role[0] = rq;
+    two.role[1] = rk;
+    NNCU_TRY(lin_any(s, two, 2, st));
     return lin_any(s, all, 1, st);
 }
 

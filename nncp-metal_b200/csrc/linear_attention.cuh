@@ -305,6 +305,23 @@ template <int D> __device__ __forceinline__ uint32_t tile_at(int r, int c)
 }
 template <int D> struct Rows16 { static constexpr int BYTES = D == 32 ? 16 * 64 : 16 * 128; };
 
+// 64 tokens of one head from time t0 on as TMA lays them, zeros outside [0, n) and behind value d.  src: the head's first row
+template <int D, int THR> __device__ __forceinline__ void tile_copy(uint32_t dst, const bf16 *src, long long pitch, int d, int t0, int n)
+{
+    constexpr int CPR = D / 8, ROWS = THR / CPR; // pieces of a row, rows at a time: a multiple of eight, so that pieces keep their order
+    static_assert(ROWS % 8 == 0, "");
+    const int r = threadIdx.x / CPR, x = threadIdx.x % CPR;
+    const bf16 *from = src + (t0 + r) * pitch + x * 8;
+    dst += tile_at<D>(r, x);
+#pragma unroll
+    for (int i = 0; i < (TC + ROWS - 1) / ROWS; i++, from += ROWS * pitch, dst += ROWS * (D == 32 ? 64 : 128)) {
+        const int t = t0 + r + i * ROWS;
+        const bool in = t >= 0 && t < n && x * 8 < d;
+        if (TC % ROWS == 0 || r < TC)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(in ? from : src), "r"(in ? 16 : 0) : "memory");
+    }
+}
+
 // a pair of bf16 values times their weights as three bf16 terms that add up to 24 bits of them
 __device__ __forceinline__ void split3(uint32_t v, float w0, float w1, uint32_t &hi, uint32_t &mid, uint32_t &lo)
 {
@@ -316,7 +333,9 @@ __device__ __forceinline__ void split3(uint32_t v, float w0, float w1, uint32_t 
     lo = fa::pack2(x - __uint_as_float(mid << 16), y - __uint_as_float(mid & 0xffff0000u));
 }
 
-template <int DA, int DC, bool STATES>
+// TMA: tiles come by tensor maps; otherwise (streams of one chunk, where there is nothing to fetch ahead and twelve maps
+// for a step cost the host 6 us) all threads copy 16 bytes at a time.
+template <int DA, int DC, bool STATES, bool TMA>
 __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kernel(const __grid_constant__ MmaArgs args)
 {
     using SM = MmaSmem<DA, DC>;
@@ -336,21 +355,29 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     const size_t pair = blockIdx.x;
     const int g = blockIdx.y, b = (int)(pair / p.H), h = (int)(pair % p.H);
     const float rate = p.rate[h];
-    if (tid == 0) {
-        abort_s = 0;
-        tc::mbar_init(bar, 1);
-        tc::mbar_init(bar + 8, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if constexpr (TMA) {
+        if (tid == 0) {
+            abort_s = 0;
+            tc::mbar_init(bar, 1);
+            tc::mbar_init(bar + 8, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncthreads();
     }
-    __syncthreads();
     pdl_wait(); // no early trigger: successors resident beside these CTAs cost more than their launch
     const Rows rows(p, q, b);
     const size_t nn = (size_t)q.da * q.dc;
     const int begin = g * p.seg, end = min(rows.n, begin + p.seg), total = max(end - begin, 0), chunks = (total + TC - 1) / TC;
     bool ok = true; // this thread's waits; behind one that ran out results are NaN and nothing more is asked for
     auto fetch = [&](int k) {
-        if (tid == 0 && ok) {
-            const int u0 = begin + k * TC, buf = k & 1, t0 = q.reverse ? rows.n - TC - u0 : u0;
+        const int u0 = begin + k * TC, buf = k & 1, t0 = q.reverse ? rows.n - TC - u0 : u0;
+        if constexpr (!TMA) {
+            if (!STATES)
+                tile_copy<DA, THR>(base + SM::A + buf * SM::TA, reinterpret_cast<const bf16 *>(q.a) + b * q.lda + h * q.da, p.B * q.lda, q.da, t0, rows.n);
+            tile_copy<DA, THR>(base + SM::B + buf * SM::TA, reinterpret_cast<const bf16 *>(q.b) + b * q.ldb + h * q.da, p.B * q.ldb, q.da, t0, rows.n);
+            tile_copy<DC, THR>(base + SM::C + buf * SM::TB, reinterpret_cast<const bf16 *>(q.c) + b * q.ldc + h * q.dc, p.B * q.ldc, q.dc, t0, rows.n);
+            fa::cp_commit();
+        } else if (tid == 0 && ok) {
             const uint32_t full = bar + 8 * buf;
             tc::mbar_expect_tx(full, (STATES ? 1 : 2) * SM::TA + SM::TB);
 #pragma unroll
@@ -377,18 +404,28 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int n = 0; n < NT; n++)
+            s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.0f;
+    if (first && q.s0) {
+        const float *from = q.s0 + pair * nn + (q.s0_t ? (32 * cg + 2 * t) * q.da + 16 * r + gq : (16 * r + gq) * q.dc + 32 * cg + 2 * t);
+        const int row = q.s0_t ? 1 : q.dc, col = q.s0_t ? q.da : 1;
 #pragma unroll
-            for (int c = 0; c < 4; c += 2) {
-                const int x = 16 * (r + 4 * m) + gq + 4 * c, y = 32 * cg + 8 * n + 2 * t;
-                float2 f = make_float2(0.0f, 0.0f);
-                if (first && q.s0 && x < q.da && y < q.dc) {
-                    const float *from = q.s0 + pair * nn;
-                    f = q.s0_t ? make_float2(from[y * q.da + x], from[(y + 1) * q.da + x])
-                               : *reinterpret_cast<const float2 *>(from + x * q.dc + y);
-                }
-                s[m][n][c] = f.x;
-                s[m][n][c + 1] = f.y;
-            }
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c += 2)
+                    if (16 * (r + 4 * m) + gq + 4 * c < q.da && 32 * cg + 8 * n + 2 * t < q.dc) {
+                        const float *at = from + (64 * m + 4 * c) * row + 8 * n * col;
+                        if (q.s0_t) {
+                            s[m][n][c] = at[0];
+                            s[m][n][c + 1] = at[col];
+                        } else {
+                            const float2 f = *reinterpret_cast<const float2 *>(at);
+                            s[m][n][c] = f.x;
+                            s[m][n][c + 1] = f.y;
+                        }
+                    }
+    }
     const int n_last = total - (chunks - 1) * TC;
     const float l_seg = power(rate, p.seg), l_full = power(rate, TC), l_last = power(rate, n_last);
     if (tid < TC) {
@@ -464,8 +501,11 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     for (int k = 0; k < chunks; k++) {
         const int buf = k & 1, u0 = begin + k * TC, n = min(TC, end - u0);
         const bool last = k == chunks - 1;
-        ok = ok && tc::mbar_wait(bar + 8 * buf, (k >> 1) & 1, &abort_s, &flag, 81);
-        if (n < TC && p.len && !q.reverse) // rows behind the stream's end hold anything: the tile's are zeros
+        if constexpr (TMA)
+            ok = ok && tc::mbar_wait(bar + 8 * buf, (k >> 1) & 1, &abort_s, &flag, 81);
+        else
+            fa::cp_wait<0>();
+        if (TMA && n < TC && p.len && !q.reverse) // rows behind the stream's end hold anything: the tile's are zeros
             for (int i = tid; i < (TC - n) * (DA / 8 + DC / 8); i += THR) {
                 const int row = n + i / (DA / 8 + DC / 8), x = i % (DA / 8 + DC / 8);
                 unsigned char *to = sm + (x < DA / 8 ? SM::B + buf * SM::TA + tile_at<DA>(row, x) : SM::C + buf * SM::TB + tile_at<DC>(row, x - DA / 8));
@@ -625,7 +665,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
             for (int x = 0; x < NT; x++)
                 s[m][x][0] = s[m][x][1] = s[m][x][2] = s[m][x][3] = NAN;
-        for (int x = 0; x < 2; x++) // copies in flight may land before the CTA leaves
+        for (int x = 0; x < 2 && TMA; x++) // copies in flight may land before the CTA leaves
             tc::mbar_wait(bar + 8 * x, 0, &abort_s, &flag, 81, tc::DRAIN_TRIES);
     }
     if (STATES) {

@@ -52,8 +52,11 @@ static qkn::Args qk_args(const nncu_qk_norm_shape *s, const void *q, const void 
     a.rows_per = qk_rows_per(s);
     for (int i = 0; i < 2; i++)
         a.inverse[i] = a.heads[i] > 1 ? (uint32_t)(((1ull << 32) + a.heads[i] - 1) / a.heads[i]) : 0;
-    for (int i = 0; i < s->d_rot / 2; i++)
-        a.turns[i] = pow((double)s->rope_base, -2.0 * i / s->d_rot) / 6.283185307179586476925;
+    // pair by pair in 64 bits behind the point: one power for all of them
+    const long double step = s->d_rot ? powl((long double)s->rope_base, -2.0L / s->d_rot) : 1.0L;
+    long double turn = 1.0L / 6.283185307179586476925L;
+    for (int i = 0; i < s->d_rot / 2; i++, turn *= step)
+        a.turns[i] = (double)turn;
     return a;
 }
 
