@@ -21,20 +21,20 @@ static int qk_check(const nncu_qk_norm_shape *s)
     return NNCU_OK;
 }
 
-// Rows that a CTA takes at a time: heads for its eight warps at least (a lane holds eight pairs or so), and eight where
-// that leaves two CTAs an SM.
+// Rows that a CTA takes at a time: four rounds of heads for its eight warps (a lane holds eight pairs or so), or as many as
+// leave two CTAs an SM.
 static int qk_rows_per(const nncu_qk_norm_shape *s)
 {
-    const int heads = s->n_head + s->n_head_k, per_warp = std::max(1, 32 * 16 / s->d_key);
+    const int per_warp = std::max(1, 32 * 16 / s->d_key), kinds = s->n_head_k ? 2 : 1;
     int n = 1;
-    while (n < 8 && (n * heads < 8 * per_warp || ceil_div(s->n_rows, 2 * n) >= 2 * SMS))
+    while (n < qkn::ROWS_MAX && n * s->n_head < 32 * per_warp && (n * s->n_head < 8 * per_warp || (long long)ceil_div(s->n_rows, 2 * n) * kinds >= 2 * SMS))
         n *= 2;
     return n;
 }
 static int qk_blocks(const nncu_qk_norm_shape *s, bool back)
 {
-    const int blocks = ceil_div(s->n_rows, qk_rows_per(s));
-    return back ? std::min(blocks, 2 * SMS) : blocks; // each leaves a partial sum of dgain
+    const int blocks = ceil_div(s->n_rows, qk_rows_per(s)), kinds = s->n_head_k ? 2 : 1;
+    return std::min(blocks, (back ? 2 : 8) * SMS / kinds); // backward: each leaves a partial sum of dgain
 }
 
 static qkn::Args qk_args(const nncu_qk_norm_shape *s, const void *q, const void *k, const float *gain_q, const float *gain_k, const int32_t *pos)
@@ -45,10 +45,10 @@ static qkn::Args qk_args(const nncu_qk_norm_shape *s, const void *q, const void 
     a.gain[0] = gain_q; a.gain[1] = gain_k;
     a.pos = pos;
     const long long wq = (long long)s->n_head * s->d_key, wk = (long long)s->n_head_k * s->d_key;
-    a.ldx[0] = s->ld_q ? s->ld_q : wq; a.ldx[1] = s->ld_k ? s->ld_k : wk;
-    a.ldy[0] = s->ld_q_out ? s->ld_q_out : wq; a.ldy[1] = s->ld_k_out ? s->ld_k_out : wk;
+    a.ldx[0] = s->ld_q ? s->ld_q : (int)wq; a.ldx[1] = s->ld_k ? s->ld_k : (int)wk;
+    a.ldy[0] = s->ld_q_out ? s->ld_q_out : (int)wq; a.ldy[1] = s->ld_k_out ? s->ld_k_out : (int)wk;
     a.heads[0] = s->n_head; a.heads[1] = s->n_head_k;
-    a.N = s->n_rows; a.d = s->d_key; a.rot = s->d_rot; a.adjacent = s->adjacent != 0; a.eps = s->eps;
+    a.N = s->n_rows; a.d = s->d_key; a.rot = s->d_rot; a.eps = s->eps;
     a.rows_per = qk_rows_per(s);
     for (int i = 0; i < 2; i++)
         a.inverse[i] = a.heads[i] > 1 ? (uint32_t)(((1ull << 32) + a.heads[i] - 1) / a.heads[i]) : 0;
@@ -65,8 +65,12 @@ template <typename T, int W, int NG, bool BACK> static int qk_launch(const nncu_
     a.lanes = 1;
     while (a.lanes * W * NG < a.d / 2)
         a.lanes *= 2;
-    const size_t smem = sizeof(float) * ((size_t)a.rows_per * a.rot + (BACK ? 10 : 2) * a.d);
-    CUDA_TRY(launch_k(qkn::kernel<T, W, NG, BACK>, dim3(qk_blocks(s, BACK)), dim3(256), smem, st, a));
+    const size_t smem = sizeof(float) * (size_t)(a.rows_per + (BACK ? 9 : 1)) * a.d;
+    const dim3 grid(qk_blocks(s, BACK), s->n_head_k ? 2 : 1);
+    if (s->adjacent)
+        CUDA_TRY(launch_k(qkn::kernel<T, W, NG, true, BACK>, grid, dim3(256), smem, st, a));
+    else
+        CUDA_TRY(launch_k(qkn::kernel<T, W, NG, false, BACK>, grid, dim3(256), smem, st, a));
     KERNEL_CHECK();
     return NNCU_OK;
 }
