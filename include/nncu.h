@@ -194,7 +194,19 @@ int nncu_eval_gradient_dev(nncu_model *m, const int32_t *expected_dev);
  */
 int nncu_eval_gradient_update(nncu_model *m, const int32_t *expected_host, float *loss_out);
 int nncu_eval_gradient_update_dev(nncu_model *m, const int32_t *expected_dev);
-/* Reads the loss of the last nncu_eval_gradient / _dev.  The loss is copied to the host right
+/*
+ * The same with a student's loss (no counterpart in the reference): a teacher's n_top entries a row,
+ * top_ids_host int32 and top_logits_host fp32 [T][B][n_top], with q the softmax of the logits of the entries
+ * whose symbol is inside the alphabet:
+ *   loss = sum over rows of (1 - teacher_share) ln p[target] + teacher_share sum_k q_k (ln p[id_k] - ln q_k)
+ * A row without such an entry learns from its target alone.  Losses of one forward pass may follow one another.  The first
+ * call, and one with another n_top, allocates room for the entries and waits for the stream; so does every
+ * call for its copies.
+ */
+int nncu_eval_gradient_distill(nncu_model *m, const int32_t *expected_host, int n_top,
+                               const int32_t *top_ids_host, const float *top_logits_host,
+                               float teacher_share, float *loss_out);
+/* Reads the loss of the last nncu_eval_gradient / _dev / _distill.  The loss is copied to the host right
    behind the backward pass, and this call waits for that copy only: work the host has queued
    since (nncu_update, the next nncu_eval) keeps running. */
 int nncu_read_loss(nncu_model *m, float *loss_out);

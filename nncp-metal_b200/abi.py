@@ -115,6 +115,7 @@ PROTOTYPES = {
     "nncu_eval_gradient_dev": (_i, [_vp, _vp]),
     "nncu_eval_gradient_update": (_i, [_vp, _vp, C.POINTER(C.c_float)]),
     "nncu_eval_gradient_update_dev": (_i, [_vp, _vp]),
+    "nncu_eval_gradient_distill": (_i, [_vp, _vp, _i, _vp, _vp, C.c_float, _pf]),
     "nncu_read_loss": (_i, [_vp, _pf]),
     "nncu_update": (_i, [_vp]),
     "nncu_optimizer_step": (_i, [_vp]),

@@ -958,6 +958,85 @@ loss_fix_kernel(const float *__restrict__ probs, const int32_t *__restrict__ tar
     logp[r] = logf(pt);
 }
 
+// The gradient of the logits that a teacher's entries name, put back to the p * scale of the forward pass: what
+// loss_top_kernel has changed, before another loss of the same forward pass.
+template <typename T>
+__global__ void top_undo_kernel(const float *__restrict__ probs, const int32_t *__restrict__ top_ids, int K, T *__restrict__ dz, size_t n, int V,
+                                float scale)
+{
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    pdl_wait();
+    if (i >= n)
+        return;
+    const int id = top_ids[i];
+    if (id >= 0 && id < V) {
+        const size_t at = i / K * V + id;
+        dz[at] = from_f<T>(probs[at] * scale);
+    }
+}
+
+// Behind loss_fix_kernel, whose loss and gradient are the target's alone: a row whose teacher names symbols
+// (top_logits, a softmax q over the entries inside the alphabet) gets
+//   logp = (1 - share) ln p[t] + share sum_k q_k (ln p[id_k] - ln q_k),  d = (p - (1 - share) 1_t - share sum_k q_k 1_{id_k}) scale
+// at t and the id_k; everywhere else d is p * scale already.  A warp a row.
+template <typename T>
+__global__ void __launch_bounds__(128)
+loss_top_kernel(const float *__restrict__ probs, const int32_t *__restrict__ targets, const int32_t *__restrict__ top_ids,
+                const float *__restrict__ top_logits, int K, float share, T *__restrict__ dz, float *__restrict__ logp, int rows, int V, float scale)
+{
+    const int r = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    pdl_wait();
+    if (r >= rows)
+        return;
+    const float *pr = probs + (size_t)r * V;
+    T *d = dz + (size_t)r * V;
+    const int32_t *ids = top_ids + (size_t)r * K;
+    const float *z = top_logits + (size_t)r * K;
+    auto there = [&](int k) { return ids[k] >= 0 && ids[k] < V; };
+    float most = -INFINITY;
+    for (int k = lane; k < K; k += 32)
+        if (there(k))
+            most = fmaxf(most, z[k]);
+    most = warp_max(most);
+    if (most == -INFINITY) // no teacher: the target alone
+        return;
+    float sum = 0.0f;
+    for (int k = lane; k < K; k += 32)
+        if (there(k))
+            sum += expf(z[k] - most);
+    sum = warp_sum(sum);
+    const float inv = 1.0f / sum, ln_sum = logf(sum);
+    int t = targets[r];
+    t = t < 0 ? 0 : (t >= V ? V - 1 : t);
+    float gain = 0.0f;
+    bool named = false; // the target, by an entry of this lane
+    for (int k = lane; k < K; k += 32) {
+        if (!there(k))
+            continue;
+        const int id = ids[k];
+        const float q = expf(z[k] - most) * inv, p = pr[id];
+        if (q > 0.0f)
+            gain += q * (logf(p) - (z[k] - most - ln_sum));
+        float of_id = 0.0f; // of all entries that name it; the first of them writes
+        bool first = true;
+        for (int j = 0; j < K; j++)
+            if (ids[j] == id) {
+                of_id += expf(z[j] - most) * inv;
+                first = first && j >= k;
+            }
+        named = named || id == t;
+        if (first)
+            d[id] = from_f<T>((p - (id == t ? 1.0f - share : 0.0f) - share * of_id) * scale);
+    }
+    gain = warp_sum(gain);
+    named = __any_sync(0xffffffffu, named);
+    if (lane == 0) {
+        logp[r] = (share < 1.0f ? (1.0f - share) * logp[r] : 0.0f) + (share > 0.0f ? share * gain : 0.0f);
+        if (!named)
+            d[t] = from_f<T>((pr[t] - (1.0f - share)) * scale);
+    }
+}
+
 __global__ void __launch_bounds__(256) loss_sum_kernel(const float *__restrict__ v, int n, float *__restrict__ out,
                                                        int *__restrict__ dz_fixed)
 {

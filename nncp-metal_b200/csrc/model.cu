@@ -25,6 +25,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <functional>
 #include <initializer_list>
 #include <string>
 #include <vector>
@@ -138,6 +139,9 @@ constexpr int SPLITK = 4, SPLITK_MIN_K = 8192; // split-K of the output head's d
 // three times: the main stream goes on with layer l - 1 while the side stream is still at layer l, and waits for it
 // only before layer l - 2 (side_release).
 constexpr int POOL = 4, POOLS = 3 * POOL;
+// passes that are captured into graphs: forward, backward, backward with the optimizer step, backward of a student's loss
+enum { GRAPH_FWD = 0, GRAPH_BWD = 1, GRAPH_BWD_UPD = 2, GRAPH_BWD_TOP = 3, N_GRAPH_KINDS = 4 };
+
 struct nncu_model {
     nncu_params p;
     int D, H, dk, HD, F, F1, T, B, M, L, V, TB, LB, Bt, nl;
@@ -154,7 +158,14 @@ struct nncu_model {
         cudaGraphExec_t exec;
         unsigned long long launches;
         int calls;
-    } graphs[3][2]; // [forward, backward, backward with the optimizer step][memory twin]
+    } graphs[N_GRAPH_KINDS][2]; // [kind][memory twin]
+    // a teacher's entries (nncu_eval_gradient_distill): [TB][top_most] symbols, then as many logits
+    int32_t *top_ids = nullptr;
+    int top_most = 0;
+    int top_now = 0;  // of the pass that is being queued; 0: no teacher
+    int top_left = 0; // those that the last loss of this forward pass has left in the logit gradient
+    float top_share = 0.0f;
+    float *top_logits() const { return reinterpret_cast<float *>(top_ids + (size_t)TB * top_most); }
     bool graphs_on;
     std::vector<StepGraph> step_graphs; // device decoder: one-symbol step + trees + decode, [t][memory twin]
     uint8_t *dec_payload = nullptr;     // the coded bytes on the device (nncu_decoder_begin)
@@ -566,7 +577,6 @@ static nncu_attn_shape attn_shape(nncu_model *m, int l, int t0, int t1)
 // copied into fixed staging buffers before the graph runs, and the two memory twins have
 // a graph each.  One-symbol steps, the optimizer (its learning rate is a launch argument) and
 // the timed-GEMM profiling pass stay eager.
-enum { GRAPH_FWD = 0, GRAPH_BWD = 1, GRAPH_BWD_UPD = 2, N_GRAPH_KINDS = 3 };
 
 template <typename F>
 static int run_graphed(nncu_model *m, nncu_model::StepGraph &g, F body)
@@ -941,6 +951,11 @@ static int backward(nncu_model *m)
     launch_k(loss_fix_kernel<AT>, dim3(ceil_div(TB, 256)), dim3(256), 0, m->st, (const float *)m->probs, (const int32_t *)m->tgt_dev,
              m->tgt_fixed, (const int *)m->dz_fixed, dz, m->logp, TB, V, sc);
     KERNEL_CHECK();
+    if (m->top_now) {
+        launch_k(loss_top_kernel<AT>, dim3(ceil_div(TB, 4)), dim3(128), 0, m->st, (const float *)m->probs, (const int32_t *)m->tgt_dev,
+                 (const int32_t *)m->top_ids, (const float *)m->top_logits(), m->top_now, m->top_share, dz, m->logp, TB, V, sc);
+        KERNEL_CHECK();
+    }
     launch_k(loss_sum_kernel, dim3(1), dim3(256), 0, m->st, (const float *)m->logp, TB, m->loss_dev, m->dz_fixed);
     KERNEL_CHECK();
     const AT *xf = (p.ln_flags & NNCU_LN_FINAL) ? atc<AT>(m->xf, 0) : atc<AT>(m->xlast, 0);
@@ -1320,7 +1335,7 @@ int nncu_destroy(nncu_model *m)
     cudaSetDevice(m->device);
     cudaStreamSynchronize(m->st);
     // graphs first: a captured ncclAllReduce keeps its communicator busy until the graph is gone
-    for (int k = 0; k < 3; k++)
+    for (int k = 0; k < N_GRAPH_KINDS; k++)
         for (int c = 0; c < 2; c++)
             if (m->graphs[k][c].exec)
                 cudaGraphExecDestroy(m->graphs[k][c].exec);
@@ -1329,6 +1344,7 @@ int nncu_destroy(nncu_model *m)
             cudaGraphExecDestroy(g.exec);
     if (m->ids_all) cudaFree(m->ids_all);
     if (m->dx_all) cudaFree(m->dx_all);
+    if (m->top_ids) cudaFree(m->top_ids);
     if (m->dec_payload) cudaFree(m->dec_payload);
     if (m->dec_state) cudaFree(m->dec_state);
     if (m->st3) cudaStreamSynchronize(m->st3);
@@ -1783,6 +1799,7 @@ static int eval_common(nncu_model *m, int output_index)
         return rc;
     m->steps_done = t1;
     m->have_forward = (t1 == m->T);
+    m->top_left = 0; // the pass has written the logit gradient anew
     return NNCU_OK;
 }
 
@@ -1875,7 +1892,8 @@ static bool sparse_embed_enabled()
     return on != 0;
 }
 
-static int gradient_common(nncu_model *m, bool fused = false)
+// top: brings a teacher's entries to the device
+static int gradient_common(nncu_model *m, bool fused = false, const std::function<int(nncu_model *)> &top = nullptr)
 {
     if (!fused && m->master_stale)
         return nncu_fail(NNCU_ERR_STATE, "the optimizer state is sharded over the ranks: nncu_comm_gather_master first");
@@ -1892,11 +1910,29 @@ static int gradient_common(nncu_model *m, bool fused = false)
     m->fuse_update = fused;
     m->shard_update = fused && m->comm && m->comm_ranks > 1 && shard_enabled();
     m->sparse_embed = fused && m->comm && m->comm_ranks > 1 && (m->shard_update || sparse_embed_enabled());
-    int rc = run_graphed(m, fused ? GRAPH_BWD_UPD : GRAPH_BWD,
+    // entries of a teacher that an earlier loss of this forward pass has left in the logit gradient
+    if (m->top_left) {
+        const size_t n = (size_t)m->TB * m->top_left;
+        const float sc = 1.0f / ((float)m->T * (float)m->Bt);
+        if (m->bf)
+            launch_k(top_undo_kernel<bf16>, dim3(ceil_div(n, 256)), dim3(256), 0, m->st, (const float *)m->probs, (const int32_t *)m->top_ids,
+                     m->top_left, (bf16 *)m->dz, n, m->V, sc);
+        else
+            launch_k(top_undo_kernel<float>, dim3(ceil_div(n, 256)), dim3(256), 0, m->st, (const float *)m->probs, (const int32_t *)m->top_ids,
+                     m->top_left, (float *)m->dz, n, m->V, sc);
+        KERNEL_CHECK();
+        m->top_left = 0;
+    }
+    if (top) { // behind what has read the entries before them
+        NNCU_TRY(top(m));
+        m->top_left = m->top_now;
+    }
+    int rc = run_graphed(m, top ? GRAPH_BWD_TOP : fused ? GRAPH_BWD_UPD : GRAPH_BWD,
                          [&]() { return m->bf ? backward<bf16>(m) : backward<float>(m); });
     if (m->shard_update)
         m->master_stale = true;
     m->fuse_update = false;
+    m->top_now = 0;
     m->shard_update = m->sparse_embed = false;
     if (rc == NNCU_OK && fused)
         rc = refresh_transposed(m);
@@ -1954,6 +1990,51 @@ int nncu_eval_gradient_dev(nncu_model *m, const int32_t *expected_dev)
     CUDA_TRY(cudaMemcpyAsync(m->tgt_dev, expected_dev, sizeof(int32_t) * m->TB, cudaMemcpyDeviceToDevice, m->st));
     NNCU_TRY(gradient_common(m));
     return queue_loss(m);
+}
+
+int nncu_eval_gradient_distill(nncu_model *m, const int32_t *expected_host, int n_top, const int32_t *top_ids_host,
+                               const float *top_logits_host, float teacher_share, float *loss_out)
+{
+    if (!m || !expected_host || !top_ids_host || !top_logits_host)
+        return nncu_fail(NNCU_ERR_INVALID, "null argument");
+    if (n_top < 1 || n_top > NNCU_DISTILL_TOP_MAX || !(teacher_share >= 0.0f && teacher_share <= 1.0f))
+        return nncu_fail(NNCU_ERR_INVALID, "distillation: 1 to %d entries and a share from 0 to 1", NNCU_DISTILL_TOP_MAX);
+    CUDA_TRY(cudaSetDevice(m->device));
+    if (!m->have_forward)
+        return nncu_fail(NNCU_ERR_STATE, "eval_gradient needs a complete forward pass first");
+    CUDA_TRY(cudaEventSynchronize(m->ev_tgt));
+    memcpy(m->tgt_pin, expected_host, sizeof(int32_t) * m->TB);
+    CUDA_TRY(cudaMemcpyAsync(m->tgt_dev, m->tgt_pin, sizeof(int32_t) * m->TB, cudaMemcpyHostToDevice, m->st));
+    CUDA_TRY(cudaEventRecord(m->ev_tgt, m->st));
+    const size_t n = (size_t)m->TB * n_top;
+    NNCU_TRY(gradient_common(m, false, [&](nncu_model *mm) -> int {
+        if (n_top != mm->top_most || teacher_share != mm->top_share) { // what a captured pass holds
+            CUDA_TRY(cudaStreamSynchronize(mm->st));                    // which nothing runs, and nothing reads the old entries
+            for (auto &g : mm->graphs[GRAPH_BWD_TOP]) {
+                if (g.exec)
+                    CUDA_TRY(cudaGraphExecDestroy(g.exec));
+                g = nncu_model::StepGraph{nullptr, 0, 0};
+            }
+            if (n_top != mm->top_most) {
+                if (mm->top_ids)
+                    CUDA_TRY(cudaFree(mm->top_ids));
+                mm->top_ids = nullptr;
+                mm->top_most = 0;
+                CUDA_TRY(cudaMalloc(&mm->top_ids, n * (sizeof(int32_t) + sizeof(float))));
+            }
+            mm->top_most = n_top;
+            mm->top_share = teacher_share;
+        }
+        CUDA_TRY(cudaMemcpyAsync(mm->top_ids, top_ids_host, n * sizeof(int32_t), cudaMemcpyHostToDevice, mm->st));
+        CUDA_TRY(cudaMemcpyAsync(mm->top_logits(), top_logits_host, n * sizeof(float), cudaMemcpyHostToDevice, mm->st));
+        CUDA_TRY(cudaStreamSynchronize(mm->st)); // the arrays are the caller's again
+        mm->top_now = n_top;
+        return NNCU_OK;
+    }));
+    NNCU_TRY(queue_loss(m));
+    if (loss_out)
+        return nncu_read_loss(m, loss_out);
+    return NNCU_OK;
 }
 
 int nncu_eval_gradient_update(nncu_model *m, const int32_t *expected_host, float *loss_out)
@@ -2449,6 +2530,7 @@ int nncu_decode_steps(nncu_model *m, int t0, int nt, const int32_t *ids_t0_host,
         m->steps_done = t + 1;
     }
     m->have_forward = (m->steps_done == m->T);
+    m->top_left = 0;
     CUDA_TRY(cudaEventSynchronize(m->ev_sym));
     CUDA_TRY(cudaMemcpyAsync(m->sym_pin, m->tgt_dev + (size_t)t0 * B, sizeof(int32_t) * (size_t)nt * B, cudaMemcpyDeviceToHost,
                              m->st));

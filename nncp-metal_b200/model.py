@@ -91,6 +91,15 @@ class TrfModel:
         self._ck(self.lib.nncu_eval_gradient(self.h, _ptr(t), C.byref(loss)))
         return loss.value
 
+    def eval_gradient_distill(self, targets, top_ids, top_logits, teacher_share):
+        """Backward pass of a student's loss: a teacher's likeliest symbols and their logits, [T, B, n_top] each."""
+        t = np.ascontiguousarray(targets, np.int32)
+        ids, top = np.ascontiguousarray(top_ids, np.int32), np.ascontiguousarray(top_logits, np.float32)
+        assert ids.shape == top.shape and ids.ndim == 3 and ids.shape[:2] == (self.T, self.B) and t.size == self.T * self.B
+        loss = C.c_float()
+        self._ck(self.lib.nncu_eval_gradient_distill(self.h, _ptr(t), ids.shape[2], _ptr(ids), _ptr(top), float(teacher_share), C.byref(loss)))
+        return loss.value
+
     def eval_gradient_dev(self, targets_dev_ptr):
         self._ck(self.lib.nncu_eval_gradient_dev(self.h, _vp(targets_dev_ptr)))
 

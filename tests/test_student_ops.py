@@ -760,3 +760,63 @@ def test_two_streams_at_once(pkg):
     for (b, *_), w in zip((one, two), want):
         for n, x in b.items():
             assert torch.equal(x, w[n]), n
+
+
+# ---------------------------------------------------------------- the model's own path
+
+@gpu
+@pytest.mark.parametrize("bf16,V", [(0, 256), (0, 1024), (1, 300)])
+def test_model_learns_from_a_teacher(pkg, bf16, V):
+    """The gradient is linear in what a row is to predict: a teacher with the same q in every row gives the weighted sum of the
+    gradients of its symbols as targets, (1 - share) of the target's beside it; the loss is the weighted sum of theirs
+    less share sum q ln q a row.  fp32: sums in another order (2^-24 times some thousand terms); bf16: a rounding of every
+    operand, 2^-8, in each of two layers."""
+    np = pytest.importorskip("numpy")
+    kw = dict(n_layer=2, d_model=64, n_head=2, d_key=32, d_inner=128, d_pos=24, mem_len=16, seg_len=16, n_streams=4, n_symbols=V,
+              use_bf16=bf16, init_range=0.2)
+    T, B, K, share = 16, 4, 3, 0.6
+    rng = np.random.default_rng(V)
+    m = pkg.TrfModel(pkg.abi.make_params(**kw))
+    m.reset()
+    m._ck(m.lib.nncu_own_stream(m.h))
+    logits = np.array([0.3, -1.0, 0.8], np.float32)
+    q = np.exp(logits.astype(np.float64)); q /= q.sum()
+    tol = 4e-2 if bf16 else 2e-4
+    for step in range(4):  # eager, captured, replayed, both memory twins
+        ids_in = rng.integers(0, V, (T, B)).astype(np.int32)
+        tg = rng.integers(0, V, (T, B)).astype(np.int32)
+        top = np.stack([rng.permutation(V)[:K] for _ in range(T * B)]).reshape(T, B, K).astype(np.int32)
+        top[0, 0] = tg[0, 0]            # the target three times
+        top[1, 1, 1] = top[1, 1, 0]     # a symbol twice
+        rows = np.broadcast_to(logits, (T, B, K)).copy()
+        m.eval(-1, ids_in, read=False)
+        loss_t = m.eval_gradient(tg)
+        want = {n: (1 - share) * m.get_grad(n).astype(np.float64) for n in m.info}
+        loss = (1 - share) * loss_t
+        for k in range(K):
+            loss += share * q[k] * m.eval_gradient(np.ascontiguousarray(top[:, :, k]))
+            for n in want:
+                want[n] += share * q[k] * m.get_grad(n)
+        loss -= share * (q * np.log(q)).sum() * T * B
+        got = m.eval_gradient_distill(tg, top, rows, share)
+        assert abs(got - loss) < tol * abs(loss), (got, loss)
+        for n in want:
+            scale = max(np.abs(want[n]).max(), 1e-9)
+            assert np.abs(m.get_grad(n) - want[n]).max() < tol * scale, n
+        # entries outside the alphabet: no teacher; and the plain loss behind a teacher's is what it was before
+        plain = {n: m.get_grad(n) for n in m.info} if m.eval_gradient(tg) == loss_t else None
+        assert plain is not None
+        assert m.eval_gradient_distill(tg, np.full((T, B, K), -1, np.int32), rows, share) == loss_t
+        for n in plain:
+            assert np.array_equal(m.get_grad(n), plain[n]), n
+        m.update()
+    with pytest.raises(Exception):
+        m.eval_gradient_distill(tg, top, rows, 1.5)
+    m.close()
+
+
+def test_model_distillation_refuses_bad_arguments(pkg):
+    import ctypes
+    lib = pkg.library()
+    one, loss = 4096, ctypes.c_float()
+    assert lib.nncu_eval_gradient_distill(None, one, 1, one, one, 0.5, ctypes.byref(loss)) == pkg.abi.ERR_INVALID
