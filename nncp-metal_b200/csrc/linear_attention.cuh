@@ -595,14 +595,6 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                     to[64] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
-            const float l_n = last ? l_last : l_full;
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int x = 0; x < NT; x++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        s[m][x][c] *= l_n;
         }
         if constexpr (CG > 1)
             asm volatile("bar.sync %0, %1;" ::"r"(1 + r), "n"(32 * CG) : "memory"); // the warps of these rows
@@ -610,6 +602,13 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             __syncwarp();
         // the third term where a state is a result; 17 bits are more than the roundings behind them keep
         const bool third = q.s_end != nullptr;
+        // what the chunk adds has sums of its own: products cut the sum they are added to, the state is rounded
+        float add[MT][NT][4];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+                add[m][x][0] = add[m][x][1] = add[m][x][2] = add[m][x][3] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < TC / 16; ks++) {
             uint32_t f[NT / 2][4];
@@ -633,10 +632,19 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                             const uint32_t bf[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                             for (int x = 0; x < NT; x++)
-                                fa::mma(s[m][x], bf, f[x / 2][x % 2 * 2], f[x / 2][x % 2 * 2 + 1]);
+                                fa::mma(add[m][x], bf, f[x / 2][x % 2 * 2], f[x / 2][x % 2 * 2 + 1]);
                         }
             }
         }
+        const float l_n = last ? l_last : l_full;
+        if (carries)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        s[m][x][c] = fmaf(l_n, s[m][x][c], add[m][x][c]);
         if (!STATES) {
             if (!ok)
 #pragma unroll

@@ -13,8 +13,8 @@ static int qk_check(const nncu_qk_norm_shape *s)
     if (!s || s->n_rows < 1 || s->n_head < 1 || s->n_head_k < 0 || s->d_key < 2 || (s->d_key & 1) || s->d_rot < 0 ||
         (s->d_rot & 1) || s->d_rot > s->d_key || !(s->eps >= 0.0f) || !isfinite(s->eps) || (s->d_rot && !(s->rope_base > 0.0f && isfinite(s->rope_base))))
         return nncu_fail(NNCU_ERR_INVALID, "qk norm: bad shape");
-    if (s->d_key > NNCU_QK_NORM_DIM_MAX || s->n_head > NNCU_QK_NORM_HEADS_MAX || s->n_head_k > NNCU_QK_NORM_HEADS_MAX)
-        return nncu_fail(NNCU_ERR_RANGE, "qk norm: d_key over %d or more than %d heads", NNCU_QK_NORM_DIM_MAX, NNCU_QK_NORM_HEADS_MAX);
+    if (s->d_key > NNCU_QK_NORM_DIM_MAX || s->n_head > NNCU_QK_NORM_HEADS_MAX || s->n_head_k > NNCU_QK_NORM_HEADS_MAX || s->n_rows > 1 << 30)
+        return nncu_fail(NNCU_ERR_RANGE, "qk norm: d_key over %d, more than %d heads or too many rows", NNCU_QK_NORM_DIM_MAX, NNCU_QK_NORM_HEADS_MAX);
     const long long wq = (long long)s->n_head * s->d_key, wk = (long long)s->n_head_k * s->d_key;
     if ((s->ld_q && s->ld_q < wq) || (s->ld_q_out && s->ld_q_out < wq) || (s->ld_k && s->ld_k < wk) || (s->ld_k_out && s->ld_k_out < wk))
         return nncu_fail(NNCU_ERR_INVALID, "qk norm: a row pitch is less than the row");
