@@ -30,7 +30,9 @@ static void lin_parts(const nncu_linear_attn_shape *s, int roles, int *n_seg, in
 {
     const long long ctas = (long long)s->n_streams * s->n_head * roles;
     const int chunk = s->dtype_bf16 ? lin::TC : lin::FC, chunks = ceil_div(s->seg_len, chunk);
-    const int n = (int)std::min<long long>(std::max<long long>(SMS / ctas, 1), std::max(chunks / 4, 1));
+    // fp32: an SM takes three CTAs of head size 64 and one of 128
+    const int most = std::max(s->d_key, s->d_value), want = s->dtype_bf16 ? SMS : SMS * (most <= 64 ? 3 : 1);
+    const int n = (int)std::min<long long>(std::max<long long>(want / ctas, 1), std::max(chunks / 4, 1));
     const int each = ceil_div(chunks, n);
     *seg = each * chunk;
     *n_seg = ceil_div(chunks, each);
@@ -89,14 +91,14 @@ template <typename T, int VEC> static int lin_step(const lin::Args &a, int roles
     return NNCU_OK;
 }
 
-template <typename T, bool STATES> static int lin_core(const lin::Args &a, int roles, cudaStream_t st)
+template <typename T, bool STATES, bool PIECES> static int lin_core(const lin::Args &a, int roles, cudaStream_t st)
 {
     static DeviceOnce once;
-    NNCU_TRY(smem_limit(once, lin::core_kernel<T, STATES>, 4 * lin::CoreSmem(lin::DIM_MAX, lin::DIM_MAX).floats));
+    NNCU_TRY(smem_limit(once, lin::core_kernel<T, STATES, PIECES>, 4 * lin::CoreSmem(lin::DIM_MAX, lin::DIM_MAX, PIECES).floats));
     int floats = 0;
     for (int i = 0; i < roles; i++)
-        floats = std::max(floats, lin::CoreSmem(a.role[i].da, a.role[i].dc).floats);
-    CUDA_TRY(launch_k(lin::core_kernel<T, STATES>, dim3(a.B * a.H, STATES ? a.n_seg - 1 : a.n_seg, roles), dim3(256), 4 * floats, st, a));
+        floats = std::max(floats, lin::CoreSmem(a.role[i].da, a.role[i].dc, PIECES).floats);
+    CUDA_TRY(launch_k(lin::core_kernel<T, STATES, PIECES>, dim3(a.B * a.H, STATES ? a.n_seg - 1 : a.n_seg, roles), dim3(256), 4 * floats, st, a));
     KERNEL_CHECK();
     return NNCU_OK;
 }
@@ -165,22 +167,36 @@ static bool lin_pieces(const lin::Role &q, long long B)
            aligned(q.s_end, 8);
 }
 
+// the same for fp32 rows, which need no tensor map
+static bool lin_quads(const lin::Role &q)
+{
+    return q.da % 4 == 0 && q.dc % 4 == 0 && q.lda % 4 == 0 && q.ldb % 4 == 0 && q.ldc % 4 == 0 && q.ldo % 4 == 0 && aligned(q.a, 16) &&
+           aligned(q.b, 16) && aligned(q.c, 16) && aligned(q.o, 16);
+}
+
 // Roles of the same head sizes, side by side in one launch, in the form at the head of linear_attention.cuh
 template <typename T> static int lin_run(const lin::Args &a, int roles, cudaStream_t st)
 {
-    bool pieces = sizeof(T) == 2, wide = true;
+    bool pieces = sizeof(T) == 2, quads = sizeof(T) == 4, wide = true;
     for (int i = 0; i < roles; i++) {
         const lin::Role &q = a.role[i];
         pieces = pieces && lin_pieces(q, a.B);
+        quads = quads && lin_quads(q);
         wide = wide && q.dc % 4 == 0 && aligned(q.s0, 16) && aligned(q.s_end, 16);
     }
     if (a.T <= lin::STEP_TOKENS)
         return wide ? lin_step<T, 4>(a, roles, a.role[0].dc, st) : lin_step<T, 1>(a, roles, a.role[0].dc, st);
     if (pieces)
         return lin_mma(a, roles, st);
+    if constexpr (sizeof(T) == 4)
+        if (quads) {
+            if (a.n_seg > 1)
+                NNCU_TRY((lin_core<T, true, true>(a, roles, st)));
+            return lin_core<T, false, true>(a, roles, st);
+        }
     if (a.n_seg > 1)
-        NNCU_TRY((lin_core<T, true>(a, roles, st)));
-    return lin_core<T, false>(a, roles, st);
+        NNCU_TRY((lin_core<T, true, false>(a, roles, st)));
+    return lin_core<T, false, false>(a, roles, st);
 }
 
 static int lin_any(const nncu_linear_attn_shape *s, const lin::Args &a, int roles, cudaStream_t st)

@@ -20,6 +20,8 @@
 //
 // with e1 = 1, e2 = 0 in the sequence's order and e1 = 0, e2 = 1 in the reverse one.
 #pragma once
+#include <type_traits>
+
 #include "gemm_tc.cuh"
 #include "warp_mma.cuh"
 
@@ -89,55 +91,89 @@ __device__ __forceinline__ bool ends_in(const Args &p, int n, int g) { return g 
 
 // ---------------- CUDA cores: fp32, and bf16 whose rows are not laid out in 16-byte pieces ----------------
 //
-// A CTA of 256 threads goes through one part of one (stream, head) in chunks of 32 tokens; the tiles and the
-// state are fp32 in shared memory, a thread takes 4 x 4 results at a time.  Bound by shared-memory reads: five loads
-// for sixteen multiply-adds.
+// A CTA of 256 threads goes through one part of one (stream, head) in chunks of 32 tokens; tiles and state are fp32 in
+// shared memory, a thread takes 2 x 2 pair weights and 4 x 4 results or 8 x 4 elements of the state at a time.  Bound by
+// fp32 arithmetic and its shared-memory reads (eight of 16 bytes for 64 multiply-adds of a result).
+// fp32 rows laid out in 16-byte pieces (PIECES) are copied asynchronously, the next chunk's under the present one.
 
 constexpr int FC = 32; // tokens in a chunk
 
 struct CoreSmem {
-    int da4, dc4, ld_a, ld_c, b, c, s, p, w, floats;
-    __host__ __device__ CoreSmem(int da, int dc)
+    int da4, dc4, ld_a, ld_c, tile, b, c, s, p, w, floats;
+    __host__ __device__ CoreSmem(int da, int dc, bool twice)
     {
         da4 = (da + 3) & ~3; dc4 = (dc + 3) & ~3;
         ld_a = da4 + 4; ld_c = dc4 + 4; // rows four banks on
-        b = FC * ld_a; c = b + FC * ld_a; s = c + FC * ld_c; p = s + da4 * ld_c; w = p + FC * (FC + 1);
+        b = FC * ld_a; c = b + FC * ld_a; tile = c + FC * ld_c;
+        s = twice ? 2 * tile : tile; p = s + da4 * ld_c; w = p + FC * (FC + 4);
         floats = w + 2 * (FC + 2);
     }
 };
 
-template <typename T>
+// 32 rows of a matrix as a tile, zeros behind row n and column d
+template <typename T, bool PIECES>
 __device__ __forceinline__ void core_load(float *dst, int ld, int d4, int d, const void *src, long long ldr, int h, const Rows &rows, int u0, int n)
 {
     const T *base = reinterpret_cast<const T *>(src) + (size_t)h * d;
-    for (int i = threadIdx.x; i < FC * d4; i += 256) {
-        const int r = i / d4, x = i % d4;
-        dst[r * ld + x] = r < n && x < d ? to_f(base[rows.row(u0 + r) * ldr + x]) : 0.0f;
+    if constexpr (PIECES) {
+        const int q4 = d4 / 4;
+        for (int i = threadIdx.x; i < FC * q4; i += 256) {
+            const int r = i / q4, x = (i - r * q4) * 4;
+            const bool ok = r < n;
+            fa::cp16(dst + r * ld + x, base + (ok ? rows.row(u0 + r) * ldr + x : 0), ok);
+        }
+    } else {
+        for (int i = threadIdx.x; i < FC * d4; i += 256) {
+            const int r = i / d4, x = i - r * d4;
+            dst[r * ld + x] = r < n && x < d ? to_f(base[rows.row(u0 + r) * ldr + x]) : 0.0f;
+        }
     }
 }
 
+__device__ __forceinline__ float4 quad(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ void add4(float4 &s, float u, const float4 &v)
+{
+    s.x = fmaf(u, v.x, s.x); s.y = fmaf(u, v.y, s.y); s.z = fmaf(u, v.z, s.z); s.w = fmaf(u, v.w, s.w);
+}
+__device__ __forceinline__ float dot4(const float4 &u, const float4 &v, float s)
+{
+    return fmaf(u.x, v.x, fmaf(u.y, v.y, fmaf(u.z, v.z, fmaf(u.w, v.w, s))));
+}
+
 // STATES: the first pass over a sequence in several parts: what each part but the last adds to the state
-template <typename T, bool STATES>
+template <typename T, bool STATES, bool PIECES>
 __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args p)
 {
     extern __shared__ __align__(16) float smf[];
     const Role &q = p.role[blockIdx.z];
-    const CoreSmem sm(q.da, q.dc);
-    float *As = smf, *Bs = smf + sm.b, *Cs = smf + sm.c, *Ss = smf + sm.s, *Ps = smf + sm.p, *pw = smf + sm.w, *wt = pw + FC + 2;
+    const CoreSmem sm(q.da, q.dc, PIECES);
+    float *Ss = smf + sm.s, *Ps = smf + sm.p, *pw = smf + sm.w, *wt = pw + FC + 2;
+    constexpr int LP = FC + 4;
     const int tid = threadIdx.x;
     const size_t pair = blockIdx.x;
     const int g = blockIdx.y, b = (int)(pair / p.H), h = (int)(pair % p.H);
     const float rate = p.rate[h];
-    pdl_trigger();
     pdl_wait();
     const Rows rows(p, q, b);
     const size_t nn = (size_t)q.da * q.dc;
     const int begin = g * p.seg, end = min(rows.n, begin + p.seg);
+    auto fetch = [&](int u0, float *to) {
+        const int n = end - u0;
+        if (!STATES)
+            core_load<T, PIECES>(to, sm.ld_a, sm.da4, q.da, q.a, q.lda, h, rows, u0, n);
+        core_load<T, PIECES>(to + sm.b, sm.ld_a, sm.da4, q.da, q.b, q.ldb, h, rows, u0, n);
+        core_load<T, PIECES>(to + sm.c, sm.ld_c, sm.dc4, q.dc, q.c, q.ldc, h, rows, u0, n);
+        if (PIECES)
+            fa::cp_commit();
+    };
+    if (PIECES && begin < end)
+        fetch(begin, smf);
     const float l_seg = power(rate, p.seg);
     for (int i = tid; i < FC + 2; i += 256)
         pw[i] = power(rate, i);
+    const int c4 = sm.dc4 / 4;
     for (int i = tid; i < sm.da4 * sm.dc4; i += 256) {
-        const int x = i / sm.dc4, y = i % sm.dc4;
+        const int x = i / sm.dc4, y = i - x * sm.dc4;
         float s = 0.0f;
         if (x < q.da && y < q.dc) {
             float *part = q.parts + pair * p.n_seg * p.slot + (size_t)x * q.dc + y;
@@ -154,92 +190,120 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
     }
     if (!STATES)
         zero_behind<T>(p, q, rows, b, h, g, tid >> 5, 8, tid & 31);
-    for (int u0 = begin; u0 < end; u0 += FC) {
+    int turn = 0;
+    for (int u0 = begin; u0 < end; u0 += FC, turn ^= PIECES) {
         const int n = min(FC, end - u0);
+        float *As = smf + turn * sm.tile, *Bs = As + sm.b, *Cs = As + sm.c;
+        if (PIECES) {
+            fa::cp_wait<0>();
+        } else {
+            __syncthreads(); // the chunk before has been read
+            fetch(u0, As);
+        }
         __syncthreads();
-        if (!STATES)
-            core_load<T>(As, sm.ld_a, sm.da4, q.da, q.a, q.lda, h, rows, u0, n);
-        core_load<T>(Bs, sm.ld_a, sm.da4, q.da, q.b, q.ldb, h, rows, u0, n);
-        core_load<T>(Cs, sm.ld_c, sm.dc4, q.dc, q.c, q.ldc, h, rows, u0, n);
-        for (int i = tid; i < FC; i += 256)
-            wt[i] = i < n ? q.s_in * pw[n - 1 - i + q.e2] : 0.0f;
-        __syncthreads();
+        if (PIECES && u0 + FC < end)
+            fetch(u0 + FC, smf + (turn ^ 1) * sm.tile);
+        if (tid < FC)
+            wt[tid] = tid < n ? q.s_in * pw[n - 1 - tid + q.e2] : 0.0f;
         if (!STATES) {
-            for (int k = 0; k < FC * FC / 256; k++) {
-                const int i = tid / 8, j = tid % 8 + 8 * k;
-                float s = 0.0f;
-                if (j <= i) {
-                    for (int x = 0; x < sm.da4; x += 4) {
-                        const float4 u = *reinterpret_cast<const float4 *>(As + i * sm.ld_a + x), v = *reinterpret_cast<const float4 *>(Bs + j * sm.ld_a + x);
-                        s = fmaf(u.x, v.x, fmaf(u.y, v.y, fmaf(u.z, v.z, fmaf(u.w, v.w, s))));
-                    }
-                    s *= q.s_pair * pw[i - j];
+            {
+                const int i0 = tid / 16, j0 = tid % 16; // rows i0, i0 + 16, keys j0, j0 + 16
+                float w[2][2] = {};
+                for (int x = 0; x < sm.da4; x += 4) {
+                    const float4 a0 = quad(As + i0 * sm.ld_a + x), a1 = quad(As + (i0 + 16) * sm.ld_a + x);
+                    const float4 b0 = quad(Bs + j0 * sm.ld_a + x), b1 = quad(Bs + (j0 + 16) * sm.ld_a + x);
+                    w[0][0] = dot4(a0, b0, w[0][0]);
+                    w[1][0] = dot4(a1, b0, w[1][0]);
+                    w[1][1] = dot4(a1, b1, w[1][1]);
                 }
-                Ps[i * (FC + 1) + j] = s;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int v = 0; v < 2; v++) {
+                        const int i = i0 + 16 * u, j = j0 + 16 * v;
+                        Ps[i * LP + j] = j <= i ? w[u][v] * q.s_pair * pw[i - j] : 0.0f;
+                    }
             }
             __syncthreads();
-            for (int it = tid; it < FC / 4 * (sm.dc4 / 4); it += 256) {
-                const int i0 = it / (sm.dc4 / 4) * 4, c0 = it % (sm.dc4 / 4) * 4;
-                float acc[4][4] = {};
-                for (int x = 0; x < q.da; x++) {
-                    const float4 s = *reinterpret_cast<const float4 *>(Ss + x * sm.ld_c + c0);
+            constexpr int R = 4;
+            for (int it = tid; it < FC / R * c4; it += 256) {
+                const int i0 = it / c4 * R, c0 = (it - it / c4 * c4) * 4;
+                float4 o[R];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float u = As[(i0 + r) * sm.ld_a + x];
-                        acc[r][0] = fmaf(u, s.x, acc[r][0]); acc[r][1] = fmaf(u, s.y, acc[r][1]);
-                        acc[r][2] = fmaf(u, s.z, acc[r][2]); acc[r][3] = fmaf(u, s.w, acc[r][3]);
+                for (int r = 0; r < R; r++)
+                    o[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                // four columns of the R rows at u against four rows of four columns at v
+                auto product = [&](const float *u, int ldu, const float *v) {
+                    const float4 v0 = quad(v), v1 = quad(v + sm.ld_c), v2 = quad(v + 2 * sm.ld_c), v3 = quad(v + 3 * sm.ld_c);
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        const float4 w = quad(u + r * ldu);
+                        add4(o[r], w.x, v0); add4(o[r], w.y, v1); add4(o[r], w.z, v2); add4(o[r], w.w, v3);
                     }
-                }
+                };
+                for (int x = 0; x < sm.da4; x += 4)
+                    product(As + i0 * sm.ld_a + x, sm.ld_a, Ss + x * sm.ld_c + c0);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
+                for (int r = 0; r < R; r++) {
                     const float f = q.s_state * pw[i0 + r + q.e1];
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        acc[r][c] *= f;
+                    o[r].x *= f; o[r].y *= f; o[r].z *= f; o[r].w *= f;
                 }
-                for (int j = 0; j < min(i0 + 4, n); j++) {
-                    const float4 s = *reinterpret_cast<const float4 *>(Cs + j * sm.ld_c + c0);
+                for (int j = 0; j < min(i0 + R, n); j += 4) // weights behind the row are zeros, and so are rows behind the last
+                    product(Ps + i0 * LP + j, LP, Cs + j * sm.ld_c + c0);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float u = Ps[(i0 + r) * (FC + 1) + j];
-                        acc[r][0] = fmaf(u, s.x, acc[r][0]); acc[r][1] = fmaf(u, s.y, acc[r][1]);
-                        acc[r][2] = fmaf(u, s.z, acc[r][2]); acc[r][3] = fmaf(u, s.w, acc[r][3]);
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 4; r++)
+                for (int r = 0; r < R; r++)
                     if (i0 + r < n) {
-                        T *o = reinterpret_cast<T *>(q.o) + rows.row(u0 + i0 + r) * q.ldo + (size_t)h * q.dc + c0;
+                        T *to = reinterpret_cast<T *>(q.o) + rows.row(u0 + i0 + r) * q.ldo + (size_t)h * q.dc + c0;
+                        if constexpr (PIECES) {
+                            *reinterpret_cast<float4 *>(to) = o[r];
+                        } else {
+                            const float v[4] = {o[r].x, o[r].y, o[r].z, o[r].w};
 #pragma unroll
-                        for (int c = 0; c < 4; c++)
-                            if (c0 + c < q.dc)
-                                o[c] = from_f<T>(acc[r][c]);
+                            for (int c = 0; c < 4; c++)
+                                if (c0 + c < q.dc)
+                                    to[c] = from_f<T>(v[c]);
+                        }
                     }
             }
-            __syncthreads();
         }
+        __syncthreads(); // the state has been read, the weights stand
+        if (!STATES && u0 + FC >= end && !q.s_end)
+            break;
         const float l_n = pw[n];
-        for (int it = tid; it < (sm.da4 / 4) * (sm.dc4 / 4); it += 256) {
-            const int x0 = it / (sm.dc4 / 4) * 4, c0 = it % (sm.dc4 / 4) * 4;
-            float acc[4][4] = {};
-            for (int j = 0; j < n; j++) {
-                const float4 s = *reinterpret_cast<const float4 *>(Cs + j * sm.ld_c + c0);
-                const float w = wt[j];
+        // R rows of the state at a time, eight where that leaves work for every thread
+        auto carry = [&](auto size) {
+            constexpr int R = decltype(size)::value;
+            for (int it = tid; it < sm.da4 / R * c4; it += 256) {
+                const int x0 = it / c4 * R, c0 = (it - it / c4 * c4) * 4;
+                float4 add[R];
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float u = w * Bs[j * sm.ld_a + x0 + r];
-                    acc[r][0] = fmaf(u, s.x, acc[r][0]); acc[r][1] = fmaf(u, s.y, acc[r][1]);
-                    acc[r][2] = fmaf(u, s.z, acc[r][2]); acc[r][3] = fmaf(u, s.w, acc[r][3]);
+                for (int r = 0; r < R; r++)
+                    add[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                for (int j = 0; j < n; j++) {
+                    const float4 v = quad(Cs + j * sm.ld_c + c0);
+                    const float w = wt[j];
+#pragma unroll
+                    for (int r = 0; r < R; r += 4) {
+                        const float4 u = quad(Bs + j * sm.ld_a + x0 + r);
+                        add4(add[r], w * u.x, v); add4(add[r + 1], w * u.y, v);
+                        add4(add[r + 2], w * u.z, v); add4(add[r + 3], w * u.w, v);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    float4 *s = reinterpret_cast<float4 *>(Ss + (x0 + r) * sm.ld_c + c0);
+                    float4 now = *s;
+                    now.x = fmaf(l_n, now.x, add[r].x); now.y = fmaf(l_n, now.y, add[r].y);
+                    now.z = fmaf(l_n, now.z, add[r].z); now.w = fmaf(l_n, now.w, add[r].w);
+                    *s = now;
                 }
             }
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    float *s = Ss + (x0 + r) * sm.ld_c + c0 + c;
-                    *s = fmaf(l_n, *s, acc[r][c]);
-                }
-        }
+        };
+        if (sm.da4 % 8 == 0 && sm.da4 / 8 * c4 >= 256)
+            carry(std::integral_constant<int, 8>());
+        else
+            carry(std::integral_constant<int, 4>());
     }
     __syncthreads();
     float *to = STATES ? q.parts + (pair * p.n_seg + g + 1) * p.slot : (q.s_end && ends_in(p, rows.n, g) ? q.s_end + pair * nn : nullptr);
