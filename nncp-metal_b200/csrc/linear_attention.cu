@@ -84,6 +84,13 @@ static lin::Args lin_args(const nncu_linear_attn_shape *s, int roles, const floa
     return a;
 }
 
+// A state goes out where it came in, or somewhere else altogether
+static bool lin_apart(const nncu_linear_attn_shape *s, const float *from, const float *to)
+{
+    const size_t n = (size_t)s->n_streams * s->n_head * s->d_key * s->d_value;
+    return !from || !to || from + n <= to || to + n <= from;
+}
+
 template <typename T, int VEC> static int lin_step(const lin::Args &a, int roles, int dc, cudaStream_t st)
 {
     CUDA_TRY(launch_k(lin::step_kernel<T, VEC>, dim3(a.B * a.H, ceil_div(dc, 8 * VEC), roles), dim3(128), 0, st, a));
@@ -225,6 +232,8 @@ int nncu_linear_attention_forward(const nncu_linear_attn_shape *s, const void *q
     NNCU_TRY(lin_common(s, 1, decay_host, workspace, workspace_bytes));
     if (out == q || out == k || out == v)
         return nncu_fail(NNCU_ERR_INVALID, "linear attention: the result cannot go over q, k or v");
+    if (state_in != state_out && !lin_apart(s, state_in, state_out))
+        return nncu_fail(NNCU_ERR_INVALID, "linear attention: the states overlap");
     NNCU_TRY(elements_aligned({q, k, v, out}, s->dtype_bf16 ? 2 : 4));
     NNCU_TRY(elements_aligned({len, state_in, state_out}, 4));
     NNCU_TRY(on_device({q, k, v, len, state_in, out, state_out, lin_need(s, 1) ? workspace : nullptr}));
@@ -253,6 +262,8 @@ int nncu_linear_attention_backward(const nncu_linear_attn_shape *s, const void *
     for (const void *to : {dq, dk, dv})
         if (to == q || to == k || to == v || to == dout || (to == dq) + (to == dk) + (to == dv) > 1)
             return nncu_fail(NNCU_ERR_INVALID, "linear attention: a gradient needs a place of its own");
+    if ((dstate_in != dstate_out && !lin_apart(s, dstate_out, dstate_in)) || !lin_apart(s, state_in, dstate_in))
+        return nncu_fail(NNCU_ERR_INVALID, "linear attention: the states overlap");
     NNCU_TRY(elements_aligned({q, k, v, dout, dq, dk, dv}, s->dtype_bf16 ? 2 : 4));
     NNCU_TRY(elements_aligned({len, state_in, dstate_out, dstate_in}, 4));
     NNCU_TRY(on_device({q, k, v, len, state_in, dout, dstate_out, dq, dk, dv, dstate_in, lin_need(s, 3) ? workspace : nullptr}));
@@ -276,9 +287,7 @@ int nncu_linear_attention_backward(const nncu_linear_attn_shape *s, const void *
     rq.s_in = rk.s_state = rv.s_state = 1.0f;
     // one launch for all three, or dv behind the others: where its head sizes are other than theirs, and where
     // dstate_in lies over the dstate_out that they read
-    const float *from = dstate_out, *to = dstate_in;
-    const size_t states = (size_t)s->n_streams * wk * s->d_value;
-    if (s->d_key == s->d_value && !(from && to && from < to + states && to < from + states))
+    if (s->d_key == s->d_value && lin_apart(s, dstate_out, dstate_in))
         return lin_any(s, all, 3, st);
     lin::Args two = all;
     two.role[0] = rq;

@@ -96,6 +96,20 @@ template <typename T, bool BACK> static int qk_any(const nncu_qk_norm_shape *s, 
     return w == 4 ? qk_launch<T, 4, 1, BACK>(s, a, st) : w == 2 ? qk_launch<T, 2, 2, BACK>(s, a, st) : qk_launch<T, 1, 4, BACK>(s, a, st);
 }
 
+// Results lie over an input only where every value is written by the thread that has read it: over the same rows
+static int qk_places(const qkn::Args &a)
+{
+    for (int i = 0; i < 2; i++) {
+        const void *y = a.y[i], *x = a.x[i], *dy = a.dy[i];
+        if (!y)
+            continue;
+        const int ldy = a.dy[i] ? a.ldx[i] : a.ldy[i]; // pitch of y: of the results, or backward of x
+        if ((y == x && ldy != a.ldx[i]) || (y == dy && ldy != a.ldy[i]) || y == a.y[1 - i] || y == a.x[1 - i] || y == a.dy[1 - i])
+            return nncu_fail(NNCU_ERR_INVALID, "qk norm: results in place need the pitch of their inputs, and a place each");
+    }
+    return NNCU_OK;
+}
+
 extern "C" {
 
 int nncu_qk_norm_rope_forward(const nncu_qk_norm_shape *s, const void *q, const void *k, const float *gain_q, const float *gain_k,
@@ -106,8 +120,7 @@ int nncu_qk_norm_rope_forward(const nncu_qk_norm_shape *s, const void *q, const 
         return nncu_fail(NNCU_ERR_INVALID, "null tensor");
     qkn::Args a = qk_args(s, q, s->n_head_k ? k : nullptr, gain_q, gain_k, pos);
     a.y[0] = q_out; a.y[1] = s->n_head_k ? k_out : nullptr;
-    if ((a.x[0] == a.y[0] && a.ldx[0] != a.ldy[0]) || (a.y[1] && a.x[1] == a.y[1] && a.ldx[1] != a.ldy[1]) || a.y[0] == a.y[1])
-        return nncu_fail(NNCU_ERR_INVALID, "qk norm: results in place need the pitch of their inputs, and a place each");
+    NNCU_TRY(qk_places(a));
     NNCU_TRY(elements_aligned({a.x[0], a.x[1], a.y[0], a.y[1]}, s->dtype_bf16 ? 2 : 4));
     NNCU_TRY(elements_aligned({gain_q, gain_k, pos}, 4));
     NNCU_TRY(on_device({a.x[0], a.x[1], gain_q, gain_k, pos, a.y[0], a.y[1]}));
@@ -132,7 +145,7 @@ int nncu_qk_norm_rope_backward(const nncu_qk_norm_shape *s, const void *q, const
     NNCU_TRY(nncu_qk_norm_rope_workspace(s, &need));
     if (!q || !dq_out || !dq || (s->n_head_k && (!k || !dk_out || !dk)) || (s->d_rot && !pos))
         return nncu_fail(NNCU_ERR_INVALID, "null tensor");
-    if ((dgain_q && !gain_q) || (dgain_k && !gain_k))
+    if ((dgain_q && !gain_q) || (dgain_k && (!gain_k || !s->n_head_k)))
         return nncu_fail(NNCU_ERR_INVALID, "qk norm: the gradient of a gain that is not there");
     const bool gains = dgain_q || dgain_k;
     if (gains && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
@@ -141,8 +154,7 @@ int nncu_qk_norm_rope_backward(const nncu_qk_norm_shape *s, const void *q, const
     a.dy[0] = dq_out; a.dy[1] = s->n_head_k ? dk_out : nullptr;
     a.y[0] = dq; a.y[1] = s->n_head_k ? dk : nullptr;
     a.part = gains ? (float *)workspace : nullptr;
-    if ((a.dy[0] == a.y[0] && a.ldx[0] != a.ldy[0]) || (a.y[1] && a.dy[1] == a.y[1] && a.ldx[1] != a.ldy[1]) || a.y[0] == a.y[1])
-        return nncu_fail(NNCU_ERR_INVALID, "qk norm: results in place need the pitch of their inputs, and a place each");
+    NNCU_TRY(qk_places(a));
     NNCU_TRY(elements_aligned({a.x[0], a.x[1], a.dy[0], a.dy[1], a.y[0], a.y[1]}, s->dtype_bf16 ? 2 : 4));
     NNCU_TRY(elements_aligned({gain_q, gain_k, pos, dgain_q, dgain_k}, 4));
     NNCU_TRY(on_device({a.x[0], a.x[1], a.dy[0], a.dy[1], gain_q, gain_k, pos, a.y[0], a.y[1], dgain_q, dgain_k, a.part}));

@@ -76,6 +76,31 @@ def test_qk_norm_refuses_bad_arguments(pkg):
         _refused(pkg, backward(**over))
 
 
+def test_qk_norm_refuses_results_over_the_other_input(pkg):
+    lib, a, b, c, d = pkg.library(), 4096, 8192, 12288, 16384
+    s = pkg.abi.QkNormShape(n_rows=4, n_head=1, n_head_k=1, d_key=8, d_rot=0, eps=1e-6, dtype_bf16=1)
+    for q_out, k_out in ((b, c), (c, a), (c, c)):
+        _refused(pkg, lib.nncu_qk_norm_rope_forward(C.byref(s), a, b, None, None, None, q_out, k_out, None))
+    for dq, dk in ((b, 5 * a), (5 * a, a), (d, 5 * a), (5 * a, c), (5 * a, 5 * a)):  # dq_out at c, dk_out at d
+        _refused(pkg, lib.nncu_qk_norm_rope_backward(C.byref(s), a, b, None, None, None, c, d, dq, dk, None, None, None, 0, None))
+    # a gain of keys that are not there
+    one = pkg.abi.QkNormShape(n_rows=4, n_head=1, n_head_k=0, d_key=8, d_rot=0, eps=1e-6, dtype_bf16=1)
+    _refused(pkg, lib.nncu_qk_norm_rope_backward(C.byref(one), a, None, a, a, None, c, None, d, None, a, a, a, 1 << 20, None))
+
+
+def test_linear_attention_refuses_states_that_overlap(pkg):
+    lib, one = pkg.library(), 1 << 20
+    s = pkg.abi.LinearAttnShape(n_streams=2, n_head=1, d_key=16, d_value=16, seg_len=4, scale=1.0, dtype_bf16=1)
+    d, size = (C.c_float * 1)(0.5), 2 * 16 * 16 * 4
+    for off in (4, size - 4, -4):
+        _refused(pkg, lib.nncu_linear_attention_forward(C.byref(s), one, one, one, d, None, 2 * one, 3 * one, 2 * one + off, None, 0, None))
+        _refused(pkg, lib.nncu_linear_attention_backward(C.byref(s), one, one, one, d, None, None, 3 * one, 2 * one, 4 * one, 5 * one, 6 * one,
+                                                         2 * one + off, None, 0, None))
+    # the state that dq reads is not a place for dstate_in
+    _refused(pkg, lib.nncu_linear_attention_backward(C.byref(s), one, one, one, d, None, 2 * one, 3 * one, None, 4 * one, 5 * one, 6 * one,
+                                                     2 * one, None, 0, None))
+
+
 def test_linear_attention_refuses_bad_arguments(pkg):
     lib, one = pkg.library(), 4096
     good = dict(n_streams=2, n_head=2, d_key=16, d_value=16, seg_len=4096, scale=0.25, dtype_bf16=1)
@@ -820,3 +845,46 @@ def test_model_distillation_refuses_bad_arguments(pkg):
     lib = pkg.library()
     one, loss = 4096, ctypes.c_float()
     assert lib.nncu_eval_gradient_distill(None, one, 1, one, one, 0.5, ctypes.byref(loss)) == pkg.abi.ERR_INVALID
+
+
+# ---------------------------------------------------------------- offsets beyond 32 bits
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_far_apart(pkg, kind):
+    """Row pitches that put rows more than 2^32 bytes from the first: the bits of rows that lie close together"""
+    B, T, d = 2, 1100, 64
+    N, pitch = B * T, 1 << (20 if kind == torch.bfloat16 else 19)
+    buf = torch.empty(N * pitch, device="cuda", dtype=kind).view(N, pitch)
+    assert N * pitch * buf.element_size() > 1 << 32
+    g = torch.Generator(device="cuda").manual_seed(4)
+    near, far = {}, {}
+    for i, x in enumerate(("q", "k", "v", "dout")):
+        near[x] = torch.randn(N, d, generator=g, device="cuda").to(kind)
+        far[x] = buf[:, 4096 * i:4096 * i + d]
+        far[x].copy_(near[x])
+    decay, s0 = torch.tensor([0.97]), torch.randn(B, 1, d, d, generator=g, device="cuda")
+    results = []
+    for t in (near, far):
+        op = Linear(pkg, (B, 1, d, d, T), kind, t, decay, s0, s0.clone(), None)
+        op.out = torch.empty(N, d, device="cuda", dtype=kind) if t is near else buf[:, 32768:32768 + d]
+        if t is far:
+            op.dq, op.dk, op.dv = (buf[:, 40000 + 1000 * i:40000 + 1000 * i + d] for i in range(3))
+        results.append([x.clone() for x in (*op.forward(), *op.backward())])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    # norms of rows that far apart, and logits
+    pos = torch.arange(N, device="cuda").int()
+    outs = []
+    for t in (near, far):
+        p = t["q"].stride(0)
+        s = pkg.abi.QkNormShape(n_rows=N, n_head=1, n_head_k=1, d_key=d, d_rot=d, ld_q=p, ld_k=p, ld_q_out=p, ld_k_out=p, eps=1e-6, rope_base=1e4,
+                                dtype_bf16=int(kind == torch.bfloat16))
+        q, k = (torch.empty(N, d, device="cuda", dtype=kind) for _ in range(2)) if t is near else (buf[:, 50000 + 1000 * i:50000 + 1000 * i + d] for i in range(2))
+        _ok(pkg, pkg.library().nncu_qk_norm_rope_forward(C.byref(s), _ptr(t["q"]), _ptr(t["k"]), None, None, _ptr(pos), _ptr(q), _ptr(k), _stream()))
+        outs.append((q.clone(), k.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    z, ids, top, targets, weight = _distill_data(N, 2000, 20, kind)
+    far_z = buf[:, 100000:102000]
+    far_z.copy_(z)
+    one, two = (_distill_calls(pkg, x, ids, top, targets, weight, 2.0, 0.5, kind) for x in (z, far_z))
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
