@@ -110,12 +110,12 @@ template <typename T, bool STATES, bool PIECES> static int lin_core(const lin::A
     return NNCU_OK;
 }
 
-template <int DA, int DC, bool STATES, bool TMA> static int lin_mma_launch(const lin::MmaArgs &m, int roles, cudaStream_t st)
+template <int DA, int DC, bool STATES, bool TMA, bool TWO> static int lin_mma_launch(const lin::MmaArgs &m, int roles, cudaStream_t st)
 {
+    constexpr int bytes = lin::MmaSmem<DA, DC, TWO>::BYTES;
     static DeviceOnce once;
-    NNCU_TRY(smem_limit(once, lin::mma_kernel<DA, DC, STATES, TMA>, lin::MmaSmem<DA, DC>::BYTES));
-    CUDA_TRY(launch_k(lin::mma_kernel<DA, DC, STATES, TMA>, dim3(m.p.B * m.p.H, STATES ? m.p.n_seg - 1 : m.p.n_seg, roles), dim3(4 * DC),
-                      lin::MmaSmem<DA, DC>::BYTES, st, m));
+    NNCU_TRY(smem_limit(once, lin::mma_kernel<DA, DC, STATES, TMA, TWO>, bytes));
+    CUDA_TRY(launch_k(lin::mma_kernel<DA, DC, STATES, TMA, TWO>, dim3(m.p.B * m.p.H, STATES ? m.p.n_seg - 1 : m.p.n_seg, roles), dim3(4 * DC), bytes, st, m));
     KERNEL_CHECK();
     return NNCU_OK;
 }
@@ -135,30 +135,34 @@ static int lin_map(const lin::Args &a, const void *rows, long long ld, int d, in
     return rc == CUDA_SUCCESS ? NNCU_OK : nncu_fail(NNCU_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)rc);
 }
 
-template <int DA, int DC> static int lin_mma_sized(const lin::Args &a, int roles, cudaStream_t st)
+template <int DA, int DC, bool TWO> static int lin_mma_sized(const lin::Args &a, int roles, cudaStream_t st)
 {
     lin::MmaArgs m;
     m.p = a;
     if (a.T <= lin::TC)
-        return lin_mma_launch<DA, DC, false, false>(m, roles, st);
+        return lin_mma_launch<DA, DC, false, false, TWO>(m, roles, st);
     for (int i = 0; i < roles; i++) {
         const lin::Role &q = a.role[i];
         NNCU_TRY(lin_map(a, q.a, q.lda, q.da, DA, &m.map[i][0]));
         NNCU_TRY(lin_map(a, q.b, q.ldb, q.da, DA, &m.map[i][1]));
         NNCU_TRY(lin_map(a, q.c, q.ldc, q.dc, DC, &m.map[i][2]));
+        if (q.a2)
+            NNCU_TRY(lin_map(a, q.a2, q.lda2, q.dc, DC, &m.map[i][3]));
     }
     if (a.n_seg > 1)
-        NNCU_TRY((lin_mma_launch<DA, DC, true, true>(m, roles, st)));
-    return lin_mma_launch<DA, DC, false, true>(m, roles, st);
+        NNCU_TRY((lin_mma_launch<DA, DC, true, true, false>(m, roles, st)));
+    return lin_mma_launch<DA, DC, false, true, TWO>(m, roles, st);
 }
 
 // head sizes go up to the next of 32, 64 and 128, zeros beyond their own
 static int lin_mma(const lin::Args &a, int roles, cudaStream_t st)
 {
     const int dc = a.role[0].dc, da = a.role[0].da;
+    if (a.role[0].a2)
+        return lin_mma_sized<64, 64, true>(a, roles, st);
     auto with = [&](auto size) {
         constexpr int DA = decltype(size)::value;
-        return dc <= 32 ? lin_mma_sized<DA, 32>(a, roles, st) : dc <= 64 ? lin_mma_sized<DA, 64>(a, roles, st) : lin_mma_sized<DA, 128>(a, roles, st);
+        return dc <= 32 ? lin_mma_sized<DA, 32, false>(a, roles, st) : dc <= 64 ? lin_mma_sized<DA, 64, false>(a, roles, st) : lin_mma_sized<DA, 128, false>(a, roles, st);
     };
     return da <= 32 ? with(std::integral_constant<int, 32>()) : da <= 64 ? with(std::integral_constant<int, 64>())
                                                                          : with(std::integral_constant<int, 128>());
@@ -171,7 +175,7 @@ static bool lin_pieces(const lin::Role &q, long long B)
         if (ld % 8 != 0 || ld * B * 2 >= 1ll << 40)
             return false;
     return q.da % 8 == 0 && q.dc % 8 == 0 && aligned(q.a, 16) && aligned(q.b, 16) && aligned(q.c, 16) && aligned(q.o, 16) && aligned(q.s0, 8) &&
-           aligned(q.s_end, 8);
+           aligned(q.s_end, 8) && (!q.a2 || (q.lda2 % 8 == 0 && q.ldo2 % 8 == 0 && q.lda2 * B * 2 < 1ll << 40 && aligned(q.a2, 16) && aligned(q.o2, 16)));
 }
 
 // the same for fp32 rows, which need no tensor map
@@ -285,6 +289,18 @@ int nncu_linear_attention_backward(const nncu_linear_attn_shape *s, const void *
     rk.reverse = rv.reverse = 1;
     rq.s_state = rq.s_pair = rk.s_pair = rv.s_pair = rk.s_in = rv.s_in = s->scale;
     rq.s_in = rk.s_state = rv.s_state = 1.0f;
+    // bf16 rows in 16-byte pieces, head sizes from 33 to 64: dk beside dv, from the same tiles and the same state, where three
+    // CTAs for each (stream, head) are more than the two an SM that run in one round (128 pairs of 2048 tokens, backward 151 ->
+    // 128 us, 256 of 512 75 -> 67; 32 pairs of 1024 33 -> 52), and where different head sizes would make two launches
+    const int least = std::min(s->d_key, s->d_value), most = std::max(s->d_key, s->d_value);
+    if (s->dtype_bf16 && s->seg_len > lin::STEP_TOKENS && least > 32 && most <= 64 &&
+        (3ll * s->n_streams * s->n_head * all.n_seg > 2 * SMS || s->d_key != s->d_value)) {
+        lin::Args two = all;
+        lin::Role &both = two.role[0];
+        both.a2 = v; both.lda2 = lv; both.o2 = dk; both.ldo2 = lk;
+        if (lin_pieces(both, s->n_streams) && lin_pieces(rq, s->n_streams))
+            return lin_any(s, two, 2, st);
+    }
     // one launch for all three, or dv behind the others: where its head sizes are other than theirs, and where
     // dstate_in lies over the dstate_out that they read
     if (s->d_key == s->d_value && lin_apart(s, dstate_out, dstate_in))

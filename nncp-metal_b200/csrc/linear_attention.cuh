@@ -37,7 +37,9 @@ struct Role {
     const float *s0;     // state before the first token, [B][H][da][dc] or, where s0_t, [B][H][dc][da]; NULL: zeros
     float *s_end;        // state behind the last token, [B][H][da][dc]; NULL: not wanted
     float *parts;        // [B*H][n_seg][slot]: slot 0 the state before the first token, slot g what part g - 1 adds up to
-    long long lda, ldb, ldc, ldo; // elements from row to row
+    const void *a2;      // not NULL: a second result of the same rows and state (kernels of two results)
+    void *o2;
+    long long lda, ldb, ldc, ldo, lda2, ldo2; // elements from row to row
     int da, dc, reverse, s0_t, e1, e2;
     float s_state, s_pair, s_in;
 };
@@ -70,12 +72,13 @@ struct Rows {
 
 // rows of the result behind a stream's end are zeros: those of them that part g is to write, a warp a row
 template <typename T>
-__device__ __forceinline__ void zero_behind(const Args &p, const Role &q, const Rows &rows, int b, int h, int g, int warp, int warps, int lane)
+__device__ __forceinline__ void zero_behind(const Args &p, void *out, long long ldo, int d, const Rows &rows, int b, int h, int g, int warp,
+                                            int warps, int lane)
 {
     const int hi = g == p.n_seg - 1 ? p.T : min(p.T, (g + 1) * p.seg);
     for (int t = max(rows.n, g * p.seg) + warp; t < hi; t += warps) {
-        T *o = reinterpret_cast<T *>(q.o) + ((long long)t * p.B + b) * q.ldo + (size_t)h * q.dc;
-        for (int i = lane; i < q.dc; i += 32)
+        T *o = reinterpret_cast<T *>(out) + ((long long)t * p.B + b) * ldo + (size_t)h * d;
+        for (int i = lane; i < d; i += 32)
             o[i] = from_f<T>(0.0f);
     }
 }
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
         Ss[x * sm.ld_c + y] = s;
     }
     if (!STATES)
-        zero_behind<T>(p, q, rows, b, h, g, tid >> 5, 8, tid & 31);
+        zero_behind<T>(p, q.o, q.ldo, q.dc, rows, b, h, g, tid >> 5, 8, tid & 31);
     int turn = 0;
     for (int u0 = begin; u0 < end; u0 += FC, turn ^= PIECES) {
         const int n = min(FC, end - u0);
@@ -329,15 +332,16 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
 constexpr int TC = 64; // tokens in a chunk
 
 struct __align__(64) MmaArgs {
-    CUtensorMap map[3][3]; // of a, b, c of each role
+    CUtensorMap map[3][4]; // of a, b, c, a2 of each role
     Args p;
 };
 
-template <int DA, int DC> struct MmaSmem {
+template <int DA, int DC, bool TWO> struct MmaSmem {
     static constexpr int TA = TC * DA * 2, TB = TC * DC * 2, LC = DC + 8; // tiles; pitch of the state, rows four banks on
     static constexpr int MT = DA > 64 ? DA / 64 : 1;
-    static constexpr int XP = 4 * 4 * 512, XS = 4 * 4 * MT * 3 * 512; // what warps of the same rows hand one another
-    static constexpr int A = 0, B = A + 2 * TA, C = B + 2 * TA, S = C + 2 * TB, P = S + 2 * DA * LC * 2, SP = P + XP, W = SP + XS,
+    static constexpr int XP = 10 * 512, XS = 4 * 4 * MT * 3 * 512; // what warps of the same rows hand one another
+    static constexpr int A = 0, B = A + 2 * TA, C = B + 2 * TA, A2 = C + 2 * TB, S = A2 + (TWO ? 2 * TB : 0), P = S + (TWO ? 1 : 2) * DA * LC * 2,
+                         P2 = P + XP, SP = P2 + (TWO ? XP : 0), W = SP + XS,
                          BAR = W + (2 * TC + 8) * 4, BYTES = BAR + 16 + 1024; // the tiles begin at a multiple of 1024
 };
 
@@ -399,10 +403,14 @@ __device__ __forceinline__ void split3(uint32_t v, float w0, float w1, uint32_t 
 
 // TMA: tiles come by tensor maps; otherwise (streams of one chunk, where there is nothing to fetch ahead and twelve maps
 // for a step cost the host 6 us) all threads copy 16 bytes at a time.
-template <int DA, int DC, bool STATES, bool TMA>
+// TWO: roles with a2 have a second result,
+//   o2_i = s_state l^(i+e1) a2_i S^T + s_pair sum_{j<=i} l^(i-j) (a2_i . c_j) b_j,
+// from the same tiles of b and c and the same state: dk beside dv.  One copy of the state's bf16 instead of two, so that two
+// such CTAs share an SM.
+template <int DA, int DC, bool STATES, bool TMA, bool TWO>
 __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kernel(const __grid_constant__ MmaArgs args)
 {
-    using SM = MmaSmem<DA, DC>;
+    using SM = MmaSmem<DA, DC, TWO>;
     constexpr int LC = SM::LC, NT = 4, MT = SM::MT, KS = DA / 16, THR = 4 * DC, CG = DC / 32;
     extern __shared__ __align__(16) unsigned char smraw[];
     __shared__ int abort_s, flag;
@@ -413,6 +421,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     const Args &p = args.p;
     const Role &q = p.role[blockIdx.z];
     const CUtensorMap *maps = args.map[blockIdx.z];
+    const bool two = TWO && !STATES && q.a2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
     // a scheduler's warps take rows r and 3 - r in turn: the triangle is dealt evenly
     const int cg = warp >> 2, r = cg & 1 ? 3 - (warp & 3) : warp & 3;
@@ -440,10 +449,12 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                 tile_copy<DA, THR>(base + SM::A + buf * SM::TA, reinterpret_cast<const bf16 *>(q.a) + b * q.lda + h * q.da, p.B * q.lda, q.da, t0, rows.n);
             tile_copy<DA, THR>(base + SM::B + buf * SM::TA, reinterpret_cast<const bf16 *>(q.b) + b * q.ldb + h * q.da, p.B * q.ldb, q.da, t0, rows.n);
             tile_copy<DC, THR>(base + SM::C + buf * SM::TB, reinterpret_cast<const bf16 *>(q.c) + b * q.ldc + h * q.dc, p.B * q.ldc, q.dc, t0, rows.n);
+            if (two)
+                tile_copy<DC, THR>(base + SM::A2 + buf * SM::TB, reinterpret_cast<const bf16 *>(q.a2) + b * q.lda2 + h * q.dc, p.B * q.lda2, q.dc, t0, rows.n);
             fa::cp_commit();
         } else if (tid == 0 && ok) {
             const uint32_t full = bar + 8 * buf;
-            tc::mbar_expect_tx(full, (STATES ? 1 : 2) * SM::TA + SM::TB);
+            tc::mbar_expect_tx(full, (STATES ? 1 : 2) * SM::TA + SM::TB + (two ? SM::TB : 0));
 #pragma unroll
             for (int x = 0; x < DA; x += 64) {
                 if (!STATES)
@@ -451,8 +462,11 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                 tma_load_4d(base + SM::B + buf * SM::TA + x * TC * 2, &maps[1], full, x, h, b, t0);
             }
 #pragma unroll
-            for (int x = 0; x < DC; x += 64)
+            for (int x = 0; x < DC; x += 64) {
                 tma_load_4d(base + SM::C + buf * SM::TB + x * TC * 2, &maps[2], full, x, h, b, t0);
+                if (two)
+                    tma_load_4d(base + SM::A2 + buf * SM::TB + x * TC * 2, &maps[3], full, x, h, b, t0);
+            }
         }
     };
     if (chunks)
@@ -522,7 +536,8 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     const uint32_t bt_at = base + SM::B + tile_at<DA>(row_of(lrow), 2 * r % (DA / 8) + lmid); // transposed: values 16 r
     const uint32_t c_at = base + SM::C + tile_at<DC>(row_of(l15), 4 * cg + lhi);           // transposed: rows 0 .. 15 of c
     const uint32_t s_at = base + SM::S + (l15 * LC + 32 * cg + lhi * 8) * 2;
-    uint4 *pairs = reinterpret_cast<uint4 *>(sm + SM::P) + r * 4 * 32 + lane;                  // fragments of this warp's rows
+    uint4 *pairs = reinterpret_cast<uint4 *>(sm + SM::P) + r * (r + 1) / 2 * 32 + lane;        // fragments of this warp's rows, keys not behind them
+    uint4 *pairs2 = reinterpret_cast<uint4 *>(sm + SM::P2) + r * (r + 1) / 2 * 32 + lane;
     uint4 *terms = reinterpret_cast<uint4 *>(sm + SM::SP) + r * 4 * MT * 3 * 32 + lane;
     if (p.n_seg > 1) {
         if (STATES) {
@@ -553,14 +568,16 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             for (int m = 0; m < MT; m++)
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    bf16 *to = Ss + buf * DA * LC + (16 * (r + 4 * m) + gq) * LC + 32 * cg + 8 * n + 2 * t;
+                    bf16 *to = Ss + (TWO ? 0 : buf) * DA * LC + (16 * (r + 4 * m) + gq) * LC + 32 * cg + 8 * n + 2 * t;
                     *reinterpret_cast<uint32_t *>(to) = fa::pack2(s[m][n][0], s[m][n][1]);
                     *reinterpret_cast<uint32_t *>(to + 8 * LC) = fa::pack2(s[m][n][2], s[m][n][3]);
                 }
     };
     publish(0);
     if (!STATES)
-        zero_behind<bf16>(p, q, rows, b, h, g, warp, THR / 32, lane);
+        zero_behind<bf16>(p, q.o, q.ldo, q.dc, rows, b, h, g, warp, THR / 32, lane);
+    if (two)
+        zero_behind<bf16>(p, q.o2, q.ldo2, q.da, rows, b, h, g, warp, THR / 32, lane);
 
     for (int k = 0; k < chunks; k++) {
         const int buf = k & 1, u0 = begin + k * TC, n = min(TC, end - u0);
@@ -579,16 +596,12 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
         if (!last)
             fetch(k + 1);
         const uint32_t At = a_at + buf * SM::TA, Bt = b_at + buf * SM::TA, Tt = bt_at + buf * SM::TA, Ct = c_at + buf * SM::TB,
-                       St = s_at + buf * DA * LC * 2;
+                       St = s_at + (TWO ? 0 : buf) * DA * LC * 2;
         const bool carries = has_state && (STATES || !last || q.s_end); // the state behind the chunk is of use
         const float *wt = wts + (last ? TC : 0);
-        float o[NT][4];
-        if (!STATES) {
-            // pair weights of every CG-th sixteen keys, for all warps of these rows
-            uint32_t aq[KS][4];
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-                ldsm4_at(aq[ks], (At ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128));
+        float o[NT][4], o2[TWO ? NT : 1][4];
+        // pair weights of every CG-th sixteen keys, for all warps of these rows: rows `u` against the tile's rows at v
+        auto weights = [&](const uint32_t (&u)[KS][4], uint32_t v, int step, uint4 *to) {
 #pragma unroll
             for (int i = 0; i < 4 / CG; i++) {
                 const int pc = cg + i * CG;
@@ -598,9 +611,9 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     uint32_t f[4];
-                    ldsm4_at(f, ((Bt ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128)) + pc * step_a);
-                    fa::mma(w[0], aq[ks], f[0], f[1]);
-                    fa::mma(w[1], aq[ks], f[2], f[3]);
+                    ldsm4_at(f, ((v ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128)) + pc * step);
+                    fa::mma(w[0], u[ks], f[0], f[1]);
+                    fa::mma(w[1], u[ks], f[2], f[3]);
                 }
                 if (pc == r) {
 #pragma unroll
@@ -616,15 +629,20 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                         for (int c = 0; c < 4; c++)
                             w[x][c] *= f * apart[(c >> 1) - x + 1][c & 1];
                 }
-                pairs[pc * 32] = make_uint4(fa::pack2(w[0][0], w[0][1]), fa::pack2(w[0][2], w[0][3]), fa::pack2(w[1][0], w[1][1]),
-                                            fa::pack2(w[1][2], w[1][3]));
+                to[pc * 32] = make_uint4(fa::pack2(w[0][0], w[0][1]), fa::pack2(w[0][2], w[0][3]), fa::pack2(w[1][0], w[1][1]),
+                                         fa::pack2(w[1][2], w[1][3]));
             }
+        };
+        if (!STATES) {
+            uint32_t aq[KS][4];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+                ldsm4_at(aq[ks], (At ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128));
+            weights(aq, Bt, step_a, pairs);
             // what the state gives
 #pragma unroll
             for (int x = 0; x < NT; x++)
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    o[x][c] = 0.0f;
+                o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
@@ -638,6 +656,33 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             for (int x = 0; x < NT; x++) {
                 o[x][0] *= f_a; o[x][1] *= f_a;
                 o[x][2] *= f_b; o[x][3] *= f_b;
+            }
+            if constexpr (TWO) {
+                static_assert(DA == DC, "");
+                if (two) {
+                    const uint32_t A2t = a_at - SM::A + SM::A2 + buf * SM::TB, C2t = b_at - SM::B + SM::C + buf * SM::TB;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++)
+                        ldsm4_at(aq[ks], (A2t ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128));
+                    weights(aq, C2t, step_c, pairs2);
+#pragma unroll
+                    for (int x = 0; x < NT; x++)
+                        o2[x][0] = o2[x][1] = o2[x][2] = o2[x][3] = 0.0f;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                        for (int x = 0; x < NT; x += 2) { // the state's rows are columns here
+                            uint32_t f[4];
+                            ldsm4_at(f, base + SM::S + ((32 * cg + 8 * x + lrow) * LC + ks * 16 + lmid * 8) * 2);
+                            fa::mma(o2[x], aq[ks], f[0], f[1]);
+                            fa::mma(o2[x + 1], aq[ks], f[2], f[3]);
+                        }
+#pragma unroll
+                    for (int x = 0; x < NT; x++) {
+                        o2[x][0] *= f_a; o2[x][1] *= f_a;
+                        o2[x][2] *= f_b; o2[x][3] *= f_b;
+                    }
+                }
             }
         }
         // decayed values of every CG-th sixteen tokens, in three terms
@@ -679,6 +724,18 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
             for (int x = 0; x < NT; x += 2)
                 ldsm4t_at(f[x / 2], (Ct ^ (x << 4)) + ks * step_c);
+            if constexpr (TWO)
+                if (two && ks <= r) {
+                    const uint4 u = pairs2[ks * 32];
+                    const uint32_t pf[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int x = 0; x < NT; x += 2) {
+                        uint32_t v[4];
+                        ldsm4t_at(v, ((c_at - SM::C + SM::B + buf * SM::TA) ^ (x << 4)) + ks * step_a);
+                        fa::mma(o2[x], pf, v[0], v[1]);
+                        fa::mma(o2[x + 1], pf, v[2], v[3]);
+                    }
+                }
             if (!STATES && ks <= r) {
                 const uint4 u = pairs[ks * 32];
                 const uint32_t pf[4] = {u.x, u.y, u.z, u.w};
@@ -709,25 +766,28 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
                     for (int c = 0; c < 4; c++)
                         s[m][x][c] = fmaf(l_n, s[m][x][c], add[m][x][c]);
-        if (!STATES) {
-            if (!ok)
-#pragma unroll
-                for (int x = 0; x < NT; x++)
-                    o[x][0] = o[x][1] = o[x][2] = o[x][3] = NAN;
-            // rows out: a quad's 32 columns in four pieces of 16 bytes
+        // rows out: a quad's 32 columns in four pieces of 16 bytes
+        auto rows_out = [&](const float (&x)[NT][4], void *out, long long ldo, int d) {
 #pragma unroll
             for (int c = 0; c < 4; c += 2) {
                 const int i = 16 * r + gq + 4 * c;
-                bf16 *to = reinterpret_cast<bf16 *>(q.o) + (i < n ? rows.row(u0 + i) * q.ldo : 0) + (size_t)h * q.dc + 32 * cg;
+                bf16 *to = reinterpret_cast<bf16 *>(out) + (i < n ? rows.row(u0 + i) * ldo : 0) + (size_t)h * d + 32 * cg;
                 uint32_t v[4];
 #pragma unroll
-                for (int x = 0; x < NT; x++)
-                    v[x] = fa::pack2(o[x][c], o[x][c + 1]);
+                for (int k = 0; k < NT; k++)
+                    v[k] = ok ? fa::pack2(x[k][c], x[k][c + 1]) : 0x7fff7fffu; // NaN behind a wait that ran out
                 fa::quad_transpose(v, t);
-                if (i < n && 32 * cg + 8 * t < q.dc)
+                if (i < n && 32 * cg + 8 * t < d)
                     *reinterpret_cast<uint4 *>(to + 8 * t) = make_uint4(v[0], v[1], v[2], v[3]);
             }
-        }
+        };
+        if (!STATES)
+            rows_out(o, q.o, q.ldo, q.dc);
+        if constexpr (TWO)
+            if (two)
+                rows_out(o2, q.o2, q.ldo2, q.da);
+        if (TWO && !STATES && !last)
+            __syncthreads(); // the state of this chunk has been read: its one place is free
         if (!last)
             publish(buf ^ 1);
     }

@@ -344,7 +344,9 @@ LINEAR_CASES = [  # streams, heads, d_key, d_value, tokens, lengths, states
     (2, 2, 16, 16, 9, (9, 0), 1), (1, 2, 64, 64, 63, None, 1), (3, 2, 64, 64, 64, None, 0), (2, 1, 64, 32, 65, (65, 64), 1), (1, 3, 32, 64, 128, (97,), 1),
     (2, 2, 128, 128, 130, (130, 1), 1), (1, 1, 128, 64, 200, None, 1), (2, 1, 8, 8, 77, (50, 77), 1), (1, 2, 96, 104, 150, (149,), 1),
     (1, 1, 5, 7, 100, None, 1), (1, 1, 64, 64, 1025, (1000,), 1), (2, 1, 128, 128, 700, (700, 333), 1), (1, 2, 32, 32, 513, None, 0),
-    (5, 3, 40, 16, 300, (0, 300, 63, 64, 299), 1), (1, 1, 16, 128, 2048, None, 1), (150, 1, 64, 64, 100, None, 1)]
+    (5, 3, 40, 16, 300, (0, 300, 63, 64, 299), 1), (1, 1, 16, 128, 2048, None, 1), (150, 1, 64, 64, 100, None, 1),
+    (2, 2, 40, 64, 333, (333, 100), 1), (13, 8, 64, 64, 50, (50, 0, 1, 49, 33, 50, 7, 50, 16, 17, 50, 2, 48), 1), (100, 1, 48, 56, 129, None, 0),
+    (3, 1, 64, 40, 700, (700, 0, 257), 1)]
 
 
 def _linear_data(case, kind, seed=5):
