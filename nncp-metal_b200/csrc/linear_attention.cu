@@ -53,7 +53,7 @@ static size_t lin_need(const nncu_linear_attn_shape *s, int roles)
         return 0;
     int n_seg, seg;
     lin_parts(s, roles, &n_seg, &seg);
-    return n_seg > 1 ? sizeof(float) * (size_t)roles * s->n_streams * s->n_head * n_seg * lin_slot(s) : 0;
+    return n_seg > 1 ? sizeof(float) * (size_t)roles * s->n_streams * s->n_head * (n_seg + 1) * lin_slot(s) : 0;
 }
 
 static int lin_common(const nncu_linear_attn_shape *s, int roles, const float *decay_host, const void *workspace, size_t workspace_bytes)
@@ -78,7 +78,7 @@ static lin::Args lin_args(const nncu_linear_attn_shape *s, int roles, const floa
     lin_parts(s, roles, &a.n_seg, &a.seg);
     a.slot = lin_slot(s);
     for (int i = 0; i < roles; i++)
-        a.role[i].parts = (float *)workspace + (size_t)i * a.B * a.H * a.n_seg * a.slot;
+        a.role[i].parts = (float *)workspace + (size_t)i * a.B * a.H * (a.n_seg + 1) * a.slot;
     for (int h = 0; h < s->n_head; h++)
         a.rate[h] = (float)log2((double)decay_host[h]);
     return a;
@@ -115,7 +115,7 @@ template <int DA, int DC, bool STATES, bool TMA, bool TWO> static int lin_mma_la
     constexpr int bytes = lin::MmaSmem<DA, DC, TWO>::BYTES;
     static DeviceOnce once;
     NNCU_TRY(smem_limit(once, lin::mma_kernel<DA, DC, STATES, TMA, TWO>, bytes));
-    CUDA_TRY(launch_k(lin::mma_kernel<DA, DC, STATES, TMA, TWO>, dim3(m.p.B * m.p.H, STATES ? m.p.n_seg - 1 : m.p.n_seg, roles), dim3(4 * DC), bytes, st, m));
+    CUDA_TRY(launch_k(lin::mma_kernel<DA, DC, STATES, TMA, TWO>, dim3(m.p.B * m.p.H, m.p.n_seg, roles), dim3(4 * DC), bytes, st, m));
     KERNEL_CHECK();
     return NNCU_OK;
 }

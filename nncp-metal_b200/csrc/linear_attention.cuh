@@ -36,7 +36,7 @@ struct Role {
     void *o;
     const float *s0;     // state before the first token, [B][H][da][dc] or, where s0_t, [B][H][dc][da]; NULL: zeros
     float *s_end;        // state behind the last token, [B][H][da][dc]; NULL: not wanted
-    float *parts;        // [B*H][n_seg][slot]: slot 0 the state before the first token, slot g what part g - 1 adds up to
+    float *parts;        // [B*H][n_seg + 1][slot]: slot 0 the state before the first token, slot g what part g - 1 adds up to
     const void *a2;      // not NULL: a second result of the same rows and state (kernels of two results)
     void *o2;
     long long lda, ldb, ldc, ldo, lda2, ldo2; // elements from row to row
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
         const int x = i / sm.dc4, y = i - x * sm.dc4;
         float s = 0.0f;
         if (x < q.da && y < q.dc) {
-            float *part = q.parts + pair * p.n_seg * p.slot + (size_t)x * q.dc + y;
+            float *part = q.parts + pair * (p.n_seg + 1) * p.slot + (size_t)x * q.dc + y;
             const float first = q.s0 && (p.n_seg == 1 || (STATES && g == 0)) ? state_at(q, q.s0 + pair * nn, x, y) : 0.0f;
             if (STATES && g == 0) // the state before the first token is kept: s_end may lie where it lies
                 *part = first;
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
             carry(std::integral_constant<int, 4>());
     }
     __syncthreads();
-    float *to = STATES ? q.parts + (pair * p.n_seg + g + 1) * p.slot : (q.s_end && ends_in(p, rows.n, g) ? q.s_end + pair * nn : nullptr);
+    float *to = STATES ? q.parts + (pair * (p.n_seg + 1) + g + 1) * p.slot : (q.s_end && ends_in(p, rows.n, g) ? q.s_end + pair * nn : nullptr);
     if (to)
         for (int i = tid; i < q.da * q.dc; i += 256)
             to[i] = Ss[i / q.dc * sm.ld_c + i % q.dc];
@@ -440,6 +440,8 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     pdl_wait(); // no early trigger: successors resident beside these CTAs cost more than their launch
     const Rows rows(p, q, b);
     const size_t nn = (size_t)q.da * q.dc;
+    if (STATES && !q.s_end && g == p.n_seg - 1) // nobody asks for the last part's sum
+        return;
     const int begin = g * p.seg, end = min(rows.n, begin + p.seg), total = max(end - begin, 0), chunks = (total + TC - 1) / TC;
     bool ok = true; // this thread's waits; behind one that ran out results are NaN and nothing more is asked for
     auto fetch = [&](int k) {
@@ -477,7 +479,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     float s[MT][NT][4];
     const bool has_state = r * 16 < DA; // of 32 rows the warps r = 2, 3 own none
     const bool first = p.n_seg == 1 || (STATES && g == 0);
-    float4 *part = reinterpret_cast<float4 *>(q.parts + pair * p.n_seg * p.slot) + tid;
+    float4 *part = reinterpret_cast<float4 *>(q.parts + pair * (p.n_seg + 1) * p.slot) + tid;
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -562,6 +564,37 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                     }
         }
     }
+    // fp32 values that lie as the state does, out
+    auto state_out = [&](const float (&x)[MT][NT][4]) {
+        float *to = q.s_end + pair * nn;
+        if (has_state)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int c = 0; c < 4; c += 2) {
+                        const int i = 16 * (r + 4 * m) + gq + 4 * c, y = 32 * cg + 8 * n + 2 * t;
+                        if (i < q.da && y < q.dc)
+                            *reinterpret_cast<float2 *>(to + i * q.dc + y) = make_float2(x[m][n][c], x[m][n][c + 1]);
+                    }
+    };
+    // Of several parts the last one's sum stands in the slot behind the others, exact to the third term: the state behind the
+    // last token is known before the first chunk, and the chunks need no third term.
+    const bool ends = q.s_end && ends_in(p, rows.n, g), follows = STATES || (q.s_end && p.n_seg == 1); // follows: s is a result
+    if (!STATES && ends && p.n_seg > 1) {
+        const float l_total = power(rate, total);
+        float x[MT][NT][4];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float4 f = part[(m * NT + n) * THR]; // behind the loop above: slot g + 1
+                x[m][n][0] = fmaf(l_total, s[m][n][0], f.x); x[m][n][1] = fmaf(l_total, s[m][n][1], f.y);
+                x[m][n][2] = fmaf(l_total, s[m][n][2], f.z); x[m][n][3] = fmaf(l_total, s[m][n][3], f.w);
+            }
+        state_out(x);
+    }
     auto publish = [&](int buf) {
         if (!STATES && has_state)
 #pragma unroll
@@ -597,7 +630,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             fetch(k + 1);
         const uint32_t At = a_at + buf * SM::TA, Bt = b_at + buf * SM::TA, Tt = bt_at + buf * SM::TA, Ct = c_at + buf * SM::TB,
                        St = s_at + (TWO ? 0 : buf) * DA * LC * 2;
-        const bool carries = has_state && (STATES || !last || q.s_end); // the state behind the chunk is of use
+        const bool carries = has_state && (follows || !last); // the state behind the chunk is of use
         const float *wt = wts + (last ? TC : 0);
         float o[NT][4], o2[TWO ? NT : 1][4];
         // pair weights of every CG-th sixteen keys, for all warps of these rows: rows `u` against the tile's rows at v
@@ -710,7 +743,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
         else
             __syncwarp();
         // the third term where a state is a result; 17 bits are more than the roundings behind them keep
-        const bool third = q.s_end != nullptr;
+        const bool third = follows && q.s_end;
         // what the chunk adds has sums of its own: products cut the sum they are added to, the state is rounded
         float add[MT][NT][4];
 #pragma unroll
@@ -807,18 +840,8 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
             for (int x = 0; x < NT; x++)
                 part[(m * NT + x) * THR] = make_float4(s[m][x][0], s[m][x][1], s[m][x][2], s[m][x][3]);
-    } else if (q.s_end && has_state && ends_in(p, rows.n, g)) {
-        float *to = q.s_end + pair * nn;
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int x = 0; x < NT; x++)
-#pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    const int i = 16 * (r + 4 * m) + gq + 4 * c, y = 32 * cg + 8 * x + 2 * t;
-                    if (i < q.da && y < q.dc)
-                        *reinterpret_cast<float2 *>(to + i * q.dc + y) = make_float2(s[m][x][c], s[m][x][c + 1]);
-                }
+    } else if (ends && p.n_seg == 1) {
+        state_out(s);
     }
 }
 
