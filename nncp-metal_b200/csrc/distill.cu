@@ -4,6 +4,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "distill.cuh"
 #include "op_checks.h"
@@ -24,11 +25,11 @@ static int distill_check(const nncu_distill_shape *s)
 // three places 78).  Some 1024 threads an SM share them.
 template <typename TZ, typename TG, int WHAT, int HARD> static int distill_launch(distill::Args &a, cudaStream_t st)
 {
-    const int entries = 2 * 3 * 4 * a.K4, fixed = entries + 4 * distill::PLACES + 2048; // static arrays and what a CTA costs
+    const int entries = 2 * 3 * 4 * a.K4, fixed = entries + 4 * distill::PLACES + 2560; // static arrays and what a CTA costs
     const long long row = (((long long)a.V * sizeof(TZ)) + 31) & ~15ll;
     if (row + fixed > SMEM_MOST) {
         a.slots = a.slot_bytes = 0;
-        CUDA_TRY(launch_k(distill::kernel<TZ, TG, WHAT, HARD, false>, dim3(a.N), dim3(distill::THREADS_MAX), (size_t)entries, st, a));
+        CUDA_TRY(launch_k(distill::kernel<TZ, TG, WHAT, HARD, false, false>, dim3(a.N), dim3(distill::THREADS_MAX), (size_t)entries, st, a));
         KERNEL_CHECK();
         return NNCU_OK;
     }
@@ -38,12 +39,16 @@ template <typename TZ, typename TG, int WHAT, int HARD> static int distill_launc
     while (threads < distill::THREADS_MAX && 2 * threads * ctas <= 1024)
         threads *= 2;
     a.slots = std::max(1, std::min(distill::SLOTS_MAX, (SMEM_MOST / ctas - fixed) / a.slot_bytes));
-    static DeviceOnce once;
-    NNCU_TRY(smem_limit(once, distill::kernel<TZ, TG, WHAT, HARD, true>, SMEM_MOST - 4 * distill::PLACES - 1024));
-    CUDA_TRY(launch_k(distill::kernel<TZ, TG, WHAT, HARD, true>, dim3(std::min(a.N, ctas * SMS)), dim3(threads), (size_t)a.slots * a.slot_bytes + entries,
-                      st, a));
-    KERNEL_CHECK();
-    return NNCU_OK;
+    const int grid = std::min(a.N, ctas * SMS);
+    auto launch = [&](auto late) {
+        constexpr bool LATE = decltype(late)::value;
+        static DeviceOnce once;
+        NNCU_TRY(smem_limit(once, distill::kernel<TZ, TG, WHAT, HARD, true, LATE>, SMEM_MOST - 4 * distill::PLACES - 1536));
+        CUDA_TRY(launch_k(distill::kernel<TZ, TG, WHAT, HARD, true, LATE>, dim3(grid), dim3(threads), (size_t)a.slots * a.slot_bytes + entries, st, a));
+        KERNEL_CHECK();
+        return (int)NNCU_OK;
+    };
+    return (WHAT & distill::GRAD) && a.N > grid ? launch(std::bool_constant<(WHAT & distill::GRAD) != 0>()) : launch(std::false_type());
 }
 
 template <typename TZ, typename TG, int WHAT> static int distill_run(distill::Args &a, cudaStream_t st)

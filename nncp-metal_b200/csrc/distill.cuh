@@ -105,18 +105,30 @@ struct Entries {
     float *e, *z;
 };
 
+// What the symbols that entries name are computed again from
+struct Kept {
+    float g, g_tau, inv_e, f, shift, shift1; // of what p is over, of e, of e_k; the target's; shifts of e and p
+    int target, any;
+    void *dz;
+};
+
 // RING: rows through shared memory; otherwise rows too long for it are read from global memory each time, one to a CTA.
+//
+// LATE: what the entries' symbols get is computed while the next row is on its way, from what the warps have kept, and not
+// before the dense gradient: for CTAs of several rows (2048 of 16384 fp32 logits: 49.0 -> 46.2 us; at one row a CTA there is
+// nothing to wait for, 650 of 9208 bf16 logits, loss and gradient apart: 12.65 -> 13.0).
 //
 // Two barriers a row.  What one row leaves for behind a barrier -- the named entries over its dense gradient, its place in the
 // ring for the next copy -- is done behind the first one of the next row; entries and partial sums lie in two
 // places that rows take in turn.
-template <typename TZ, typename TG, int WHAT, int HARD, bool RING>
+template <typename TZ, typename TG, int WHAT, int HARD, bool RING, bool LATE>
 __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__ Args a)
 {
     extern __shared__ __align__(128) unsigned char ring[]; // rows, then twice the entries: symbols, e, the student's logits
     __shared__ float red[2][6 * 16];
     __shared__ __align__(8) uint64_t bars[SLOTS_MAX];
     __shared__ int abort_s, flag;
+    __shared__ Kept kept[LATE ? THREADS_MAX / 32 : 1]; // each warp's of the row before
     __shared__ __align__(4) uint16_t last[PLACES], many[PLACES]; // of the entries of a place: one of them; the row in which it had several
     const int tid = threadIdx.x, thr = blockDim.x, V = a.V, K = a.K;
     const uint32_t bar0 = fa::smem_addr(bars), ring0 = fa::smem_addr(ring);
@@ -169,6 +181,48 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
     };
     const float scale = LOG2E * a.inv_tau;
     const bool defer = K + 1 <= 2 * thr; // a thread keeps two entries at most
+    const int warp_at = tid & ~31;
+    const bool names = (WHAT & GRAD) && defer && warp_at <= K;
+    if (LATE && names && tid == warp_at)
+        kept[tid >> 5].any = 0;
+    auto soft_at = [&](float v, float shift) { return ex2(fmaf(v, scale, -shift)); };
+    auto hard_at = [&](float v, float e, float shift1) { return HARD == SAME ? e : HARD == SQUARE ? e * e : ex2(fmaf(v, LOG2E, -shift1)); };
+    auto entries = [&](int turn) {
+        Entries en;
+        en.id = reinterpret_cast<int32_t *>(ring + a.slots * a.slot_bytes) + turn * 3 * a.K4;
+        en.e = reinterpret_cast<float *>(en.id) + a.K4;
+        en.z = en.e + a.K4;
+        return en;
+    };
+    // The gradient of the symbol of entry k: f less at the target, and inv_e times the sum of e over all entries that
+    // name it.  The first of them writes.  Entries alone in their place are alone.
+    auto named = [&](const Kept &of, const Entries &en, uint16_t round, int k, TG *&to, float &value) {
+        const int id = k <= K ? en.id[k] : -1;
+        to = nullptr;
+        if (id < 0)
+            return;
+        float off = en.e[k];
+        bool first = true;
+        if (many[(unsigned)id % PLACES] == round) {
+            off = 0.0f;
+#pragma unroll 1
+            for (int j = 0; j < a.K4; j += 4) {
+                const int4 like = *reinterpret_cast<const int4 *>(en.id + j);
+                if (like.x == id || like.y == id || like.z == id || like.w == id)
+                    for (int i = j; i < j + 4; i++)
+                        if (en.id[i] == id) {
+                            off += en.e[i];
+                            first = first && i >= k;
+                        }
+            }
+        }
+        if (first) {
+            const float e = soft_at(en.z[k], of.shift);
+            to = reinterpret_cast<TG *>(of.dz) + id;
+            value = (HARD == SAME ? (of.g + of.g_tau) * e : fmaf(of.g, hard_at(en.z[k], e, of.shift1), of.g_tau * e)) - (id == of.target ? of.f : 0.0f) -
+                    off * of.inv_e;
+        }
+    };
     long long r = blockIdx.x;
     for (int i = 0; i < a.slots; i++)
         fetch(i, r + (long long)i * gridDim.x);
@@ -177,6 +231,19 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
     TG *late[2] = {nullptr, nullptr}; // entries of the row before, to be written behind a barrier
     float late_value[2];
     uint16_t round = 0;
+    auto named_two = [&](const Kept &of, const Entries &en, uint16_t round) {
+        named(of, en, round, tid, late[0], late_value[0]);
+        if (warp_at + thr <= K)
+            named(of, en, round, tid + thr, late[1], late_value[1]);
+    };
+    auto named_before = [&]() { // the entries of the row before
+        if (LATE && names) {
+            __syncwarp();
+            const Kept of = kept[tid >> 5];
+            if (of.any)
+                named_two(of, entries(turn ^ 1), round - 1);
+        }
+    };
     for (; r < a.N; r += gridDim.x, turn ^= 1, round++) {
         const Side now = next;
         if (r + gridDim.x < a.N)
@@ -188,14 +255,12 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         const TZ *row = RING ? reinterpret_cast<const TZ *>(ring + slot * a.slot_bytes) : z + lo; // logit lo + i at row[i]
         const int pieces4 = (hi - lo) / 4, edge = tid < lo ? tid : tid < lo + V - hi ? hi + tid - lo : -1; // a logit at one of the ends
         const float z_edge = edge >= 0 ? to_f(z[edge]) : -INFINITY;
+        named_before(); // while this row is on its way
         if (RING)
             ok = ok && tc::mbar_wait(bar0 + 8 * slot, phase, &abort_s, &flag, 82);
         const float w = now.w;
         const bool known = now.target >= 0 && now.target < V;
-        Entries en;
-        en.id = reinterpret_cast<int32_t *>(ring + a.slots * a.slot_bytes) + turn * 3 * a.K4;
-        en.e = reinterpret_cast<float *>(en.id) + a.K4;
-        en.z = en.e + a.K4;
+        const Entries en = entries(turn);
         float most[2] = {z_edge, -INFINITY};
 #pragma unroll 1
         for (int k = tid; k < a.K4; k += thr) {
@@ -229,6 +294,8 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
             fetch(slot ? slot - 1 : a.slots - 1, r + (long long)(a.slots - 1) * gridDim.x);
         const float m = (WHAT & LOSS) ? most[0] : now.lse_tau * a.tau, mq = most[1];
         const bool none = w == 0.0f || ((WHAT & LOSS) ? most[0] : now.lse) == -INFINITY; // no weight, or a mask that leaves no symbol
+        if (LATE && names && tid == warp_at)
+            kept[tid >> 5].any = !none;
         if (none) {
             if ((WHAT & LOSS) && tid == 0) {
                 a.loss[r] = 0.0f;
@@ -241,8 +308,8 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         } else {
             float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f}; // of what p is over, of e, of e_k, the teacher's
             const float shift = rintf(m * scale), shift1 = rintf(m * LOG2E);
-            auto soft = [&](float v) { return ex2(fmaf(v, scale, -shift)); };
-            auto hard = [&](float v, float e) { return HARD == SAME ? e : HARD == SQUARE ? e * e : ex2(fmaf(v, LOG2E, -shift1)); };
+            auto soft = [&](float v) { return soft_at(v, shift); };
+            auto hard = [&](float v, float e) { return hard_at(v, e, shift1); };
             if constexpr (WHAT & LOSS) {
 #pragma unroll 4
                 for (int i = tid; i < pieces4; i += thr) {
@@ -308,38 +375,12 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
                     const float e = soft(v);
                     return HARD == SAME ? (g + g_tau) * e : HARD == SQUARE ? e * fmaf(g, e, g_tau) : fmaf(g, hard(v, e), g_tau * e);
                 };
-                // The gradient of the symbol of entry k: f less at the target, and inv_e times the sum of e over all entries that
-                // name it.  The first of them writes.  Entries alone in their place are alone.
-                auto named = [&](int k, TG *&to, float &value) {
-                    const int id = k <= K ? en.id[k] : -1;
-                    to = nullptr;
-                    if (id < 0)
-                        return;
-                    float off = en.e[k];
-                    bool first = true;
-                    if (many[(unsigned)id % PLACES] == round) {
-                        off = 0.0f;
-#pragma unroll 1
-                        for (int j = 0; j < a.K4; j += 4) {
-                            const int4 like = *reinterpret_cast<const int4 *>(en.id + j);
-                            if (like.x == id || like.y == id || like.z == id || like.w == id)
-                                for (int i = j; i < j + 4; i++)
-                                    if (en.id[i] == id) {
-                                        off += en.e[i];
-                                        first = first && i >= k;
-                                    }
-                        }
-                    }
-                    if (first) {
-                        to = dz + id;
-                        value = both(en.z[k]) - (id == now.target ? f : 0.0f) - off * inv_e;
-                    }
-                };
-                if (defer) {
-                    if (tid <= K)
-                        named(tid, late[0], late_value[0]);
-                    if (tid + thr <= K)
-                        named(tid + thr, late[1], late_value[1]);
+                const Kept of = {g, g_tau, inv_e, f, shift, shift1, now.target, 1, dz};
+                if (names) {
+                    if (!LATE)
+                        named_two(of, entries(turn), round);
+                    else if (tid == warp_at)
+                        kept[tid >> 5] = of;
                 }
                 TG *to = dz + lo;
                 if (reinterpret_cast<uintptr_t>(to) % (4 * sizeof(TG)) == 0) {
@@ -364,7 +405,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
                     for (int k = tid; k <= K; k += thr) {
                         TG *at;
                         float value;
-                        named(k, at, value);
+                        named(of, en, round, k, at, value);
                         if (at)
                             *at = from_f<TG>(value);
                     }
@@ -381,6 +422,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         }
     }
     if constexpr (WHAT & GRAD) {
+        named_before();
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 2; i++)
