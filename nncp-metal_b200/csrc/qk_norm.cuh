@@ -92,13 +92,14 @@ template <int W, bool ADJACENT> struct Place {
     }
 };
 
-// N floats of shared memory; four at a time where they lie so
-template <int N, bool QUADS> __device__ __forceinline__ void floats(float (&v)[N], const float *p)
+// A lane's N floats of shared memory; four at a time where they lie so, `apart` floats from four to four: the lanes' fours
+// stand side by side, and a warp's read touches each bank once
+template <int N, bool QUADS> __device__ __forceinline__ void floats(float (&v)[N], const float *p, int apart)
 {
     if constexpr (QUADS) {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const float4 f = *reinterpret_cast<const float4 *>(p + i);
+            const float4 f = *reinterpret_cast<const float4 *>(p + i / 4 * apart);
             v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
         }
     } else {
@@ -108,11 +109,18 @@ template <int N, bool QUADS> __device__ __forceinline__ void floats(float (&v)[N
     }
 }
 
+// Where pair p's angle lies among a row's, n lanes of W pairs: two pairs of each lane, then the next two
+template <int W> __device__ __forceinline__ int angle_at(int p, int n)
+{
+    const int k = p % W;
+    return W < 2 ? p : (k / 2 * n + p / W) * 2 + k % 2;
+}
+
 // the W pairs of a lane turned by the angles at cs (cosine, sine); TO: +1 there, -1 back.  x[0], x[1]: the two runs
-template <int W, int TO, bool ADJACENT> __device__ __forceinline__ void turn(float (&x)[2][W], const float2 *cs)
+template <int W, int TO, bool ADJACENT> __device__ __forceinline__ void turn(float (&x)[2][W], const float2 *cs, int n)
 {
     float at[2 * W];
-    floats<2 * W, (W >= 2)>(at, reinterpret_cast<const float *>(cs));
+    floats<2 * W, (W >= 2)>(at, reinterpret_cast<const float *>(cs), 4 * n);
     if constexpr (ADJACENT) { // pair k: values 2k, 2k + 1 of both runs in a row
 #pragma unroll
         for (int k = 0; k < W; k++) {
@@ -134,7 +142,7 @@ template <int W, int TO, bool ADJACENT> __device__ __forceinline__ void turn(flo
 
 // Cosines and sines of rows r0 .. r0 + n - 1, [n][d / 2] (one and zero for pairs that are only normed), and which of them
 // are no padding
-__device__ __forceinline__ void angles(const Args &a, float2 *cs, int *live, int r0, int n, int tid)
+template <int W> __device__ __forceinline__ void angles(const Args &a, float2 *cs, int *live, int r0, int n, int tid)
 {
     const int half = a.d / 2;
     for (int i = tid; i < n * half; i += 256) {
@@ -144,7 +152,7 @@ __device__ __forceinline__ void angles(const Args &a, float2 *cs, int *live, int
             const double t = (double)a.pos[r0 + r] * a.turns[p];
             sincospif((float)(2.0 * (t - rint(t))), &s, &c);
         }
-        cs[i] = make_float2(c, s);
+        cs[r * half + angle_at<W>(p, half / W)] = make_float2(c, s);
     }
     if (tid < n)
         live[tid] = !a.pos || a.pos[r0 + tid] >= 0;
@@ -177,8 +185,17 @@ __global__ void __launch_bounds__(256, BACK ? 2 : 4) kernel(const __grid_constan
     }
     const float inv_d = 1.0f / (float)a.d;
     pdl_wait();
-    for (int i = tid; i < a.d; i += 256)
-        gain[i] = a.gain[what] ? a.gain[what][i] : 1.0f;
+    const int n_lanes = half / W;
+    if (tid < G) // runs one behind the other; in each the lanes' first fours, then their second fours
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+            if (mine[g])
+#pragma unroll
+                for (int k = 0; k < W; k++) {
+                    const int to = W < 4 ? p0[g] + k : (k / 4 * n_lanes + p0[g] / W) * 4 + k % 4;
+                    gain[to] = a.gain[what] ? a.gain[what][lo[g] + k] : 1.0f;
+                    gain[half + to] = a.gain[what] ? a.gain[what][hi[g] + k] : 1.0f;
+                }
     float acc[NG][2][W] = {};
     struct Item {
         raw_t<T, W> x[NG][2], dy[BACK ? NG : 1][2];
@@ -216,7 +233,7 @@ __global__ void __launch_bounds__(256, BACK ? 2 : 4) kernel(const __grid_constan
         if (warp * per_warp < heads)
             next = fetch(warp * per_warp);
         __syncthreads();
-        angles(a, cs, live, r0, n, tid);
+        angles<W>(a, cs, live, r0, n, tid);
         __syncthreads();
 #pragma unroll 1
         for (int i0 = warp * per_warp; i0 < heads; i0 += 8 * per_warp) { // all lanes of a warp go through every round (shuffles)
@@ -256,11 +273,11 @@ __global__ void __launch_bounds__(256, BACK ? 2 : 4) kernel(const __grid_constan
                     continue;
                 const int p = mine[g] ? p0[g] : 0;
                 if (BACK)
-                    turn<W, -1, ADJACENT>(u[g], turns + p);
+                    turn<W, -1, ADJACENT>(u[g], turns + (W < 2 ? p : p / W * 2), n_lanes);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     float by[W];
-                    floats<W, (W >= 4)>(by, gain + (j ? hi[g] : lo[g]));
+                    floats<W, (W >= 4)>(by, gain + j * half + (W < 4 ? p : p / W * 4), 4 * n_lanes);
 #pragma unroll
                     for (int k = 0; k < W; k++) {
                         x[g][j][k] *= rs;
@@ -274,7 +291,7 @@ __global__ void __launch_bounds__(256, BACK ? 2 : 4) kernel(const __grid_constan
                     }
                 }
                 if (!BACK)
-                    turn<W, 1, ADJACENT>(u[g], turns + p);
+                    turn<W, 1, ADJACENT>(u[g], turns + (W < 2 ? p : p / W * 2), n_lanes);
             }
             if (BACK) {
                 for (int o = G / 2; o > 0; o >>= 1)
