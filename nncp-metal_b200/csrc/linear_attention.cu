@@ -98,14 +98,26 @@ template <typename T, int VEC> static int lin_step(const lin::Args &a, int roles
     return NNCU_OK;
 }
 
-template <typename T, bool STATES, bool PIECES> static int lin_core(const lin::Args &a, int roles, cudaStream_t st)
+template <typename T, bool STATES> static int lin_core(const lin::Args &a, int roles, cudaStream_t st)
 {
     static DeviceOnce once;
-    NNCU_TRY(smem_limit(once, lin::core_kernel<T, STATES, PIECES>, 4 * lin::CoreSmem(lin::DIM_MAX, lin::DIM_MAX, PIECES).floats));
+    NNCU_TRY(smem_limit(once, lin::core_kernel<T, STATES>, 4 * lin::CoreSmem(lin::DIM_MAX, lin::DIM_MAX).floats));
     int floats = 0;
     for (int i = 0; i < roles; i++)
-        floats = std::max(floats, lin::CoreSmem(a.role[i].da, a.role[i].dc, PIECES).floats);
-    CUDA_TRY(launch_k(lin::core_kernel<T, STATES, PIECES>, dim3(a.B * a.H, STATES ? a.n_seg - 1 : a.n_seg, roles), dim3(256), 4 * floats, st, a));
+        floats = std::max(floats, lin::CoreSmem(a.role[i].da, a.role[i].dc).floats);
+    CUDA_TRY(launch_k(lin::core_kernel<T, STATES>, dim3(a.B * a.H, STATES ? a.n_seg - 1 : a.n_seg, roles), dim3(256), 4 * floats, st, a));
+    KERNEL_CHECK();
+    return NNCU_OK;
+}
+
+template <bool STATES> static int lin_quad(const lin::Args &a, int roles, cudaStream_t st)
+{
+    static DeviceOnce once;
+    NNCU_TRY(smem_limit(once, lin::quad_kernel<STATES>, 4 * lin::QuadSmem(lin::DIM_MAX, lin::DIM_MAX).floats));
+    int floats = 0;
+    for (int i = 0; i < roles; i++)
+        floats = std::max(floats, lin::QuadSmem(a.role[i].da, a.role[i].dc).floats);
+    CUDA_TRY(launch_k(lin::quad_kernel<STATES>, dim3(a.B * a.H, STATES ? a.n_seg - 1 : a.n_seg, roles), dim3(32 * ceil_div(a.role[0].dc, 16)), 4 * floats, st, a));
     KERNEL_CHECK();
     return NNCU_OK;
 }
@@ -202,12 +214,12 @@ template <typename T> static int lin_run(const lin::Args &a, int roles, cudaStre
     if constexpr (sizeof(T) == 4)
         if (quads) {
             if (a.n_seg > 1)
-                NNCU_TRY((lin_core<T, true, true>(a, roles, st)));
-            return lin_core<T, false, true>(a, roles, st);
+                NNCU_TRY(lin_quad<true>(a, roles, st));
+            return lin_quad<false>(a, roles, st);
         }
     if (a.n_seg > 1)
-        NNCU_TRY((lin_core<T, true, false>(a, roles, st)));
-    return lin_core<T, false, false>(a, roles, st);
+        NNCU_TRY((lin_core<T, true>(a, roles, st)));
+    return lin_core<T, false>(a, roles, st);
 }
 
 static int lin_any(const nncu_linear_attn_shape *s, const lin::Args &a, int roles, cudaStream_t st)

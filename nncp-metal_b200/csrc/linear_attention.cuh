@@ -92,44 +92,34 @@ __device__ __forceinline__ float state_at(const Role &q, const float *s, int i, 
 // ends in part 0.
 __device__ __forceinline__ bool ends_in(const Args &p, int n, int g) { return g * p.seg < max(n, 1) && max(n, 1) <= g * p.seg + p.seg; }
 
-// ---------------- CUDA cores: fp32, and bf16 whose rows are not laid out in 16-byte pieces ----------------
+// ---------------- CUDA cores: rows that are not laid out in 16-byte pieces ----------------
 //
 // A CTA of 256 threads goes through one part of one (stream, head) in chunks of 32 tokens; tiles and state are fp32 in
 // shared memory, a thread takes 2 x 2 pair weights and 4 x 4 results or 8 x 4 elements of the state at a time.  Bound by
 // fp32 arithmetic and its shared-memory reads (eight of 16 bytes for 64 multiply-adds of a result).
-// fp32 rows laid out in 16-byte pieces (PIECES) are copied asynchronously, the next chunk's under the present one.
 
 constexpr int FC = 32; // tokens in a chunk
 
 struct CoreSmem {
     int da4, dc4, ld_a, ld_c, tile, b, c, s, p, w, floats;
-    __host__ __device__ CoreSmem(int da, int dc, bool twice)
+    __host__ __device__ CoreSmem(int da, int dc)
     {
         da4 = (da + 3) & ~3; dc4 = (dc + 3) & ~3;
         ld_a = da4 + 4; ld_c = dc4 + 4; // rows four banks on
         b = FC * ld_a; c = b + FC * ld_a; tile = c + FC * ld_c;
-        s = twice ? 2 * tile : tile; p = s + da4 * ld_c; w = p + FC * (FC + 4);
+        s = tile; p = s + da4 * ld_c; w = p + FC * (FC + 4);
         floats = w + 2 * (FC + 2);
     }
 };
 
 // 32 rows of a matrix as a tile, zeros behind row n and column d
-template <typename T, bool PIECES>
+template <typename T>
 __device__ __forceinline__ void core_load(float *dst, int ld, int d4, int d, const void *src, long long ldr, int h, const Rows &rows, int u0, int n)
 {
     const T *base = reinterpret_cast<const T *>(src) + (size_t)h * d;
-    if constexpr (PIECES) {
-        const int q4 = d4 / 4;
-        for (int i = threadIdx.x; i < FC * q4; i += 256) {
-            const int r = i / q4, x = (i - r * q4) * 4;
-            const bool ok = r < n;
-            fa::cp16(dst + r * ld + x, base + (ok ? rows.row(u0 + r) * ldr + x : 0), ok);
-        }
-    } else {
-        for (int i = threadIdx.x; i < FC * d4; i += 256) {
-            const int r = i / d4, x = i - r * d4;
-            dst[r * ld + x] = r < n && x < d ? to_f(base[rows.row(u0 + r) * ldr + x]) : 0.0f;
-        }
+    for (int i = threadIdx.x; i < FC * d4; i += 256) {
+        const int r = i / d4, x = i - r * d4;
+        dst[r * ld + x] = r < n && x < d ? to_f(base[rows.row(u0 + r) * ldr + x]) : 0.0f;
     }
 }
 
@@ -144,12 +134,12 @@ __device__ __forceinline__ float dot4(const float4 &u, const float4 &v, float s)
 }
 
 // STATES: the first pass over a sequence in several parts: what each part but the last adds to the state
-template <typename T, bool STATES, bool PIECES>
+template <typename T, bool STATES>
 __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args p)
 {
     extern __shared__ __align__(16) float smf[];
     const Role &q = p.role[blockIdx.z];
-    const CoreSmem sm(q.da, q.dc, PIECES);
+    const CoreSmem sm(q.da, q.dc);
     float *Ss = smf + sm.s, *Ps = smf + sm.p, *pw = smf + sm.w, *wt = pw + FC + 2;
     constexpr int LP = FC + 4;
     const int tid = threadIdx.x;
@@ -160,17 +150,7 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
     const Rows rows(p, q, b);
     const size_t nn = (size_t)q.da * q.dc;
     const int begin = g * p.seg, end = min(rows.n, begin + p.seg);
-    auto fetch = [&](int u0, float *to) {
-        const int n = end - u0;
-        if (!STATES)
-            core_load<T, PIECES>(to, sm.ld_a, sm.da4, q.da, q.a, q.lda, h, rows, u0, n);
-        core_load<T, PIECES>(to + sm.b, sm.ld_a, sm.da4, q.da, q.b, q.ldb, h, rows, u0, n);
-        core_load<T, PIECES>(to + sm.c, sm.ld_c, sm.dc4, q.dc, q.c, q.ldc, h, rows, u0, n);
-        if (PIECES)
-            fa::cp_commit();
-    };
-    if (PIECES && begin < end)
-        fetch(begin, smf);
+    float *As = smf, *Bs = As + sm.b, *Cs = As + sm.c;
     const float l_seg = power(rate, p.seg);
     for (int i = tid; i < FC + 2; i += 256)
         pw[i] = power(rate, i);
@@ -193,19 +173,14 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
     }
     if (!STATES)
         zero_behind<T>(p, q.o, q.ldo, q.dc, rows, b, h, g, tid >> 5, 8, tid & 31);
-    int turn = 0;
-    for (int u0 = begin; u0 < end; u0 += FC, turn ^= PIECES) {
+    for (int u0 = begin; u0 < end; u0 += FC) {
         const int n = min(FC, end - u0);
-        float *As = smf + turn * sm.tile, *Bs = As + sm.b, *Cs = As + sm.c;
-        if (PIECES) {
-            fa::cp_wait<0>();
-        } else {
-            __syncthreads(); // the chunk before has been read
-            fetch(u0, As);
-        }
+        __syncthreads(); // the chunk before has been read
+        if (!STATES)
+            core_load<T>(As, sm.ld_a, sm.da4, q.da, q.a, q.lda, h, rows, u0, n);
+        core_load<T>(Bs, sm.ld_a, sm.da4, q.da, q.b, q.ldb, h, rows, u0, n);
+        core_load<T>(Cs, sm.ld_c, sm.dc4, q.dc, q.c, q.ldc, h, rows, u0, n);
         __syncthreads();
-        if (PIECES && u0 + FC < end)
-            fetch(u0 + FC, smf + (turn ^ 1) * sm.tile);
         if (tid < FC)
             wt[tid] = tid < n ? q.s_in * pw[n - 1 - tid + q.e2] : 0.0f;
         if (!STATES) {
@@ -257,15 +232,11 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
                 for (int r = 0; r < R; r++)
                     if (i0 + r < n) {
                         T *to = reinterpret_cast<T *>(q.o) + rows.row(u0 + i0 + r) * q.ldo + (size_t)h * q.dc + c0;
-                        if constexpr (PIECES) {
-                            *reinterpret_cast<float4 *>(to) = o[r];
-                        } else {
-                            const float v[4] = {o[r].x, o[r].y, o[r].z, o[r].w};
+                        const float v[4] = {o[r].x, o[r].y, o[r].z, o[r].w};
 #pragma unroll
-                            for (int c = 0; c < 4; c++)
-                                if (c0 + c < q.dc)
-                                    to[c] = from_f<T>(v[c]);
-                        }
+                        for (int c = 0; c < 4; c++)
+                            if (c0 + c < q.dc)
+                                to[c] = from_f<T>(v[c]);
                     }
             }
         }
@@ -313,6 +284,305 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
     if (to)
         for (int i = tid; i < q.da * q.dc; i += 256)
             to[i] = Ss[i / q.dc * sm.ld_c + i % q.dc];
+}
+
+// ---------------- fp32 on warp-level tensor-core products ----------------
+//
+// A CTA goes through one part of one (stream, head) in chunks of 32 tokens, rows in 16-byte pieces copied asynchronously, the
+// next chunk's under the present one.  An fp32 value is two tf32 values of 11 bits and a rest of 2^-22 of it at most; a
+// product of two takes three tf32 products (high by high in one sum, the mixed ones in another), the fourth is below 2^-22 too.
+// Each warp has sixteen columns of the results and of the state, so that a split left factor serves four products of tiles.  The
+// state stays in shared memory in fp32: what a chunk adds to it has sums of its own, since products cut the sum that they
+// are added to.
+//
+// Tiles [token][value] lie with rows four banks on where products take them by rows (a, b) and eight banks on where by
+// columns (c, the state): a fragment's 32 words touch 32 banks.  Only b as the state's left factor goes two to a bank.
+
+struct QuadSmem {
+    int da16, dc16, ld_a, ld_c, tile, b, c, s, p, w, floats;
+    __host__ __device__ QuadSmem(int da, int dc)
+    {
+        da16 = (da + 15) & ~15; dc16 = (dc + 15) & ~15;
+        ld_a = da16 + 4; ld_c = dc16 + 8;
+        b = FC * ld_a; c = b + FC * ld_a; tile = c + FC * ld_c;
+        s = 2 * tile; p = s + da16 * ld_c; w = p + FC * (FC + 4);
+        floats = w + FC + 4;
+    }
+};
+
+// This thread's fours of a matrix that all threads of a CTA go through: column x of rows r, r + step, ...
+struct Fours {
+    int r, x, step;
+    __device__ __forceinline__ explicit Fours(int columns)
+    {
+        const int n = columns / 4;
+        step = blockDim.x / n;
+        r = threadIdx.x / n;
+        x = (threadIdx.x - r * n) * 4;
+        if (r >= step) // threads of no whole row
+            r = 1 << 30;
+    }
+};
+
+// 32 rows of a matrix as a tile, zeros behind row n and column d
+__device__ __forceinline__ void quad_load(float *dst, int ld, const Fours &f, int d, const void *src, long long ldr, int h, const Rows &rows, int u0, int n)
+{
+    if (f.r >= FC)
+        return;
+    const float *base = reinterpret_cast<const float *>(src) + (size_t)h * d + (f.x < d ? f.x : 0), *from = base + rows.row(u0 + f.r) * ldr;
+    const long long step = f.step * rows.step * ldr;
+    for (int r = f.r; r < FC; r += f.step, from += step)
+        fa::cp16(dst + r * ld + f.x, r < n ? from : base, r < n && f.x < d);
+}
+
+struct Two {
+    uint32_t hi, lo;
+    __device__ __forceinline__ Two() {}
+    __device__ __forceinline__ explicit Two(float x)
+    {
+        hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u; // to the nearest: halves go up
+        lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+    }
+};
+__device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 "
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16 x 16 sums, column groups x = 0, 1
+struct Sums {
+    float big[2][4], small[2][4];
+    __device__ __forceinline__ Sums()
+    {
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                big[x][c] = small[x][c] = 0.0f;
+    }
+    __device__ __forceinline__ void add(const Two (&a)[4], const Two (&b)[2][2])
+    {
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+            mma_tf32(small[x], a[0].lo, a[1].lo, a[2].lo, a[3].lo, b[x][0].hi, b[x][1].hi);
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+            mma_tf32(big[x], a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[x][0].hi, b[x][1].hi);
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+            mma_tf32(small[x], a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[x][0].lo, b[x][1].lo);
+    }
+    __device__ __forceinline__ float sum(int x, int c) const { return big[x][c] + small[x][c]; }
+};
+// fragments: at is this lane's first value; `row` and `k` go from row (column) to row and from one contracted place to the next
+__device__ __forceinline__ void left16(Two (&a)[4], const float *at, int row, int k)
+{
+    a[0] = Two(at[0]);
+    a[1] = Two(at[8 * row]);
+    a[2] = Two(at[4 * k]);
+    a[3] = Two(at[8 * row + 4 * k]);
+}
+__device__ __forceinline__ void right16(Two (&b)[2][2], const float *at, int column, int k)
+{
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        b[x][0] = Two(at[8 * x * column]);
+        b[x][1] = Two(at[8 * x * column + 4 * k]);
+    }
+}
+
+// A warp for each sixteen columns of c.  Parts hold states as [da16][dc16].
+template <bool STATES> __global__ void __launch_bounds__(256) quad_kernel(const __grid_constant__ Args p)
+{
+    extern __shared__ __align__(16) float smf[];
+    const Role &q = p.role[blockIdx.z];
+    const QuadSmem sm(q.da, q.dc);
+    float *Ss = smf + sm.s, *Ps = smf + sm.p, *pw = smf + sm.w;
+    constexpr int LP = FC + 4;
+    const int tid = threadIdx.x, thr = blockDim.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, t = lane & 3, y0 = 16 * warp;
+    const size_t pair = blockIdx.x;
+    const int g = blockIdx.y, b = (int)(pair / p.H), h = (int)(pair % p.H);
+    const float rate = p.rate[h];
+    const int a_steps = (q.da + 7) / 8;
+    const Fours fours_a(sm.da16), fours_c(sm.dc16);
+    pdl_wait();
+    const Rows rows(p, q, b);
+    const size_t nn = (size_t)q.da * q.dc;
+    const int begin = g * p.seg, end = min(rows.n, begin + p.seg);
+    auto fetch = [&](int u0, float *to) {
+        const int n = end - u0;
+        if (!STATES)
+            quad_load(to, sm.ld_a, fours_a, q.da, q.a, q.lda, h, rows, u0, n);
+        quad_load(to + sm.b, sm.ld_a, fours_a, q.da, q.b, q.ldb, h, rows, u0, n);
+        quad_load(to + sm.c, sm.ld_c, fours_c, q.dc, q.c, q.ldc, h, rows, u0, n);
+        fa::cp_commit();
+    };
+    if (begin < end)
+        fetch(begin, smf);
+    const float l_seg = power(rate, p.seg);
+    for (int i = tid; i < FC + 2; i += thr)
+        pw[i] = power(rate, i);
+    // the state before this part, several rows at a time on their way
+    float *parts = p.n_seg > 1 ? q.parts + pair * (p.n_seg + 1) * p.slot : nullptr;
+    constexpr int WAY = 8;
+    for (int x0 = fours_c.r; x0 < sm.da16; x0 += WAY * fours_c.step) {
+        float4 s[WAY];
+#pragma unroll
+        for (int i = 0; i < WAY; i++) {
+            const int x = x0 + i * fours_c.step;
+            s[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (q.s0 && (p.n_seg == 1 || (STATES && g == 0)) && x < q.da && fours_c.x < q.dc) {
+                const float *s0 = q.s0 + pair * nn;
+                s[i] = make_float4(state_at(q, s0, x, fours_c.x), state_at(q, s0, x, fours_c.x + 1), state_at(q, s0, x, fours_c.x + 2),
+                                   state_at(q, s0, x, fours_c.x + 3));
+            }
+        }
+        if (p.n_seg > 1 && (!STATES || g == 0))
+            for (int k = 0; k <= g; k++) {
+#pragma unroll
+                for (int i = 0; i < WAY; i++) {
+                    const int x = x0 + i * fours_c.step;
+                    if (x < sm.da16) {
+                        float4 *at = reinterpret_cast<float4 *>(parts + (size_t)k * p.slot + (size_t)x * sm.dc16 + fours_c.x);
+                        if (STATES) { // the state before the first token is kept: s_end may lie where it lies
+                            *at = s[i];
+                            s[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        } else {
+                            const float4 f = *at;
+                            s[i].x = fmaf(l_seg, s[i].x, f.x); s[i].y = fmaf(l_seg, s[i].y, f.y);
+                            s[i].z = fmaf(l_seg, s[i].z, f.z); s[i].w = fmaf(l_seg, s[i].w, f.w);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < WAY; i++)
+            if (x0 + i * fours_c.step < sm.da16)
+                *reinterpret_cast<float4 *>(Ss + (x0 + i * fours_c.step) * sm.ld_c + fours_c.x) = s[i];
+    }
+    if (!STATES)
+        zero_behind<float>(p, q.o, q.ldo, q.dc, rows, b, h, g, warp, thr >> 5, lane);
+    int turn = 0;
+    for (int u0 = begin; u0 < end; u0 += FC, turn ^= 1) {
+        const int n = min(FC, end - u0);
+        const float *As = smf + turn * sm.tile, *Bs = As + sm.b, *Cs = As + sm.c + y0 + g4;
+        fa::cp_wait<0>();
+        __syncthreads(); // this chunk's tiles and the state stand, the chunk before has been read
+        if (u0 + FC < end)
+            fetch(u0 + FC, smf + (turn ^ 1) * sm.tile);
+        Two left[4], right[2][2];
+        if (!STATES) {
+            for (int it = warp; it < 3; it += thr >> 5) { // pair weights: sixteen rows by sixteen keys that are not all behind them
+                const int m = it > 0, k16 = it > 1;
+                const float *at = As + (16 * m + g4) * sm.ld_a + t, *bt = Bs + (16 * k16 + g4) * sm.ld_a + t;
+                Sums w;
+#pragma unroll 2
+                for (int ks = 0; ks < a_steps; ks++) {
+                    left16(left, at + 8 * ks, sm.ld_a, 1);
+                    right16(right, bt + 8 * ks, sm.ld_a, 1);
+                    w.add(left, right);
+                }
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const int i = 16 * m + g4 + 4 * (c & 2), j = 16 * k16 + 8 * x + 2 * t + (c & 1);
+                        Ps[i * LP + j] = j <= i ? w.sum(x, c) * q.s_pair * pw[i - j] : 0.0f;
+                    }
+            }
+            // what the state gives
+            Sums o[2];
+            const float *at = As + g4 * sm.ld_a + t, *st = Ss + t * sm.ld_c + y0 + g4;
+#pragma unroll 2
+            for (int ks = 0; ks < a_steps; ks++) {
+                right16(right, st + 8 * ks * sm.ld_c, 1, sm.ld_c);
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+                    left16(left, at + 16 * m * sm.ld_a + 8 * ks, sm.ld_a, 1);
+                    o[m].add(left, right);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const float l = q.s_state * pw[16 * m + g4 + 4 * (c & 2) + q.e1];
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        o[m].big[x][c] *= l;
+                        o[m].small[x][c] *= l;
+                    }
+                }
+            __syncthreads(); // the weights stand, the state has been read
+#pragma unroll
+            for (int ks = 0; ks < FC / 8; ks++) {
+                right16(right, Cs + (8 * ks + t) * sm.ld_c, 1, sm.ld_c);
+#pragma unroll
+                for (int m = 0; m < 2; m++)
+                    if (ks < 2 * m + 2) {
+                        left16(left, Ps + (16 * m + g4) * LP + 8 * ks + t, LP, 1);
+                        o[m].add(left, right);
+                    }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int c = 0; c < 4; c += 2) {
+                    const int i = 16 * m + g4 + 4 * c;
+                    if (i < n) {
+                        float *to = reinterpret_cast<float *>(q.o) + rows.row(u0 + i) * q.ldo + (size_t)h * q.dc + y0 + 2 * t;
+#pragma unroll
+                        for (int x = 0; x < 2; x++)
+                            if (y0 + 8 * x + 2 * t < q.dc)
+                                *reinterpret_cast<float2 *>(to + 8 * x) = make_float2(o[m].sum(x, c), o[m].sum(x, c + 1));
+                    }
+                }
+            if (u0 + FC >= end && !q.s_end)
+                break;
+        }
+        const float l_n = pw[n];
+        Two weighted[FC / 8][2][2];
+#pragma unroll
+        for (int ks = 0; ks < FC / 8; ks++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int j = 8 * ks + t + 4 * c;
+                const float w = j < n ? q.s_in * pw[n - 1 - j + q.e2] : 0.0f;
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+                    weighted[ks][x][c] = Two(w * Cs[j * sm.ld_c + 8 * x]);
+            }
+#pragma unroll 1
+        for (int x0 = 0; x0 < q.da; x0 += 16) {
+            Sums add;
+#pragma unroll
+            for (int ks = 0; ks < FC / 8; ks++) {
+                left16(left, Bs + (8 * ks + t) * sm.ld_a + x0 + g4, 1, sm.ld_a);
+                add.add(left, weighted[ks]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c += 2)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    float2 *s = reinterpret_cast<float2 *>(Ss + (x0 + g4 + 4 * c) * sm.ld_c + y0 + 8 * x + 2 * t);
+                    const float2 now = *s;
+                    *s = make_float2(fmaf(l_n, now.x, add.sum(x, c)), fmaf(l_n, now.y, add.sum(x, c + 1)));
+                }
+        }
+    }
+    __syncthreads();
+    if (STATES) {
+        for (int x = fours_c.r; x < sm.da16; x += fours_c.step)
+            *reinterpret_cast<float4 *>(parts + (size_t)(g + 1) * p.slot + (size_t)x * sm.dc16 + fours_c.x) = quad(Ss + x * sm.ld_c + fours_c.x);
+    } else if (q.s_end && ends_in(p, rows.n, g) && fours_c.x < q.dc) {
+        for (int x = fours_c.r; x < q.da; x += fours_c.step) {
+            float *to = q.s_end + pair * nn + (size_t)x * q.dc + fours_c.x;
+            const float4 f = quad(Ss + x * sm.ld_c + fours_c.x);
+            to[0] = f.x; to[1] = f.y; to[2] = f.z; to[3] = f.w;
+        }
+    }
 }
 
 // ---------------- bf16 on warp-level tensor-core products ----------------
