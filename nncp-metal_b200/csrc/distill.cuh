@@ -9,11 +9,13 @@
 // the teacher's term is sum_k e_k ((top_k - maxtop) / tau - u_k ln 2) / sum e_k - ln sum e_k + ln l.  Two reductions over a
 // row, one of maxima and one of sums.
 //
-// Bound by HBM: the logits once in, the gradient once out.  A CTA stays and takes every gridDim.x-th row; the rows behind come
+// The bytes are the logits once in, the gradient once out.  A CTA stays and takes every gridDim.x-th row; the rows behind come
 // by bulk copy into `slots` places in shared memory while one is gone through three times there: maximum, sums,
 // gradient.  (A row that is loaded, reduced twice and stored in turn leaves HBM idle most of the time: 2048 rows of 16384
 // logits, loss and gradient, took 69 us with a row in the registers of a CTA.)  What of a row does not lie in whole
-// 16-byte pieces, at its two ends, is a thread's each.
+// 16-byte pieces, at its two ends, is a thread's each.  2048 rows of 16384 fp32 logits with a bf16 gradient, 64 entries a
+// row: 45 us, 201 MB at 4.5 TB/s; bound by the issue of instructions (25 for a logit, 11 of them in the three passes, the rest
+// a row's own) and by the barriers that a row's warps wait at for those with entries.
 //
 // Exponentials are what an SM has least of, sixteen a cycle.  Where tau is 1 or 2, or one of the terms is not there, p
 // is 2^u or its square over their sum: one exponential a logit and pass instead of two.

@@ -96,7 +96,8 @@ __device__ __forceinline__ bool ends_in(const Args &p, int n, int g) { return g 
 //
 // A CTA of 256 threads goes through one part of one (stream, head) in chunks of 32 tokens; tiles and state are fp32 in
 // shared memory, a thread takes 2 x 2 pair weights and 4 x 4 results or 8 x 4 elements of the state at a time.  Bound by
-// fp32 arithmetic and its shared-memory reads (eight of 16 bytes for 64 multiply-adds of a result).
+// latency: values come one by one, and a chunk is loaded before it is computed.  8 x 8 pairs of 512 tokens of 62, fp32,
+// forward: 91 us.
 
 constexpr int FC = 32; // tokens in a chunk
 
@@ -297,6 +298,11 @@ __global__ void __launch_bounds__(256) core_kernel(const __grid_constant__ Args 
 //
 // Tiles [token][value] lie with rows four banks on where products take them by rows (a, b) and eight banks on where by
 // columns (c, the state): a fragment's 32 words touch 32 banks.  Only b as the state's left factor goes two to a bank.
+//
+// Bound by the chain of a chunk's phases: of 14800 cycles at head size 128 the products take 7600 at the rate that this
+// instruction reaches (277 TFLOP/s), the pair weights, which three warps compute, 3500, the next rows' copies 1200.
+// 8 x 8 pairs of 512 tokens of 64, forward: 37.5 us (on CUDA cores 70.6), with the backward pass 118 (257); 4 x 8 of
+// 1024 tokens of 128: 105 (228) and 371 (673).  Bulk copies of a row each instead of 16 bytes a thread: 57 us for 37.5.
 
 struct QuadSmem {
     int da16, dc16, ld_a, ld_c, tile, b, c, s, p, w, floats;
@@ -595,9 +601,14 @@ template <bool STATES> __global__ void __launch_bounds__(256) quad_kernel(const 
 // terms are the same for the CG warps of the same rows: each computes every CG-th and they meet at a barrier of their own.
 //
 // Tiles come by TMA, 64 tokens x 64 (32) values of a head a copy, from a map of (value, head, stream, token): what lies beyond
-// a head's values or the sequence arrives as zeros.  One thread asks for the next chunk's under the present chunk (copies
-// of 16 bytes by all threads took 2000 of a chunk's 4600 cycles, 128 pairs of head size 64); one barrier a chunk hands over
-// tiles and state.  In the reverse order a chunk's row i is the tile's row 63 - i.
+// a head's values or the sequence arrives as zeros.  One thread asks for the next chunk's under the present chunk; one
+// barrier a chunk hands over tiles and state.  In the reverse order a chunk's row i is the tile's row 63 - i.
+//
+// Bound by the chain of a chunk's phases (weights, what the state gives, products with c, the state to the next chunk) in
+// too few warps to hide it: the tensor pipe is active 40 to 52 % of the time, shared memory 44 to 66, an instruction
+// issues in 35 to 45.  8 x 16 pairs of 2048 tokens of 64, forward and backward: 190 us, 36 GFLOP of the chunk form's
+// products, the state's in two or three terms, 192 TFLOP/s of the 550 that this instruction reaches; the bytes alone 41.5 us.
+// 2 x 8 pairs of 4096 tokens of 128, forward, in eight parts: 69 us (both passes), bytes 10.5.
 
 constexpr int TC = 64; // tokens in a chunk
 
@@ -707,7 +718,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
         }
         __syncthreads();
     }
-    pdl_wait(); // no early trigger: successors resident beside these CTAs cost more than their launch
+    pdl_wait(); // no early trigger: successors resident beside these CTAs cost more than their launch (128 pairs of 2048 tokens 144 -> 97 us)
     const Rows rows(p, q, b);
     const size_t nn = (size_t)q.da * q.dc;
     if (STATES && !q.s_end && g == p.n_seg - 1) // nobody asks for the last part's sum
@@ -1119,7 +1130,8 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 //
 // A CTA of four warps takes 8 * VEC columns of one (stream, head)'s state into registers, sixteen rows side by side, and
 // goes through the tokens one after the other.  Bound by HBM: the state once in and once out, all of a thread's
-// loads in flight together.
+// loads in flight together.  One token of 128 x 8 states of 64 x 64, 34 MB: 7.3 us, 4.7 TB/s; of 4 x 4 of 32 x 32 2.6 us,
+// the latency of a launch and of one load behind another.
 
 constexpr int STEP_TOKENS = 8;
 

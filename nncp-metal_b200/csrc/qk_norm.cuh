@@ -5,10 +5,14 @@
 // R turns the pairs (i, i + d_rot / 2) -- or (2i, 2i + 1) -- of the first d_rot values by pos base^(-2i / d_rot).  The
 // adjoint turns back: u = R(-pos) dy, dgain = sum u x^, w = u gain, dx = (w - x^ mean(w x^)) / sqrt(mean(x^2) + eps).
 //
-// Bound by HBM: every value once in and once out (forward), twice in and once out (backward).  A head's row lies in
+// The bytes are every value once in and once out (forward), twice in and once out (backward).  A head's row lies in
 // the registers of G neighbouring lanes, each with both members of its pairs, so that neither the rotation nor a
 // second look at x costs memory; sines and cosines are taken once for a row and all its heads.  Angles are
 // reduced in 64 bits: positions of a large file leave no digit of an fp32 angle behind the point.
+//
+// Bound by the issue of instructions, some 20 for a value and pass, and by the waits for shared memory and shuffles between
+// them: 16384 rows of 16 + 16 heads of 64, bf16, forward 29.8 us (134 MB, 4.5 TB/s), backward with gains 47.4 (201 MB, 4.2).
+// Gains and angles as they come, four lanes to a bank, took 33.2 and 48.3.
 #pragma once
 #include "warp_mma.cuh"
 
