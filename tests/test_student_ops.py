@@ -445,6 +445,17 @@ def test_linear_attention_against_64_bits(pkg, case, kind):
 
 
 @gpu
+@pytest.mark.parametrize("case", [
+    (1, 2, 128, 128, 200, None, 1), (2, 1, 4, 128, 65, (65, 32), 1), (1, 2, 128, 4, 97, None, 0), (3, 2, 36, 100, 130, (130, 0, 31), 1),
+    (40, 4, 12, 20, 33, None, 1), (1, 1, 112, 116, 1000, (993,), 1), (2, 4, 68, 60, 300, (300, 129), 1), (60, 4, 64, 64, 40, None, 1)])
+def test_linear_attention_fp32_sizes(pkg, case):
+    """fp32 head sizes about the tiles of its products.  A product of two values in two parts of 11 bits is off by 2^-22 of it
+    for the part left out and 2^-23 for each rest: less than the steps that the tolerance counts"""
+    t, n, behind, decay, s0, ds, length = _linear_data(case, torch.float32, seed=6)
+    _check_linear(pkg, case, torch.float32, Linear(pkg, case, torch.float32, t, decay, s0, ds, length), t, n, behind, decay, s0, ds)
+
+
+@gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("T", [1, 70, 600])
 @pytest.mark.parametrize("shift", [0, 1])
@@ -638,6 +649,24 @@ def test_distillation_masks(pkg, kind, V):
     for x in got[1:]:
         assert bool((x[1, V // 2:] == 0).all())
     _distill_near(got[0], got[1:], want, grad, weight, 2.0, 0.6, kind, V)
+
+
+@gpu
+@pytest.mark.parametrize("N,V,K,kind,grad_kind,tau,share", [
+    (5000, 300, 20, torch.bfloat16, torch.bfloat16, 2.0, 0.7), (5000, 256, 200, torch.float32, torch.float32, 1.0, 0.5), (1400, 4096, 50, torch.float32, torch.bfloat16, 3.0, 0.7),
+    (1000, 16384, 64, torch.bfloat16, torch.float32, 2.0, 0.4), (500, 16385, 300, torch.float32, torch.bfloat16, 2.0, 1.0)])
+def test_distillation_of_more_rows_than_places(pkg, N, V, K, kind, grad_kind, tau, share):
+    """Rows that follow one another on an SM: some of them masked out, without a teacher or of weight 0, with symbols that
+    several entries name"""
+    z, ids, top, targets, weight = _distill_data(N, V, K, kind, seed=12)
+    ids[1::3, 1::2] = ids[1::3, :1]
+    ids[5::13] = -1
+    targets[4::9] = V
+    z[3::11] = -math.inf
+    weight[2::7] = 0.0
+    got = _distill_calls(pkg, z, ids, top, targets, weight, tau, share, grad_kind)
+    want, grad = _distill_ref(z, ids, top, targets, weight, tau, share)
+    _distill_near(got[0], got[1:], want, grad, weight, tau, share, grad_kind, V)
 
 
 @gpu
