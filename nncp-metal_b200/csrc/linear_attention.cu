@@ -25,15 +25,21 @@ static int lin_check(const nncu_linear_attn_shape *s)
 }
 
 // In how many parts a stream's tokens are cut.  One part is one pass over the tokens; more parts read b and c
-// twice, and pay where one CTA for each (stream, head) would leave most SMs without work.
+// twice, and pay where one CTA for each (stream, head) would leave most SMs without work.  Parts of one chunk while there are
+// 16 at most, of two behind that, since each goes through the sums of all before it (1 x 2 pairs of 1000 tokens of 128, bf16,
+// in 4, 8 and 16 parts: 37, 26 and 23 us; one pair of 4096 of 64 in 16, 32 and 64: 19.5, 18.0 and 24.2).
 static void lin_parts(const nncu_linear_attn_shape *s, int roles, int *n_seg, int *seg)
 {
     const long long ctas = (long long)s->n_streams * s->n_head * roles;
     const int chunk = s->dtype_bf16 ? lin::TC : lin::FC, chunks = ceil_div(s->seg_len, chunk);
     // fp32: an SM takes three CTAs of head size 64 and one of 128
     const int most = std::max(s->d_key, s->d_value), want = s->dtype_bf16 ? SMS : SMS * (most <= 64 ? 3 : 1);
-    const int n = (int)std::min<long long>(std::max<long long>(want / ctas, 1), std::max(chunks / 4, 1));
-    const int each = ceil_div(chunks, n);
+    const int n = (int)std::min<long long>(std::max<long long>(want / ctas, 1), std::max(std::min(chunks, 16), chunks / 2));
+    int each = ceil_div(chunks, n);
+    // a chunk of the first pass takes 0.6 of one of the second, both passes together a chunk more (two chunks of 64 tokens, 8
+    // pairs of 64: 6.4 us in one part, 7.2 in two; three 8.6 and 7.5)
+    if (8ll * each + 5 > 5ll * chunks)
+        each = chunks;
     *seg = each * chunk;
     *n_seg = ceil_div(chunks, each);
 }
