@@ -595,10 +595,12 @@ template <bool STATES> __global__ void __launch_bounds__(256) quad_kernel(const 
 //
 // A CTA of 4 CG warps goes through one part of one (stream, head) in chunks of 64 tokens.  Warp (r, cg) takes rows
 // 16 r .. 16 r + 15 of a chunk and 32 columns of c, the cg-th; of the state it owns the same columns of rows 16 r ..
-// (and 16 (r + 4) .. of 128) in fp32 accumulators.  The results need all of the state: it goes through shared memory in
-// bf16, one rounding, as the pair weights P have one; products of a decayed b with c, which the state adds up, are kept to
-// 24 bits by three bf16 terms of the decayed value, so that the state is an fp32 sum of fp32 products.  Pair weights and
-// terms are the same for the CG warps of the same rows: each computes every CG-th and they meet at a barrier of their own.
+// (and 16 (r + 4) .. of 128) in fp32 accumulators.  The results need all of the state: it goes through shared memory as two
+// bf16 terms, and so do the pair weights P.  What 16 bits leave out, 2^-16 of each, is far below a result's own rounding;
+// with one term each the errors against 64 bits were 2.35e-3 of the results instead of the 1.66e-3 of that rounding
+// (128 pairs of 2048 tokens of 64, forward: 62.7 us, now 76.6).  Products of a decayed b with c, which the state adds up, are
+// kept to 24 bits by three bf16 terms of the decayed value, so that the state is an fp32 sum of fp32 products.  Pair weights
+// and terms are the same for the CG warps of the same rows: each computes every CG-th and they meet at a barrier of their own.
 //
 // Tiles come by TMA, 64 tokens x 64 (32) values of a head a copy, from a map of (value, head, stream, token): what lies beyond
 // a head's values or the sequence arrives as zeros.  One thread asks for the next chunk's under the present chunk; one
@@ -606,9 +608,9 @@ template <bool STATES> __global__ void __launch_bounds__(256) quad_kernel(const 
 //
 // Bound by the chain of a chunk's phases (weights, what the state gives, products with c, the state to the next chunk) in
 // too few warps to hide it: the tensor pipe is active 40 to 52 % of the time, shared memory 44 to 66, an instruction
-// issues in 35 to 45.  8 x 16 pairs of 2048 tokens of 64, forward and backward: 190 us, 36 GFLOP of the chunk form's
-// products, the state's in two or three terms, 192 TFLOP/s of the 550 that this instruction reaches; the bytes alone 41.5 us.
-// 2 x 8 pairs of 4096 tokens of 128, forward, in eight parts: 69 us (both passes), bytes 10.5.
+// issues in 35 to 45.  8 x 16 pairs of 2048 tokens of 64, forward and backward: 231 us, 50 GFLOP of the chunk form's
+// products, in two or three terms but for the pair weights, 218 TFLOP/s of the 550 that this instruction reaches; the bytes
+// alone 41.5 us.  2 x 8 pairs of 4096 tokens of 128, forward, in eight parts: 77 us (both passes), bytes 10.5.
 
 constexpr int TC = 64; // tokens in a chunk
 
@@ -620,10 +622,11 @@ struct __align__(64) MmaArgs {
 template <int DA, int DC, bool TWO> struct MmaSmem {
     static constexpr int TA = TC * DA * 2, TB = TC * DC * 2, LC = DC + 8; // tiles; pitch of the state, rows four banks on
     static constexpr int MT = DA > 64 ? DA / 64 : 1;
-    static constexpr int XP = 10 * 512, XS = 4 * 4 * MT * 3 * 512; // what warps of the same rows hand one another
-    static constexpr int A = 0, B = A + 2 * TA, C = B + 2 * TA, A2 = C + 2 * TB, S = A2 + (TWO ? 2 * TB : 0), P = S + (TWO ? 1 : 2) * DA * LC * 2,
-                         P2 = P + XP, SP = P2 + (TWO ? XP : 0), W = SP + XS,
-                         BAR = W + (2 * TC + 8) * 4, BYTES = BAR + 16 + 1024; // the tiles begin at a multiple of 1024
+    static constexpr int SL = DA * LC * 2, XP = 10 * 512; // a term of the state, of the pair weights
+    static constexpr int XS = 4 * 4 * MT * 3 * 512;       // the decayed values' terms
+    static constexpr int A = 0, B = A + 2 * TA, C = B + 2 * TA, A2 = C + 2 * TB, S = A2 + (TWO ? TB : 0), P = S + 2 * SL, SP = P + 2 * XP, W = SP + XS,
+                         BAR = W + (2 * TC + 8) * 4, BYTES = BAR + 32 + 1024; // the tiles begin at a multiple of 1024
+    static_assert(BYTES <= SMEM_MOST && (DA > 64 || DC > 64 || 2 * (BYTES + 1024) <= SMEM_MOST + 1024), "");
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int h, int b, int t)
@@ -682,12 +685,19 @@ __device__ __forceinline__ void split3(uint32_t v, float w0, float w1, uint32_t 
     lo = fa::pack2(x - __uint_as_float(mid << 16), y - __uint_as_float(mid & 0xffff0000u));
 }
 
+// a pair of values as two bf16 terms each: 16 bits of them
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo)
+{
+    hi = fa::pack2(x, y);
+    lo = fa::pack2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+}
+
 // TMA: tiles come by tensor maps; otherwise (streams of one chunk, where there is nothing to fetch ahead and twelve maps
 // for a step cost the host 6 us) all threads copy 16 bytes at a time.
 // TWO: roles with a2 have a second result,
 //   o2_i = s_state l^(i+e1) a2_i S^T + s_pair sum_{j<=i} l^(i-j) (a2_i . c_j) b_j,
-// from the same tiles of b and c and the same state: dk beside dv.  One copy of the state's bf16 instead of two, so that two
-// such CTAs share an SM.
+// from the same tiles of b and c and the same state: dk beside dv.  It is computed behind the first one, in the same room for pair
+// weights, and a2 has one place, filled again while the next chunk computes its first result: so two such CTAs share an SM.
 template <int DA, int DC, bool STATES, bool TMA, bool TWO>
 __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kernel(const __grid_constant__ MmaArgs args)
 {
@@ -714,6 +724,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             abort_s = 0;
             tc::mbar_init(bar, 1);
             tc::mbar_init(bar + 8, 1);
+            tc::mbar_init(bar + 16, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncthreads();
@@ -733,11 +744,11 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             tile_copy<DA, THR>(base + SM::B + buf * SM::TA, reinterpret_cast<const bf16 *>(q.b) + b * q.ldb + h * q.da, p.B * q.ldb, q.da, t0, rows.n);
             tile_copy<DC, THR>(base + SM::C + buf * SM::TB, reinterpret_cast<const bf16 *>(q.c) + b * q.ldc + h * q.dc, p.B * q.ldc, q.dc, t0, rows.n);
             if (two)
-                tile_copy<DC, THR>(base + SM::A2 + buf * SM::TB, reinterpret_cast<const bf16 *>(q.a2) + b * q.lda2 + h * q.dc, p.B * q.lda2, q.dc, t0, rows.n);
+                tile_copy<DC, THR>(base + SM::A2, reinterpret_cast<const bf16 *>(q.a2) + b * q.lda2 + h * q.dc, p.B * q.lda2, q.dc, t0, rows.n);
             fa::cp_commit();
         } else if (tid == 0 && ok) {
             const uint32_t full = bar + 8 * buf;
-            tc::mbar_expect_tx(full, (STATES ? 1 : 2) * SM::TA + SM::TB + (two ? SM::TB : 0));
+            tc::mbar_expect_tx(full, (STATES ? 1 : 2) * SM::TA + SM::TB);
 #pragma unroll
             for (int x = 0; x < DA; x += 64) {
                 if (!STATES)
@@ -745,15 +756,23 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                 tma_load_4d(base + SM::B + buf * SM::TA + x * TC * 2, &maps[1], full, x, h, b, t0);
             }
 #pragma unroll
-            for (int x = 0; x < DC; x += 64) {
+            for (int x = 0; x < DC; x += 64)
                 tma_load_4d(base + SM::C + buf * SM::TB + x * TC * 2, &maps[2], full, x, h, b, t0);
-                if (two)
-                    tma_load_4d(base + SM::A2 + buf * SM::TB + x * TC * 2, &maps[3], full, x, h, b, t0);
-            }
         }
     };
-    if (chunks)
+    auto fetch2 = [&](int k) { // a2, when the chunk before has read its place
+        if (TMA && two && tid == 0 && ok) {
+            const int u0 = begin + k * TC, t0 = q.reverse ? rows.n - TC - u0 : u0;
+            tc::mbar_expect_tx(bar + 16, SM::TB);
+#pragma unroll
+            for (int x = 0; x < DC; x += 64)
+                tma_load_4d(base + SM::A2 + x * TC * 2, &maps[3], bar + 16, x, h, b, t0);
+        }
+    };
+    if (chunks) {
         fetch(0);
+        fetch2(0);
+    }
 
     // the state: element c of s[m][n] is row 16 (r + 4 m) + gq + 8 (c >> 1), column 32 cg + 8 n + 2 t + (c & 1); in
     // parts it lies as the threads hold it
@@ -820,7 +839,6 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     const uint32_t c_at = base + SM::C + tile_at<DC>(row_of(l15), 4 * cg + lhi);           // transposed: rows 0 .. 15 of c
     const uint32_t s_at = base + SM::S + (l15 * LC + 32 * cg + lhi * 8) * 2;
     uint4 *pairs = reinterpret_cast<uint4 *>(sm + SM::P) + r * (r + 1) / 2 * 32 + lane;        // fragments of this warp's rows, keys not behind them
-    uint4 *pairs2 = reinterpret_cast<uint4 *>(sm + SM::P2) + r * (r + 1) / 2 * 32 + lane;
     uint4 *terms = reinterpret_cast<uint4 *>(sm + SM::SP) + r * 4 * MT * 3 * 32 + lane;
     if (p.n_seg > 1) {
         if (STATES) {
@@ -876,18 +894,22 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             }
         state_out(x);
     }
-    auto publish = [&](int buf) {
+    auto publish = [&]() {
         if (!STATES && has_state)
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    bf16 *to = Ss + (TWO ? 0 : buf) * DA * LC + (16 * (r + 4 * m) + gq) * LC + 32 * cg + 8 * n + 2 * t;
-                    *reinterpret_cast<uint32_t *>(to) = fa::pack2(s[m][n][0], s[m][n][1]);
-                    *reinterpret_cast<uint32_t *>(to + 8 * LC) = fa::pack2(s[m][n][2], s[m][n][3]);
-                }
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int c = 0; c < 4; c += 2) {
+                        bf16 *to = Ss + (16 * (r + 4 * m) + gq + 4 * c) * LC + 32 * cg + 8 * n + 2 * t;
+                        uint32_t hi, lo;
+                        split2(s[m][n][c], s[m][n][c + 1], hi, lo);
+                        *reinterpret_cast<uint32_t *>(to) = hi;
+                        *reinterpret_cast<uint32_t *>(to + DA * LC) = lo;
+                    }
     };
-    publish(0);
+    publish();
     if (!STATES)
         zero_behind<bf16>(p, q.o, q.ldo, q.dc, rows, b, h, g, warp, THR / 32, lane);
     if (two)
@@ -909,13 +931,18 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
         __syncthreads(); // this chunk's tiles and state stand; the other buffers are free
         if (!last)
             fetch(k + 1);
-        const uint32_t At = a_at + buf * SM::TA, Bt = b_at + buf * SM::TA, Tt = bt_at + buf * SM::TA, Ct = c_at + buf * SM::TB,
-                       St = s_at + (TWO ? 0 : buf) * DA * LC * 2;
+        const uint32_t At = a_at + buf * SM::TA, Bt = b_at + buf * SM::TA, Tt = bt_at + buf * SM::TA, Ct = c_at + buf * SM::TB;
         const bool carries = has_state && (follows || !last); // the state behind the chunk is of use
         const float *wt = wts + (last ? TC : 0);
-        float o[NT][4], o2[TWO ? NT : 1][4];
+        float o[NT][4];
+        auto row_barrier = [&]() { // the warps of these rows
+            if constexpr (CG > 1)
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + r), "n"(32 * CG) : "memory");
+            else
+                __syncwarp();
+        };
         // pair weights of every CG-th sixteen keys, for all warps of these rows: rows `u` against the tile's rows at v
-        auto weights = [&](const uint32_t (&u)[KS][4], uint32_t v, int step, uint4 *to) {
+        auto weights = [&](const uint32_t (&u)[KS][4], uint32_t v, int step) {
 #pragma unroll
             for (int i = 0; i < 4 / CG; i++) {
                 const int pc = cg + i * CG;
@@ -943,8 +970,45 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                         for (int c = 0; c < 4; c++)
                             w[x][c] *= f * apart[(c >> 1) - x + 1][c & 1];
                 }
-                to[pc * 32] = make_uint4(fa::pack2(w[0][0], w[0][1]), fa::pack2(w[0][2], w[0][3]), fa::pack2(w[1][0], w[1][1]),
-                                         fa::pack2(w[1][2], w[1][3]));
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    split2(w[e >> 1][e % 2 * 2], w[e >> 1][e % 2 * 2 + 1], hi[e], lo[e]);
+                pairs[pc * 32] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                pairs[pc * 32 + SM::XP / 16] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+        };
+        // what the pair weights of keys 16 ks .. give, f: the products' right factors
+        auto paired = [&](float (&x)[NT][4], int ks, const uint32_t (&f)[NT / 2][4]) {
+#pragma unroll
+            for (int term = 0; term < 2; term++) {
+                const uint4 u = pairs[ks * 32 + term * (SM::XP / 16)];
+                const uint32_t pf[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+                    fa::mma(x[i], pf, f[i / 2][i % 2 * 2], f[i / 2][i % 2 * 2 + 1]);
+            }
+        };
+        auto decayed = [&](float (&x)[NT][4]) {
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                x[i][0] *= f_a; x[i][1] *= f_a;
+                x[i][2] *= f_b; x[i][3] *= f_b;
+            }
+        };
+        // rows out: a quad's 32 columns in four pieces of 16 bytes
+        auto rows_out = [&](const float (&x)[NT][4], void *out, long long ldo, int d) {
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+                const int i = 16 * r + gq + 4 * c;
+                bf16 *to = reinterpret_cast<bf16 *>(out) + (i < n ? rows.row(u0 + i) * ldo : 0) + (size_t)h * d + 32 * cg;
+                uint32_t v[4];
+#pragma unroll
+                for (int k = 0; k < NT; k++)
+                    v[k] = ok ? fa::pack2(x[k][c], x[k][c + 1]) : 0x7fff7fffu; // NaN behind a wait that ran out
+                fa::quad_transpose(v, t);
+                if (i < n && 32 * cg + 8 * t < d)
+                    *reinterpret_cast<uint4 *>(to + 8 * t) = make_uint4(v[0], v[1], v[2], v[3]);
             }
         };
         if (!STATES) {
@@ -952,7 +1016,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
                 ldsm4_at(aq[ks], (At ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128));
-            weights(aq, Bt, step_a, pairs);
+            weights(aq, Bt, step_a);
             // what the state gives
 #pragma unroll
             for (int x = 0; x < NT; x++)
@@ -960,44 +1024,15 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int x = 0; x < NT; x += 2) {
-                    uint32_t f[4];
-                    ldsm4t_at(f, St + (ks * 16 * LC + x * 8) * 2);
-                    fa::mma(o[x], aq[ks], f[0], f[1]);
-                    fa::mma(o[x + 1], aq[ks], f[2], f[3]);
-                }
+                for (int x = 0; x < NT; x += 2)
 #pragma unroll
-            for (int x = 0; x < NT; x++) {
-                o[x][0] *= f_a; o[x][1] *= f_a;
-                o[x][2] *= f_b; o[x][3] *= f_b;
-            }
-            if constexpr (TWO) {
-                static_assert(DA == DC, "");
-                if (two) {
-                    const uint32_t A2t = a_at - SM::A + SM::A2 + buf * SM::TB, C2t = b_at - SM::B + SM::C + buf * SM::TB;
-#pragma unroll
-                    for (int ks = 0; ks < KS; ks++)
-                        ldsm4_at(aq[ks], (A2t ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128));
-                    weights(aq, C2t, step_c, pairs2);
-#pragma unroll
-                    for (int x = 0; x < NT; x++)
-                        o2[x][0] = o2[x][1] = o2[x][2] = o2[x][3] = 0.0f;
-#pragma unroll
-                    for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                        for (int x = 0; x < NT; x += 2) { // the state's rows are columns here
-                            uint32_t f[4];
-                            ldsm4_at(f, base + SM::S + ((32 * cg + 8 * x + lrow) * LC + ks * 16 + lmid * 8) * 2);
-                            fa::mma(o2[x], aq[ks], f[0], f[1]);
-                            fa::mma(o2[x + 1], aq[ks], f[2], f[3]);
-                        }
-#pragma unroll
-                    for (int x = 0; x < NT; x++) {
-                        o2[x][0] *= f_a; o2[x][1] *= f_a;
-                        o2[x][2] *= f_b; o2[x][3] *= f_b;
+                    for (int term = 0; term < 2; term++) {
+                        uint32_t f[4];
+                        ldsm4t_at(f, s_at + term * SM::SL + (ks * 16 * LC + x * 8) * 2);
+                        fa::mma(o[x], aq[ks], f[0], f[1]);
+                        fa::mma(o[x + 1], aq[ks], f[2], f[3]);
                     }
-                }
-            }
+            decayed(o);
         }
         // decayed values of every CG-th sixteen tokens, in three terms
         if (carries) {
@@ -1019,10 +1054,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                 }
             }
         }
-        if constexpr (CG > 1)
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + r), "n"(32 * CG) : "memory"); // the warps of these rows
-        else
-            __syncwarp();
+        row_barrier();
         // the third term where a state is a result; 17 bits are more than the roundings behind them keep
         const bool third = follows && q.s_end;
         // what the chunk adds has sums of its own: products cut the sum they are added to, the state is rounded
@@ -1038,25 +1070,8 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
             for (int x = 0; x < NT; x += 2)
                 ldsm4t_at(f[x / 2], (Ct ^ (x << 4)) + ks * step_c);
-            if constexpr (TWO)
-                if (two && ks <= r) {
-                    const uint4 u = pairs2[ks * 32];
-                    const uint32_t pf[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                    for (int x = 0; x < NT; x += 2) {
-                        uint32_t v[4];
-                        ldsm4t_at(v, ((c_at - SM::C + SM::B + buf * SM::TA) ^ (x << 4)) + ks * step_a);
-                        fa::mma(o2[x], pf, v[0], v[1]);
-                        fa::mma(o2[x + 1], pf, v[2], v[3]);
-                    }
-                }
-            if (!STATES && ks <= r) {
-                const uint4 u = pairs[ks * 32];
-                const uint32_t pf[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int x = 0; x < NT; x++)
-                    fa::mma(o[x], pf, f[x / 2][x % 2 * 2], f[x / 2][x % 2 * 2 + 1]);
-            }
+            if (!STATES && ks <= r)
+                paired(o, ks, f);
             if (carries) {
 #pragma unroll
                 for (int m = 0; m < MT; m++)
@@ -1080,30 +1095,53 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
                     for (int c = 0; c < 4; c++)
                         s[m][x][c] = fmaf(l_n, s[m][x][c], add[m][x][c]);
-        // rows out: a quad's 32 columns in four pieces of 16 bytes
-        auto rows_out = [&](const float (&x)[NT][4], void *out, long long ldo, int d) {
-#pragma unroll
-            for (int c = 0; c < 4; c += 2) {
-                const int i = 16 * r + gq + 4 * c;
-                bf16 *to = reinterpret_cast<bf16 *>(out) + (i < n ? rows.row(u0 + i) * ldo : 0) + (size_t)h * d + 32 * cg;
-                uint32_t v[4];
-#pragma unroll
-                for (int k = 0; k < NT; k++)
-                    v[k] = ok ? fa::pack2(x[k][c], x[k][c + 1]) : 0x7fff7fffu; // NaN behind a wait that ran out
-                fa::quad_transpose(v, t);
-                if (i < n && 32 * cg + 8 * t < d)
-                    *reinterpret_cast<uint4 *>(to + 8 * t) = make_uint4(v[0], v[1], v[2], v[3]);
-            }
-        };
         if (!STATES)
             rows_out(o, q.o, q.ldo, q.dc);
-        if constexpr (TWO)
-            if (two)
-                rows_out(o2, q.o2, q.ldo2, q.da);
-        if (TWO && !STATES && !last)
-            __syncthreads(); // the state of this chunk has been read: its one place is free
-        if (!last)
-            publish(buf ^ 1);
+        if constexpr (TWO && !STATES) {
+            static_assert(DA == DC, "");
+            if (two) {
+                if constexpr (TMA)
+                    ok = ok && tc::mbar_wait(bar + 16, k & 1, &abort_s, &flag, 83);
+                row_barrier(); // the first result's pair weights have been read
+                uint32_t aq[KS][4];
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
+                    ldsm4_at(aq[ks], ((a_at - SM::A + SM::A2) ^ ((ks & 3) << 5)) + (ks >> 2) * (TC * 128));
+                weights(aq, b_at - SM::B + SM::C + buf * SM::TB, step_c);
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+                    o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                    for (int x = 0; x < NT; x += 2)
+#pragma unroll
+                        for (int term = 0; term < 2; term++) { // the state's rows are columns here
+                            uint32_t f[4];
+                            ldsm4_at(f, base + SM::S + term * SM::SL + ((32 * cg + 8 * x + lrow) * LC + ks * 16 + lmid * 8) * 2);
+                            fa::mma(o[x], aq[ks], f[0], f[1]);
+                            fa::mma(o[x + 1], aq[ks], f[2], f[3]);
+                        }
+                decayed(o);
+                row_barrier();
+#pragma unroll
+                for (int ks = 0; ks < TC / 16; ks++)
+                    if (ks <= r) {
+                        uint32_t f[NT / 2][4];
+#pragma unroll
+                        for (int x = 0; x < NT; x += 2)
+                            ldsm4t_at(f[x / 2], ((c_at - SM::C + SM::B + buf * SM::TA) ^ (x << 4)) + ks * step_a);
+                        paired(o, ks, f);
+                    }
+                rows_out(o, q.o2, q.ldo2, q.da);
+            }
+        }
+        if (!last) {
+            if (!STATES)
+                __syncthreads(); // the state of this chunk has been read: its place is free, and that of a2
+            fetch2(k + 1);
+            publish();
+        }
     }
     if (!ok) {
 #pragma unroll
@@ -1111,7 +1149,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
             for (int x = 0; x < NT; x++)
                 s[m][x][0] = s[m][x][1] = s[m][x][2] = s[m][x][3] = NAN;
-        for (int x = 0; x < 2 && TMA; x++) // copies in flight may land before the CTA leaves
+        for (int x = 0; x < 3 && TMA; x++) // copies in flight may land before the CTA leaves
             tc::mbar_wait(bar + 8 * x, 0, &abort_s, &flag, 81, tc::DRAIN_TRIES);
     }
     if (STATES) {
