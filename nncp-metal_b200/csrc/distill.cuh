@@ -59,13 +59,28 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
+// the larger, NaN where one of them is: a row of nothing but NaN is no row of nothing but -inf
+__device__ __forceinline__ float most_of(float x, float y)
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+    return m;
+}
+__device__ __forceinline__ float warp_most(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        v = most_of(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
 // block-wide reductions of a few values at once behind one barrier; every thread gets the results
 template <int N_, bool MAX> __device__ __forceinline__ void reduce(float (&v)[N_], float *red)
 {
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < N_; i++)
-        v[i] = MAX ? warp_max(v[i]) : warp_sum(v[i]);
+        v[i] = MAX ? warp_most(v[i]) : warp_sum(v[i]);
     if (lane == 0)
 #pragma unroll
         for (int i = 0; i < N_; i++)
@@ -78,7 +93,7 @@ template <int N_, bool MAX> __device__ __forceinline__ void reduce(float (&v)[N_
 #pragma unroll
         for (int i = 0; i < N_; i++) {
             const float u = __shfl_xor_sync(0xffffffffu, v[i], o);
-            v[i] = MAX ? fmaxf(v[i], u) : v[i] + u;
+            v[i] = MAX ? most_of(v[i], u) : v[i] + u;
         }
 }
 
@@ -281,7 +296,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
             for (int i = tid; i < pieces4; i += thr) {
                 float v[4];
                 load4<TZ>(v, row + 4 * i);
-                most[0] = fmaxf(fmaxf(most[0], fmaxf(v[0], v[1])), fmaxf(v[2], v[3]));
+                most[0] = most_of(most_of(most[0], most_of(v[0], v[1])), most_of(v[2], v[3]));
             }
         }
         reduce<2, true>(most, red[turn]);

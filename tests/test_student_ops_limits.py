@@ -50,3 +50,44 @@ def test_linear_attention_rounds_a_bf16_result_once(pkg, case):
         want = rows(_form(*form)[0])
         size = rows(_form(*(x.abs() if isinstance(x, torch.Tensor) and x.is_floating_point() else x for x in form))[0])
         _near(got[name], want, U[kind] * want.abs() + (2.0 ** -15 + steps * 2.0 ** -23) * size + 1e-30, name)
+
+
+# ---------------------------------------------------------------- the loss against a teacher's top logits
+
+def _distill_all(pkg, z, ids, top, targets, weight, tau, share, grad_kind):
+    """Losses of the fused call and of the forward call, gradients of the fused call and of the pair, whatever they are"""
+    lib = pkg.library()
+    N, V = z.shape
+    shape = pkg.abi.DistillShape(n_rows=N, n_symbols=V, n_top=ids.shape[1], ld_logits=z.stride(0), temperature=tau, teacher_share=share,
+                                 logits_bf16=int(z.dtype == torch.bfloat16), grad_bf16=int(grad_kind == torch.bfloat16))
+    loss, loss2, lse = (torch.full((N * k,), 7.0, device="cuda") for k in (1, 1, 2))
+    dz, dz2 = (torch.full((N, V), 7.0, device="cuda", dtype=grad_kind) for _ in range(2))
+    args = tuple(_ptr(x) for x in (z, ids, top, targets, weight))
+    _ok(pkg, lib.nncu_distill_gradient(C.byref(shape), *args, _ptr(loss), _ptr(dz), _stream()))
+    _ok(pkg, lib.nncu_distill_forward(C.byref(shape), *args, _ptr(loss2), _ptr(lse), _stream()))
+    _ok(pkg, lib.nncu_distill_backward(C.byref(shape), *args, _ptr(lse), _ptr(dz2), _stream()))
+    return (loss, loss2), (dz, dz2)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("N,V,tau,share", [(9, 300, 1.0, 0.5), (9, 300, 2.0, 1.0), (700, 5000, 3.0, 0.5), (9, 60000, 2.0, 0.5), (9, 4, 1.0, 0.0)])
+def test_distillation_of_logits_that_are_not_numbers(pkg, kind, N, V, tau, share):
+    """Rows of nothing but NaN, of NaN and -inf, with one NaN or +inf: NaN, not the zeros of a row without symbols; the rows
+    beside them are what they are alone"""
+    nan = float("nan")
+    z, ids, top, targets, weight = _distill_data(N, V, 3, kind, seed=31)
+    want, grad = _distill_ref(z, ids, top, targets, weight, tau, share)
+    z[1] = nan
+    z[2, ::2], z[2, 1::2] = -math.inf, nan
+    z[3, V - 1] = nan
+    z[4] = -math.inf
+    z[5, V // 2] = math.inf
+    z[6], weight[6] = nan, 0.0
+    bad, good = [1, 2, 3, 5], [r for r in range(N) if r == 0 or r > 6]
+    losses, grads = _distill_all(pkg, z, ids, top, targets, weight, tau, share, kind)
+    for x in (*losses, *grads):
+        assert bool(x[bad].isnan().all()), x[bad]
+        assert bool((x[[4, 6]] == 0).all())
+    for loss in losses:
+        _distill_near(loss[good], [x[good] for x in grads], want[good], grad[good], weight[good], tau, share, kind, V)
