@@ -512,7 +512,8 @@ int nncu_linear_attention_backward(const nncu_linear_attn_shape *s, const void *
  * named by several.  A row without entries has no teacher's term, one whose target is outside the alphabet (or
  * targets NULL) none of its own.  A logit of -inf is a symbol that cannot come.  A row of weight 0, and one
  * whose logits are all -inf, has loss 0 and gradient 0; the former is not looked at.  A NaN or +inf among a row's logits
- * makes its loss and its whole gradient NaN.
+ * makes its loss and its whole gradient NaN, one among the teacher's entries that are there its loss and the gradient of the
+ * symbols that the entries name (but for a teacher_share of 0).
  * n_top up to NNCU_DISTILL_TOP_MAX.  dlogits must not be logits.
  */
 #define NNCU_DISTILL_TOP_MAX 1024

@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
                 last[(unsigned)id % PLACES] = (uint16_t)k;
             en.e[k] = top;
             en.z[k] = !there ? 0.0f : to_f(RING && id >= lo && id < hi ? row[id - lo] : z[id]);
-            most[1] = fmaxf(most[1], top);
+            most[1] = most_of(most[1], top);
         }
         if constexpr (WHAT & LOSS) {
 #pragma unroll 4
@@ -323,6 +323,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
                 for (int i = tid; i < V; i += thr)
                     dz[i] = from_f<TG>(0.0f);
         } else {
+            const bool asked = a.share != 0.0f && mq != -INFINITY; // the teacher, who knows of a symbol
             float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f}; // of what p is over, of e, of e_k, the teacher's
             const float shift = rintf(m * scale), shift1 = rintf(m * LOG2E);
             auto soft = [&](float v) { return soft_at(v, shift); };
@@ -347,13 +348,13 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
             }
 #pragma unroll 1
             for (int k = tid; k < a.K4; k += thr) {
-                const float d = (en.e[k] - mq) * a.inv_tau, e = k < K && en.id[k] >= 0 ? expf(d) : 0.0f;
-                if (e > 0.0f) {
+                const float d = (en.e[k] - mq) * a.inv_tau, e = k < K && en.id[k] >= 0 && asked ? expf(d) : 0.0f;
+                if (e != 0.0f) { // NaN too
                     sums[2] += e;
                     if constexpr (WHAT & LOSS)
                         sums[3] += e * (d - fmaf(en.z[k], scale, -shift) * LN2);
                 }
-                en.e[k] = e > 0.0f ? e : 0.0f;
+                en.e[k] = e;
                 if ((WHAT & GRAD) && en.id[k] >= 0 && last[(unsigned)en.id[k] % PLACES] != k)
                     many[(unsigned)en.id[k] % PLACES] = round;
             }
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
                 float loss = 0.0f;
                 if (known && a.share != 1.0f)
                     loss += (1.0f - a.share) * (logf(sums[0]) - fmaf(en.z[K], HARD == APART ? LOG2E : HARD * scale, -whole) * LN2);
-                if (taught && a.share != 0.0f)
+                if (taught)
                     loss += a.share * a.tau * a.tau * (sums[3] / sums[2] + logf(sums[1] / sums[2]));
                 a.loss[r] = w * loss;
                 if (a.lse) {

@@ -91,3 +91,27 @@ def test_distillation_of_logits_that_are_not_numbers(pkg, kind, N, V, tau, share
         assert bool((x[[4, 6]] == 0).all())
     for loss in losses:
         _distill_near(loss[good], [x[good] for x in grads], want[good], grad[good], weight[good], tau, share, kind, V)
+
+
+@gpu
+@pytest.mark.parametrize("V,K,bad", [(300, 20, float("nan")), (300, 20, math.inf), (9000, 300, float("nan")), (60000, 20, math.inf)])
+def test_distillation_by_a_teacher_that_is_not_a_number(pkg, V, K, bad):
+    """NaN or +inf among a row's entries: NaN in its loss and at the symbols they name, not a row whose teacher is not there; an
+    entry that is not there may hold anything"""
+    z, ids, top, targets, weight = _distill_data(7, V, K, torch.float32, seed=32)
+    ids[4, 1:][ids[4, 1:] == ids[4, 0]] = -1
+    top[1, 3], top[2] = bad, bad
+    ids[3, 0], top[3, 0] = -1, bad
+    top[4, 0] = bad
+    top[5] = -math.inf
+    clean = torch.where((top - top == 0) | (top == -math.inf), top, 0)
+    want, grad = _distill_ref(z, torch.where((top == -math.inf).all(1, keepdim=True), -1, ids), clean, targets, weight, 2.0, 0.5)
+    losses, grads = _distill_all(pkg, z, ids, top, targets, weight, 2.0, 0.5, torch.float32)
+    for r in (1, 2, 4):
+        named = ids[r][ids[r] >= 0].long()
+        assert all(bool(x[r].isnan()) for x in losses) and all(bool(x[r, named].isnan().all()) for x in grads), r
+    for loss in losses:
+        _distill_near(loss[[0, 3, 5, 6]], [x[[0, 3, 5, 6]] for x in grads], want[[0, 3, 5, 6]], grad[[0, 3, 5, 6]], weight[[0, 3, 5, 6]], 2.0, 0.5, torch.float32, V)
+    # of a share of 0 nothing is asked
+    for x in (y for z in _distill_all(pkg, z, ids, top, targets, weight, 2.0, 0.0, torch.float32) for y in z):
+        assert bool(x.isfinite().all())
