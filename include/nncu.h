@@ -199,7 +199,8 @@ int nncu_eval_gradient_update_dev(nncu_model *m, const int32_t *expected_dev);
  * top_ids_host int32 and top_logits_host fp32 [T][B][n_top], with q the softmax of the logits of the entries
  * whose symbol is inside the alphabet:
  *   loss = sum over rows of (1 - teacher_share) ln p[target] + teacher_share sum_k q_k (ln p[id_k] - ln q_k)
- * A row without such an entry learns from its target alone.  Losses of one forward pass may follow one another.  The first
+ * A row without such an entry, or whose entries are all -inf, learns from its target alone; NaN or +inf among them make the loss
+ * NaN.  Losses of one forward pass may follow one another.  The first
  * call, and one with another n_top, allocates room for the entries and waits for the stream; so does every
  * call for its copies.
  */

@@ -986,7 +986,7 @@ loss_top_kernel(const float *__restrict__ probs, const int32_t *__restrict__ tar
 {
     const int r = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     pdl_wait();
-    if (r >= rows)
+    if (r >= rows || share == 0.0f)
         return;
     const float *pr = probs + (size_t)r * V;
     T *d = dz + (size_t)r * V;
@@ -994,13 +994,16 @@ loss_top_kernel(const float *__restrict__ probs, const int32_t *__restrict__ tar
     const float *z = top_logits + (size_t)r * K;
     auto there = [&](int k) { return ids[k] >= 0 && ids[k] < V; };
     float most = -INFINITY;
+    bool any = false; // an entry that is not -inf, NaN among them, which the maximum drops
     for (int k = lane; k < K; k += 32)
-        if (there(k))
+        if (there(k)) {
             most = fmaxf(most, z[k]);
+            any = any || z[k] != -INFINITY;
+        }
     most = warp_max(most);
-    if (most == -INFINITY) // no teacher: the target alone
+    if (!__any_sync(0xffffffffu, any)) // no teacher: the target alone
         return;
-    float sum = 0.0f;
+    float sum = 0.0f; // NaN or +inf among the entries: NaN
     for (int k = lane; k < K; k += 32)
         if (there(k))
             sum += expf(z[k] - most);
@@ -1015,7 +1018,7 @@ loss_top_kernel(const float *__restrict__ probs, const int32_t *__restrict__ tar
             continue;
         const int id = ids[k];
         const float q = expf(z[k] - most) * inv, p = pr[id];
-        if (q > 0.0f)
+        if (q != 0.0f) // NaN too
             gain += q * (logf(p) - (z[k] - most - ln_sum));
         float of_id = 0.0f; // of all entries that name it; the first of them writes
         bool first = true;
@@ -1031,7 +1034,7 @@ loss_top_kernel(const float *__restrict__ probs, const int32_t *__restrict__ tar
     gain = warp_sum(gain);
     named = __any_sync(0xffffffffu, named);
     if (lane == 0) {
-        logp[r] = (share < 1.0f ? (1.0f - share) * logp[r] : 0.0f) + (share > 0.0f ? share * gain : 0.0f);
+        logp[r] = (share < 1.0f ? (1.0f - share) * logp[r] : 0.0f) + share * gain;
         if (!named)
             d[t] = from_f<T>((pr[t] - (1.0f - share)) * scale);
     }

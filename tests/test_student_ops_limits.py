@@ -115,3 +115,46 @@ def test_distillation_by_a_teacher_that_is_not_a_number(pkg, V, K, bad):
     # of a share of 0 nothing is asked
     for x in (y for z in _distill_all(pkg, z, ids, top, targets, weight, 2.0, 0.0, torch.float32) for y in z):
         assert bool(x.isfinite().all())
+
+
+# ---------------------------------------------------------------- the model's own path
+
+def _model(pkg, bf16, V=300):
+    kw = dict(n_layer=2, d_model=64, n_head=2, d_key=32, d_inner=128, d_pos=24, mem_len=16, seg_len=16, n_streams=4, n_symbols=V, use_bf16=bf16, init_range=0.2)
+    m = pkg.TrfModel(pkg.abi.make_params(**kw))
+    m.reset()
+    return m
+
+
+@gpu
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_model_and_a_teacher_that_is_not_a_number(pkg, bf16):
+    """The same of the model's loss; entries of nothing but -inf are no teacher; and the plain loss behind it is what it was"""
+    np = pytest.importorskip("numpy")
+    T, B, K, V = 16, 4, 40, 300
+    rng = np.random.default_rng(7)
+    m = _model(pkg, bf16, V)
+    ids_in, tg = (rng.integers(0, V, (T, B)).astype(np.int32) for _ in range(2))
+    ids = rng.integers(0, V, (T, B, K)).astype(np.int32)
+    top = rng.normal(size=(T, B, K)).astype(np.float32)
+    m.eval(-1, ids_in, read=False)
+    plain = m.eval_gradient(tg)
+    grads = {n: m.get_grad(n) for n in m.info}
+    taught = m.eval_gradient_distill(tg, ids, top, 0.5)
+    assert math.isfinite(taught)
+    for bad in (float("nan"), math.inf):
+        for k in (slice(0, 1), slice(35, 36), slice(0, K)):
+            rows = top.copy()
+            rows[3, 1, k] = bad
+            assert math.isnan(m.eval_gradient_distill(tg, ids, rows, 0.5)), (bad, k)
+            assert m.eval_gradient_distill(tg, ids, rows, 0.0) == plain
+            assert all(np.array_equal(m.get_grad(n), grads[n]) for n in m.info)
+            away = ids.copy()
+            away[3, 1, k] = -1
+            assert math.isfinite(m.eval_gradient_distill(tg, away, rows, 0.5))
+    assert m.eval_gradient_distill(tg, ids, np.full_like(top, -np.inf), 0.5) == plain
+    assert all(np.array_equal(m.get_grad(n), grads[n]) for n in m.info)
+    assert m.eval_gradient_distill(tg, ids, top, 0.5) == taught
+    assert m.eval_gradient(tg) == plain
+    assert all(np.array_equal(m.get_grad(n), grads[n]) for n in m.info)
+    m.close()
