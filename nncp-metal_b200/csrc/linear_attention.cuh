@@ -22,6 +22,7 @@
 #pragma once
 #include <type_traits>
 
+#include "copy_ring.h"
 #include "gemm_tc.cuh"
 #include "warp_mma.cuh"
 
@@ -736,6 +737,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
         return;
     const int begin = g * p.seg, end = min(rows.n, begin + p.seg), total = max(end - begin, 0), chunks = (total + TC - 1) / TC;
     bool ok = true; // this thread's waits; behind one that ran out results are NaN and nothing more is asked for
+    CopyRing chunk_ring(2), a2_ring(1); // thread 0's
     auto fetch = [&](int k) {
         const int u0 = begin + k * TC, buf = k & 1, t0 = q.reverse ? rows.n - TC - u0 : u0;
         if constexpr (!TMA) {
@@ -748,6 +750,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             fa::cp_commit();
         } else if (tid == 0 && ok) {
             const uint32_t full = bar + 8 * buf;
+            chunk_ring.asked++;
             tc::mbar_expect_tx(full, (STATES ? 1 : 2) * SM::TA + SM::TB);
 #pragma unroll
             for (int x = 0; x < DA; x += 64) {
@@ -763,6 +766,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     auto fetch2 = [&](int k) { // a2, when the chunk before has read its place
         if (TMA && two && tid == 0 && ok) {
             const int u0 = begin + k * TC, t0 = q.reverse ? rows.n - TC - u0 : u0;
+            a2_ring.asked++;
             tc::mbar_expect_tx(bar + 16, SM::TB);
 #pragma unroll
             for (int x = 0; x < DC; x += 64)
@@ -919,7 +923,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
         const int buf = k & 1, u0 = begin + k * TC, n = min(TC, end - u0);
         const bool last = k == chunks - 1;
         if constexpr (TMA)
-            ok = ok && tc::mbar_wait(bar + 8 * buf, (k >> 1) & 1, &abort_s, &flag, 81);
+            ok = ok && tc::mbar_wait(bar + 8 * buf, chunk_ring.parity(k), &abort_s, &flag, 81);
         else
             fa::cp_wait<0>();
         if (TMA && n < TC && p.len && !q.reverse) // rows behind the stream's end hold anything: the tile's are zeros
@@ -1101,7 +1105,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             static_assert(DA == DC, "");
             if (two) {
                 if constexpr (TMA)
-                    ok = ok && tc::mbar_wait(bar + 16, k & 1, &abort_s, &flag, 83);
+                    ok = ok && tc::mbar_wait(bar + 16, a2_ring.parity(k), &abort_s, &flag, 83);
                 row_barrier(); // the first result's pair weights have been read
                 uint32_t aq[KS][4];
 #pragma unroll
@@ -1149,8 +1153,9 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
 #pragma unroll
             for (int x = 0; x < NT; x++)
                 s[m][x][0] = s[m][x][1] = s[m][x][2] = s[m][x][3] = NAN;
-        for (int x = 0; x < 3 && TMA; x++) // copies in flight may land before the CTA leaves
-            tc::mbar_wait(bar + 8 * x, 0, &abort_s, &flag, 81, tc::DRAIN_TRIES);
+        // copies in flight land before the CTA leaves
+        chunk_ring.each_open([&](int place, int parity) { tc::mbar_wait(bar + 8 * place, parity, &abort_s, &flag, 81, tc::DRAIN_TRIES); });
+        a2_ring.each_open([&](int, int parity) { tc::mbar_wait(bar + 16, parity, &abort_s, &flag, 83, tc::DRAIN_TRIES); });
     }
     if (STATES) {
         part += (size_t)(g + 1) * (p.slot / 4);
