@@ -23,6 +23,7 @@
 // The gradient is written dense first; the few entries that the target and the teacher name are computed again whole and
 // written over it, so that each value is rounded once.
 #pragma once
+#include "copy_ring.h"
 #include "gemm_tc.cuh"
 #include "warp_mma.cuh"
 
@@ -166,12 +167,14 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         lo = min(V, (int)(-at & 15) / (int)sizeof(TZ));
         hi = max(lo, V - (int)((at + (size_t)V * sizeof(TZ)) & 15) / (int)sizeof(TZ));
     };
+    CopyRing ring_of(max(a.slots, 1)); // thread 0's: places are filled in turn
     auto fetch = [&](int slot, long long r) {
         if (RING && tid == 0 && ok && r < a.N) {
             const TZ *z = reinterpret_cast<const TZ *>(a.z) + r * a.ldz;
             int lo, hi;
             pieces(z, lo, hi);
             const uint32_t bytes = (uint32_t)(hi - lo) * sizeof(TZ), bar = bar0 + 8 * slot;
+            ring_of.asked++;
             tc::mbar_expect_tx(bar, bytes);
             if (bytes)
                 asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring0 + slot * a.slot_bytes),
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
     for (int i = 0; i < a.slots; i++)
         fetch(i, r + (long long)i * gridDim.x);
     Side next = side(r);
-    int slot = 0, phase = 0, turn = 0;
+    int slot = 0, parity = 0, turn = 0; // slot, parity: those of row after row in ring_of's order
     TG *late[2] = {nullptr, nullptr}; // entries of the row before, to be written behind a barrier
     float late_value[2];
     uint16_t round = 0;
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         const float z_edge = edge >= 0 ? to_f(z[edge]) : -INFINITY;
         named_before(); // while this row is on its way
         if (RING)
-            ok = ok && tc::mbar_wait(bar0 + 8 * slot, phase, &abort_s, &flag, 82);
+            ok = ok && tc::mbar_wait(bar0 + 8 * slot, parity, &abort_s, &flag, 82);
         const float w = now.w;
         const bool known = now.target >= 0 && now.target < V;
         const Entries en = entries(turn);
@@ -436,7 +439,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         }
         if (++slot >= a.slots) {
             slot = 0;
-            phase ^= 1;
+            parity ^= 1;
         }
     }
     if constexpr (WHAT & GRAD) {
@@ -447,9 +450,8 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
             if (late[i])
                 *late[i] = from_f<TG>(late_value[i]);
     }
-    if (!ok) // copies in flight may land before the CTA leaves
-        for (int i = 0; i < a.slots; i++)
-            tc::mbar_wait(bar0 + 8 * i, phase, &abort_s, &flag, 82, tc::DRAIN_TRIES);
+    if (RING && !ok) // copies in flight land before the CTA leaves
+        ring_of.each_open([&](int place, int parity) { tc::mbar_wait(bar0 + 8 * place, parity, &abort_s, &flag, 82, tc::DRAIN_TRIES); });
 }
 
 } // namespace distill

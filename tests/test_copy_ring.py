@@ -50,7 +50,7 @@ def test_every_copy_in_flight_is_waited_for(ring, places, asked):
 
 def test_kernels_take_their_parities_from_the_ring():
     """No wait of a kernel with such a ring counts phases of its own"""
-    for name in ("linear_attention.cuh",):
+    for name in ("linear_attention.cuh", "distill.cuh"):
         text = open(os.path.join(CSRC, name)).read()
         waits = re.findall(r"mbar_wait\(([^;]*)\);", text)
         assert waits and all("parity" in w for w in waits), (name, waits)
