@@ -75,8 +75,8 @@ __device__ __forceinline__ float warp_most(float v)
     return v;
 }
 
-// block-wide reductions of a few values at once behind one barrier; every thread gets the results
-template <int N_, bool MAX> __device__ __forceinline__ void reduce(float (&v)[N_], float *red)
+// block-wide reductions of a few values at once behind one barrier; every thread gets the results, and whether all are ok
+template <int N_, bool MAX> __device__ __forceinline__ bool reduce(float (&v)[N_], float *red, bool ok = true)
 {
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
@@ -86,7 +86,10 @@ template <int N_, bool MAX> __device__ __forceinline__ void reduce(float (&v)[N_
 #pragma unroll
         for (int i = 0; i < N_; i++)
             red[i * 16 + warp] = v[i];
-    __syncthreads();
+    if (MAX)
+        ok = __syncthreads_and(ok);
+    else
+        __syncthreads();
 #pragma unroll
     for (int i = 0; i < N_; i++)
         v[i] = red[i * 16 + (lane & (warps - 1))]; // warps: a power of two, 16 at most
@@ -96,6 +99,7 @@ template <int N_, bool MAX> __device__ __forceinline__ void reduce(float (&v)[N_
             const float u = __shfl_xor_sync(0xffffffffu, v[i], o);
             v[i] = MAX ? most_of(v[i], u) : v[i] + u;
         }
+    return ok;
 }
 
 template <typename T> __device__ __forceinline__ void load4(float (&v)[4], const T *p)
@@ -160,7 +164,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         reinterpret_cast<uint32_t *>(many)[i] = 0xffffffffu;
     __syncthreads();
     pdl_wait();
-    bool ok = true; // this thread's waits; behind one that ran out results are NaN and nothing more is asked for
+    bool ok = true; // the CTA's waits; behind one that ran out results are NaN and nothing more is asked for
     // the whole pieces of row r: logits [lo, hi)
     auto pieces = [&](const TZ *z, int &lo, int &hi) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(z);
@@ -302,7 +306,9 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
                 most[0] = most_of(most_of(most[0], most_of(v[0], v[1])), most_of(v[2], v[3]));
             }
         }
-        reduce<2, true>(most, red[turn]);
+        ok = reduce<2, true>(most, red[turn], ok);
+        if (!ok) // what lies in the row's place may be another's
+            most[0] = NAN;
         // behind the barrier: what the row before has left
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -364,8 +370,6 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
             reduce<4, false>(sums, red[turn] + 2 * 16); // its barrier also lets the entries be read by all
             if constexpr (HARD == SAME)
                 sums[0] = sums[1];
-            if (!ok)
-                sums[0] = sums[1] = sums[2] = sums[3] = NAN;
             const bool taught = !(sums[2] <= 0.0f);
             if ((WHAT & LOSS) && tid == thr - 1) {
                 // log2 of e's whole part of p, for the target and for the sum
@@ -390,6 +394,8 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
                 } else {
                     g = f * ex2(fmaf(-now.lse, LOG2E, HARD == APART ? shift1 : HARD * shift));
                     g_tau = f_tau * ex2(fmaf(-now.lse_tau, LOG2E, shift));
+                    if (!ok)
+                        g = g_tau = NAN;
                 }
                 const float inv_e = taught ? __fdividef(f_tau, sums[2]) : 0.0f;
                 auto both = [&](float v) {

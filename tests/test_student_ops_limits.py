@@ -3,8 +3,12 @@ they are given: how often a result is rounded, values that are not finite or nea
 data and calls are those of test_student_ops.py; u is half a step of a type, relative (bf16 2^-8, fp32 2^-24)."""
 import ctypes as C
 import math
+import os
+import subprocess
 
 import pytest
+
+from conftest import ROOT
 
 torch = pytest.importorskip("torch")
 
@@ -158,3 +162,56 @@ def test_model_and_a_teacher_that_is_not_a_number(pkg, bf16):
     assert m.eval_gradient(tg) == plain
     assert all(np.array_equal(m.get_grad(n), grads[n]) for n in m.info)
     m.close()
+
+
+# ---------------------------------------------------------------- waits that run out
+
+@pytest.fixture(scope="module")
+def expired(tmp_path_factory, pkg):
+    """The kernels compiled with waits that give up (tests/expired_copies.cu); expire(thread, parity) says which"""
+    nvcc = pkg.loader._nvcc()
+    if nvcc is None:
+        pytest.skip("needs nvcc")
+    out = str(tmp_path_factory.mktemp("expired") / "expired.so")
+    subprocess.run([nvcc] + pkg.loader.NVCC_FLAGS + ["--split-compile=0", "-I", os.path.join(ROOT, "include"), "-I", pkg.loader.CSRC, "-o", out,
+                                                     os.path.join(ROOT, "tests", "expired_copies.cu")], check=True, capture_output=True)
+    lib = C.CDLL(out)
+    lib.nncu_last_error.restype = C.c_char_p
+    yield lib
+    lib.expire(0, 2)
+
+
+@gpu
+@pytest.mark.parametrize("slots,late", [(1, 0), (2, 0), (3, 1), (4, 1)])
+@pytest.mark.parametrize("thread,parity", [(-1, -1), (-1, 1), (0, 1), (70, 0), (127, 1)])
+def test_expired_waits_of_distillation_leave_no_result(pkg, expired, slots, late, thread, parity):
+    """Rows of 3 CTAs, row 3 n + c the n-th of CTA c, whose copy completes a phase of parity n / slots: from the first one that a
+    thread did not see arrive, all that a CTA owes is NaN, those before it are as they are otherwise"""
+    N, V, K, ctas = 40, 1003, 5, 3
+    z, ids, top, targets, _ = _distill_data(N, V, K, torch.float32, seed=41)
+    z[:, V // 2] += 1.0
+
+    def run(what, *results):
+        rc = expired.expired_distill(what, late, ctas, slots, N, V, K, *(C.c_void_p(_ptr(x)) for x in (z, ids, top, targets, *results)))
+        assert rc == 0, expired.nncu_last_error()
+
+    def all_calls(lse=None):
+        loss, loss2, dz, dz2 = (torch.ones(n, device="cuda") for n in (N, N, N * V, N * V))
+        sums = torch.ones(2 * N, device="cuda")
+        run(1, loss, sums, None)
+        run(2, None, sums if lse is None else lse, dz)
+        run(3, loss2, None, dz2)
+        torch.cuda.synchronize()
+        return loss, sums.view(N, 2), dz.view(N, V), loss2, dz2.view(N, V)
+
+    assert expired.expire(0, 2) == 0
+    want = all_calls()
+    assert all(bool(x.isfinite().all()) for x in want)
+    assert expired.expire(thread, parity) == 0
+    got = all_calls(want[1])
+    gone = torch.arange(N, device="cuda") // ctas >= (slots if parity == 1 else 0)
+    assert bool(gone.any())
+    for x, y in zip(got, want):
+        assert bool(x[gone].isnan().all()) and torch.equal(x[~gone], y[~gone])
+    assert expired.expire(0, 2) == 0
+    assert all(torch.equal(x, y) for x, y in zip(all_calls(), want))
