@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
     if (STATES && !q.s_end && g == p.n_seg - 1) // nobody asks for the last part's sum
         return;
     const int begin = g * p.seg, end = min(rows.n, begin + p.seg), total = max(end - begin, 0), chunks = (total + TC - 1) / TC;
-    bool ok = true; // this thread's waits; behind one that ran out results are NaN and nothing more is asked for
+    bool ok = true; // the CTA's waits; behind one that ran out results are NaN and nothing more is asked for
     CopyRing chunk_ring(2), a2_ring(1); // thread 0's
     auto fetch = [&](int k) {
         const int u0 = begin + k * TC, buf = k & 1, t0 = q.reverse ? rows.n - TC - u0 : u0;
@@ -932,7 +932,11 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                 unsigned char *to = sm + (x < DA / 8 ? SM::B + buf * SM::TA + tile_at<DA>(row, x) : SM::C + buf * SM::TB + tile_at<DC>(row, x - DA / 8));
                 *reinterpret_cast<uint4 *>(to) = make_uint4(0u, 0u, 0u, 0u);
             }
-        __syncthreads(); // this chunk's tiles and state stand; the other buffers are free
+        // this chunk's tiles and state stand; the other buffers are free
+        if constexpr (TMA)
+            ok = __syncthreads_and(ok);
+        else
+            __syncthreads();
         if (!last)
             fetch(k + 1);
         const uint32_t At = a_at + buf * SM::TA, Bt = b_at + buf * SM::TA, Tt = bt_at + buf * SM::TA, Ct = c_at + buf * SM::TB;
@@ -944,6 +948,17 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
                 asm volatile("bar.sync %0, %1;" ::"r"(1 + r), "n"(32 * CG) : "memory");
             else
                 __syncwarp();
+        };
+        auto row_agree = [&](bool x) { // the same, and whether x holds in all of them
+            uint32_t all;
+            asm volatile("{\n\t.reg .pred p, q;\n\t"
+                         "setp.ne.u32 p, %1, 0;\n\t"
+                         "bar.red.and.pred q, %2, %3, p;\n\t"
+                         "selp.u32 %0, 1, 0, q;\n\t}"
+                         : "=r"(all)
+                         : "r"((uint32_t)x), "r"(1 + r), "n"(32 * CG)
+                         : "memory");
+            return all != 0;
         };
         // pair weights of every CG-th sixteen keys, for all warps of these rows: rows `u` against the tile's rows at v
         auto weights = [&](const uint32_t (&u)[KS][4], uint32_t v, int step) {
@@ -1106,7 +1121,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             if (two) {
                 if constexpr (TMA)
                     ok = ok && tc::mbar_wait(bar + 16, a2_ring.parity(k), &abort_s, &flag, 83);
-                row_barrier(); // the first result's pair weights have been read
+                ok = row_agree(ok); // and the first result's pair weights have been read
                 uint32_t aq[KS][4];
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++)

@@ -16,6 +16,7 @@ __device__ __forceinline__ bool expired_wait(uint32_t bar, uint32_t parity, vola
 } // namespace tc
 #define mbar_wait expired_wait
 #include "distill.cuh"
+#include "linear_attention.cu"
 
 thread_local char g_nncu_err[512] = "";
 unsigned long long g_nncu_launches = 0;

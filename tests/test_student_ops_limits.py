@@ -215,3 +215,61 @@ def test_expired_waits_of_distillation_leave_no_result(pkg, expired, slots, late
         assert bool(x[gone].isnan().all()) and torch.equal(x[~gone], y[~gone])
     assert expired.expire(0, 2) == 0
     assert all(torch.equal(x, y) for x, y in zip(all_calls(), want))
+
+
+class _Library:
+    """The package with another library for its calls"""
+
+    def __init__(self, pkg, lib):
+        self.abi, self.lib = pkg.abi, lib
+        for name in ("nncu_linear_attention_workspace", "nncu_linear_attention_forward", "nncu_linear_attention_backward"):
+            call = getattr(lib, name)
+            call.restype, call.argtypes = pkg.abi.PROTOTYPES[name]
+
+    def library(self):
+        return self.lib
+
+
+@gpu
+@pytest.mark.parametrize("thread,parity", [(-1, -1), (-1, 0), (-1, 1), (0, 1), (70, 1), (255, 1), (130, 0)])
+def test_expired_waits_of_linear_attention_leave_no_result(pkg, expired, thread, parity):
+    """150 streams of five chunks, k-th from the end for dk and dv: chunk k's copy completes a phase of parity k / 2, the second left
+    factor's (dk) one of parity k.  What a CTA owes is NaN from the first chunk on that a thread did not see arrive, states
+    among it; in a chunk that misses the second left factor alone, the dk of that thread's sixteen rows."""
+    case = (150, 1, 64, 64, 300, None, 1)
+    B, H, d, _, T = case[:5]
+    t, n, behind, decay, s0, ds, length = _linear_data(case, torch.bfloat16, seed=42)
+    op = Linear(_Library(pkg, expired), case, torch.bfloat16, t, decay, s0, ds, length)
+    call = lambda: [x.clone() for x in (*op.forward(), *op.backward())]  # noqa: E731
+    assert expired.expire(0, 2) == 0
+    want = call()
+    assert all(bool(x.isfinite().all()) for x in want)
+    assert expired.expire(thread, parity) == 0
+    got = call()
+    torch.cuda.synchronize()
+    first = 2 if parity == 1 else 0
+    at = torch.arange(T, device="cuda")
+    for name, x, y in zip(("out", "state", "dq", "dk", "dv", "dstate"), got, want):
+        if "state" in name:
+            assert bool(x.isnan().all()), name
+            continue
+        x, y = x.view(T, -1), y.view(T, -1)
+        chunk = (at if name in ("out", "dq") else T - 1 - at) // 64
+        gone, sure = chunk >= first, chunk < first - (name == "dk")
+        assert bool(x[gone].isnan().all()) and torch.equal(x[sure], y[sure]), name
+        part, whole = x[~gone & ~sure].isnan(), (x == y)[~gone & ~sure]
+        assert bool((part | whole).all()) and (first == 0 or name != "dk" or part.sum() == (64 if thread < 0 else 16) * B * d), name
+    assert expired.expire(0, 2) == 0
+    assert all(torch.equal(x, y) for x, y in zip(call(), want))
+
+
+@gpu
+def test_expired_waits_of_linear_attention_in_parts_leave_no_result(pkg, expired):
+    """One long stream in several parts, whose sums a first pass makes"""
+    case = (1, 1, 64, 64, 2560, None, 1)
+    t, n, behind, decay, s0, ds, length = _linear_data(case, torch.bfloat16, seed=43)
+    op = Linear(_Library(pkg, expired), case, torch.bfloat16, t, decay, s0, ds, length)
+    assert op.need > 0 and expired.expire(-1, -1) == 0
+    assert all(bool(x.isnan().all()) for x in (*op.forward(), *op.backward()))
+    assert expired.expire(0, 2) == 0
+    assert all(bool(x.isfinite().all()) for x in (*op.forward(), *op.backward()))
