@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(256, BACK ? 2 : 4) kernel(const __grid_constan
             Item it = next;
             if (i0 + 8 * per_warp < heads)
                 next = fetch(i0 + 8 * per_warp);
-            const bool alive = live[it.r];
+            const bool alive = it.real && live[it.r]; // lanes without a head add nothing to dgain: no root of their zeros is taken
             const bool all_alive = __all_sync(0xffffffffu, alive);
             if (!all_alive && !alive) // padding: zeros, whatever lies there
 #pragma unroll

@@ -13,9 +13,50 @@ from conftest import ROOT
 torch = pytest.importorskip("torch")
 
 from test_student_ops import (KINDS, U, Linear, _distill_calls, _distill_data, _distill_near, _distill_ref, _form, _linear_data, _near,  # noqa: E402,F401
-                              _norm_data, _norm_shape, _ok, _ptr, _stream)
+                              _norm_data, _norm_ref, _norm_shape, _ok, _ptr, _stream)
 
 gpu = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- head norms with rotation
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("case", [(5, 3, 1, 64, 64, 0, 0, 0, 1), (33, 1, 1, 32, 32, 1, 0, 0, 1), (1, 1, 1, 2, 0, 0, 0, 0, 1), (100, 7, 3, 96, 32, 0, 0, 0, 1),
+                                  (3, 2, 0, 128, 64, 0, 0, 0, 1)])
+def test_qk_norm_without_eps(pkg, case, kind):
+    """eps 0 and rows that fill no warp, against 64 bits: nothing of lanes without a head.  Tolerances of the test with eps."""
+    N, H, Hk, d, rot, adj = case[:6]
+    t, gain, _ = _norm_data((min(N, 4), *case[1:]), kind)  # no padding: that takes more than four rows
+    t = {n: x.repeat(N // x.shape[0] + 1, 1)[:N] for n, x in t.items()}
+    assert all(x.is_contiguous() for x in t.values())
+    pos = torch.arange(N, device="cuda").int()
+    shape = _norm_shape(pkg, case, kind)
+    shape.eps = 0.0
+    lib, need = pkg.library(), C.c_size_t()
+    _ok(pkg, lib.nncu_qk_norm_rope_workspace(C.byref(shape), C.byref(need)))
+    room = torch.full((need.value,), 255, dtype=torch.uint8, device="cuda")
+    dgain = {n: torch.full((d,), float("nan"), device="cuda") for n in "qk"}
+    new, back = ({n: torch.full_like(t[n], 7.0) for n in "qk" if n in t} for _ in range(2))
+    _ok(pkg, lib.nncu_qk_norm_rope_forward(C.byref(shape), _ptr(t["q"]), _ptr(t.get("k")), _ptr(gain["q"]), _ptr(gain["k"]), _ptr(pos), _ptr(new["q"]),
+                                           _ptr(new.get("k")), _stream()))
+    _ok(pkg, lib.nncu_qk_norm_rope_backward(C.byref(shape), _ptr(t["q"]), _ptr(t.get("k")), _ptr(gain["q"]), _ptr(gain["k"]), _ptr(pos), _ptr(t["dq_out"]),
+                                            _ptr(t.get("dk_out")), _ptr(back["q"]), _ptr(back.get("k")), _ptr(dgain["q"]), _ptr(dgain["k"]) if Hk else None,
+                                            _ptr(room), need.value, _stream()))
+    f = 2.0 ** -24
+    for n, h in (("q", H), ("k", Hk)):
+        if not h:
+            continue
+        x, gn, dy = t[n].double().requires_grad_(), gain[n].double().requires_grad_(), t["d%s_out" % n].double()
+        want = _norm_ref(x, gn, pos, d, rot, adj, 0.0, 10000.0)
+        dx, dg = torch.autograd.grad(want, (x, gn), dy)
+        spread = lambda y: y.expand(-1, -1, d).reshape(N, -1)  # noqa: E731
+        size = spread(want.detach().view(N, h, d).norm(dim=-1, keepdim=True))
+        _near(new[n], want.detach(), U[kind] * want.detach().abs() + 16 * f * size, n)
+        up = dy.view(N, h, d).norm(dim=-1, keepdim=True)
+        rs = 1 / x.detach().view(N, h, d).square().mean(-1, keepdim=True).sqrt()
+        _near(back[n], dx, U[kind] * dx.abs() + (16 + d) * f * spread(up * rs * gain[n].abs().max().double()), "d" + n)
+        _near(dgain[n], dg, f * (16 + math.sqrt(N * h)) * (up * math.sqrt(d)).sum(), "dgain_" + n)
 
 
 # ---------------------------------------------------------------- attention with a decaying state
