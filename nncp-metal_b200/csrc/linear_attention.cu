@@ -85,8 +85,10 @@ static lin::Args lin_args(const nncu_linear_attn_shape *s, int roles, const floa
     a.slot = lin_slot(s);
     for (int i = 0; i < roles; i++)
         a.role[i].parts = (float *)workspace + (size_t)i * a.B * a.H * (a.n_seg + 1) * a.slot;
-    for (int h = 0; h < s->n_head; h++)
+    for (int h = 0; h < s->n_head; h++) {
         a.rate[h] = (float)log2((double)decay_host[h]);
+        a.decay[h] = decay_host[h];
+    }
     return a;
 }
 

@@ -53,6 +53,7 @@ struct Args {
     int seg;             // tokens in a part
     int slot;            // floats of a state in parts
     float rate[HEADS_MAX]; // log2 of each head's decay
+    float decay[HEADS_MAX];
 };
 
 // l^n; l^0 is 1 whatever l
@@ -1202,7 +1203,7 @@ __global__ void __launch_bounds__(128) step_kernel(const __grid_constant__ Args 
     const int tid = threadIdx.x, cg = tid & 7, rl = tid >> 3;
     const size_t pair = blockIdx.x;
     const int b = (int)(pair / p.H), h = (int)(pair % p.H), c0 = blockIdx.y * COLS;
-    const float l = exp2f(p.rate[h]);
+    const float l = p.decay[h]; // itself: what a power of its logarithm is off by adds up over the calls that carry a state
     pdl_trigger();
     pdl_wait();
     const Rows rows(p, q, b);

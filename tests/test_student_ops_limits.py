@@ -97,6 +97,25 @@ def test_linear_attention_rounds_a_bf16_result_once(pkg, case):
         _near(got[name], want, U[kind] * want.abs() + (2.0 ** -15 + steps * 2.0 ** -23) * size + 1e-30, name)
 
 
+@gpu
+@pytest.mark.parametrize("d", [16, 64, 7])
+def test_linear_attention_decays_a_token_by_the_decay_given(pkg, d):
+    """One token of nothing: the state times the decay, rounded once, forward and back: no bias that calls one after the other
+    would add up.  Half-lives from less than a token to half a million."""
+    H = 64
+    decay = (1 - 2.0 ** -torch.linspace(0.2, 19.5, H, dtype=torch.float64)).float()
+    g = torch.Generator(device="cuda").manual_seed(d)
+    s0, ds = (torch.randn(2, H, d, d, generator=g, device="cuda") for _ in range(2))
+    nothing = torch.zeros(2, H * d, device="cuda")
+    op = Linear(pkg, (2, H, d, d, 1), torch.float32, dict(q=nothing, k=nothing, v=nothing, dout=nothing), decay, s0, ds, None)
+    by = decay.cuda()[None, :, None, None]
+    assert torch.equal(op.forward()[1], s0 * by) and torch.equal(op.backward()[3], ds * by)
+    # five tokens: five times
+    five = nothing.repeat(5, 1)
+    op = Linear(pkg, (2, H, d, d, 5), torch.float32, dict(q=five, k=five, v=five, dout=five), decay, s0, ds, None)
+    assert torch.equal(op.forward()[1], s0 * by * by * by * by * by) and torch.equal(op.backward()[3], ds * by * by * by * by * by)
+
+
 # ---------------------------------------------------------------- the loss against a teacher's top logits
 
 def _distill_all(pkg, z, ids, top, targets, weight, tau, share, grad_kind):
