@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         } else {
             const bool asked = a.share != 0.0f && mq != -INFINITY; // the teacher, who knows of a symbol
             float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f}; // of what p is over, of e, of e_k, the teacher's
-            const float shift = rintf(m * scale), shift1 = rintf(m * LOG2E);
+            // by saved sums, p's exponents count from its own: lse_tau tau is up to tau ln V above it
+            const float shift = rintf(m * scale), shift1 = rintf(((WHAT & LOSS) ? m : now.lse) * LOG2E);
             auto soft = [&](float v) { return soft_at(v, shift); };
             auto hard = [&](float v, float e) { return hard_at(v, e, shift1); };
             if constexpr (WHAT & LOSS) {

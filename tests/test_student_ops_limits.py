@@ -181,6 +181,19 @@ def test_distillation_by_a_teacher_that_is_not_a_number(pkg, V, K, bad):
         assert bool(x.isfinite().all())
 
 
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("V", [300, 16384, 70000])
+@pytest.mark.parametrize("tau", [0.01, 0.25, 8.0, 20.0, 100.0, 1e4])
+def test_distillation_at_temperatures_far_from_one(pkg, kind, V, tau):
+    """The pair of calls as well as the fused one, where p and p_temperature have little in common.  Tolerances of the test at
+    ordinary temperatures."""
+    z, ids, top, targets, weight = _distill_data(8, V, 30, kind, seed=33)
+    got = _distill_calls(pkg, z, ids, top, targets, weight / tau, tau, 0.5, kind)
+    want, grad = _distill_ref(z, ids, top, targets, weight / tau, tau, 0.5)
+    _distill_near(got[0], got[1:], want, grad, weight / tau, tau, 0.5, kind, V)
+
+
 # ---------------------------------------------------------------- the model's own path
 
 def _model(pkg, bf16, V=300):
