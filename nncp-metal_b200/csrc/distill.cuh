@@ -23,6 +23,8 @@
 // The gradient is written dense first; the few entries that the target and the teacher name are computed again whole and
 // written over it, so that each value is rounded once.
 #pragma once
+#include <type_traits>
+
 #include "copy_ring.h"
 #include "gemm_tc.cuh"
 #include "warp_mma.cuh"
@@ -50,6 +52,7 @@ struct Args {
 };
 
 enum { LOSS = 1, GRAD = 2 }; // what a launch gives; GRAD alone takes the sums from lse
+enum { FAR_ROW = 2 };
 // how p follows from e: itself, its square, or an exponential of its own
 enum { SAME = 1, SQUARE = 2, APART = 0 };
 
@@ -129,8 +132,8 @@ struct Entries {
 
 // What the symbols that entries name are computed again from
 struct Kept {
-    float g, g_tau, inv_e, f, shift, shift1; // of what p is over, of e, of e_k; the target's; shifts of e and p
-    int target, any;
+    float g, g_tau, inv_e, f, shift, shift1; // of what p is over, of e, of e_k; the target's; shifts of e and p, or of a row that is far, its base
+    int target, any;                        // any: 0 nothing, 1, or FAR_ROW
     void *dz;
 };
 
@@ -241,9 +244,10 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
             }
         }
         if (first) {
-            const float e = soft_at(en.z[k], of.shift);
+            const bool far = of.any == FAR_ROW;
+            const float z = far ? en.z[k] - of.shift : en.z[k], e = soft_at(z, far ? 0.0f : of.shift);
             to = reinterpret_cast<TG *>(of.dz) + id;
-            value = (HARD == SAME ? (of.g + of.g_tau) * e : fmaf(of.g, hard_at(en.z[k], e, of.shift1), of.g_tau * e)) - (id == of.target ? of.f : 0.0f) -
+            value = (HARD == SAME ? (of.g + of.g_tau) * e : fmaf(of.g, hard_at(z, e, of.shift1), of.g_tau * e)) - (id == of.target ? of.f : 0.0f) -
                     off * of.inv_e;
         }
     };
@@ -283,6 +287,9 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         if (RING)
             ok = ok && tc::mbar_wait(bar0 + 8 * slot, parity, &abort_s, &flag, 82);
         const float w = now.w;
+        // Saved sums are logs of them above zero: of a row far from it they keep too few digits (2^-24 of 64 is what a
+        // probability may be off by), and it is gone through from the beginning
+        const bool whole_way = (WHAT & LOSS) || (w != 0.0f && now.lse != -INFINITY && !(fmaxf(fabsf(now.lse), fabsf(now.lse_tau)) <= 64.0f));
         const bool known = now.target >= 0 && now.target < V;
         const Entries en = entries(turn);
         float most[2] = {z_edge, -INFINITY};
@@ -298,7 +305,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
             en.z[k] = !there ? 0.0f : to_f(RING && id >= lo && id < hi ? row[id - lo] : z[id]);
             most[1] = most_of(most[1], top);
         }
-        if constexpr (WHAT & LOSS) {
+        if (whole_way) {
 #pragma unroll 4
             for (int i = tid; i < pieces4; i += thr) {
                 float v[4];
@@ -318,7 +325,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         }
         if (a.slots > 1 && r != blockIdx.x)
             fetch(slot ? slot - 1 : a.slots - 1, r + (long long)(a.slots - 1) * gridDim.x);
-        const float m = (WHAT & LOSS) ? most[0] : now.lse_tau * a.tau, mq = most[1];
+        const float m = whole_way ? most[0] : now.lse_tau * a.tau, mq = most[1];
         const bool none = w == 0.0f || ((WHAT & LOSS) ? most[0] : now.lse) == -INFINITY; // no weight, or a mask that leaves no symbol
         if (LATE && names && tid == warp_at)
             kept[tid >> 5].any = !none;
@@ -334,35 +341,49 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
         } else {
             const bool asked = a.share != 0.0f && mq != -INFINITY; // the teacher, who knows of a symbol
             float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f}; // of what p is over, of e, of e_k, the teacher's
+            // where the largest logit times the scale has no digits behind the point left (all logits at a type's lowest
+            // value, say), logits are taken from it; elsewhere that subtraction would be an instruction a logit and pass
+            const bool far = whole_way && !(fabsf(m) * fmaxf(scale, LOG2E) < 1048576.0f);
+            const float base = far ? m : 0.0f;
             // by saved sums, p's exponents count from its own: lse_tau tau is up to tau ln V above it
-            const float shift = rintf(m * scale), shift1 = rintf(((WHAT & LOSS) ? m : now.lse) * LOG2E);
+            const float shift = far ? 0.0f : rintf(m * scale), shift1 = far ? 0.0f : rintf((whole_way ? m : now.lse) * LOG2E);
             auto soft = [&](float v) { return soft_at(v, shift); };
             auto hard = [&](float v, float e) { return hard_at(v, e, shift1); };
-            if constexpr (WHAT & LOSS) {
-#pragma unroll 4
+            auto sum_up = [&](auto is_far) {
+                constexpr bool FAR = decltype(is_far)::value;
+                constexpr int AHEAD = FAR ? 1 : 4;
+#pragma unroll AHEAD
                 for (int i = tid; i < pieces4; i += thr) {
                     float v[4];
                     load4<TZ>(v, row + 4 * i);
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
-                        const float e = soft(v[c]);
+                        const float x = FAR ? v[c] - base : v[c], e = soft(x);
                         sums[1] += e;
                         if constexpr (HARD != SAME)
-                            sums[0] += hard(v[c], e);
+                            sums[0] += hard(x, e);
                     }
                 }
-                const float e = soft(z_edge);
+                const float x = z_edge - base, e = soft(x);
                 sums[1] += e;
                 if constexpr (HARD != SAME)
-                    sums[0] += hard(z_edge, e);
+                    sums[0] += hard(x, e);
+            };
+            if (whole_way) {
+                if (far)
+                    sum_up(std::true_type());
+                else
+                    sum_up(std::false_type());
             }
+            // ln 2 u = (z - m) / tau + this
+            const float above = fmaf(m - base, scale, -shift) * LN2;
 #pragma unroll 1
             for (int k = tid; k < a.K4; k += thr) {
                 const float d = (en.e[k] - mq) * a.inv_tau, e = k < K && en.id[k] >= 0 && asked ? expf(d) : 0.0f;
                 if (e != 0.0f) { // NaN too
                     sums[2] += e;
                     if constexpr (WHAT & LOSS)
-                        sums[3] += e * (d - fmaf(en.z[k], scale, -shift) * LN2);
+                        sums[3] += e * (d - fmaf(en.z[k] - m, a.inv_tau, above));
                 }
                 en.e[k] = e;
                 if ((WHAT & GRAD) && en.id[k] >= 0 && last[(unsigned)en.id[k] % PLACES] != k)
@@ -373,23 +394,23 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
                 sums[0] = sums[1];
             const bool taught = !(sums[2] <= 0.0f);
             if ((WHAT & LOSS) && tid == thr - 1) {
-                // log2 of e's whole part of p, for the target and for the sum
-                const float whole = HARD == APART ? shift1 : HARD * shift;
+                // p's shift, and what is above the largest logit's
+                const float whole = HARD == APART ? shift1 : HARD * shift, over = fmaf(m - base, HARD == APART ? LOG2E : HARD * scale, -whole) * LN2;
                 float loss = 0.0f;
                 if (known && a.share != 1.0f)
-                    loss += (1.0f - a.share) * (logf(sums[0]) - fmaf(en.z[K], HARD == APART ? LOG2E : HARD * scale, -whole) * LN2);
+                    loss += (1.0f - a.share) * (logf(sums[0]) - (en.z[K] - m) - over);
                 if (taught)
                     loss += a.share * a.tau * a.tau * (sums[3] / sums[2] + logf(sums[1] / sums[2]));
                 a.loss[r] = w * loss;
                 if (a.lse) {
-                    a.lse[2 * r] = fmaf(whole, LN2, logf(sums[0]));
-                    a.lse[2 * r + 1] = fmaf(shift, LN2, logf(sums[1]));
+                    a.lse[2 * r] = base + fmaf(whole, LN2, logf(sums[0]));
+                    a.lse[2 * r + 1] = base * a.inv_tau + fmaf(shift, LN2, logf(sums[1]));
                 }
             }
             if constexpr (WHAT & GRAD) {
                 const float f = known ? w * (1.0f - a.share) : 0.0f, f_tau = taught ? w * a.share * a.tau : 0.0f;
                 float g, g_tau; // of what p is over, of e
-                if constexpr (WHAT & LOSS) {
+                if (whole_way) {
                     g = __fdividef(f, sums[0]);
                     g_tau = __fdividef(f_tau, sums[1]);
                 } else {
@@ -403,7 +424,7 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
                     const float e = soft(v);
                     return HARD == SAME ? (g + g_tau) * e : HARD == SQUARE ? e * fmaf(g, e, g_tau) : fmaf(g, hard(v, e), g_tau * e);
                 };
-                const Kept of = {g, g_tau, inv_e, f, shift, shift1, now.target, 1, dz};
+                const Kept of = {g, g_tau, inv_e, f, far ? base : shift, shift1, now.target, far ? FAR_ROW : 1, dz};
                 if (names) {
                     if (!LATE)
                         named_two(of, entries(turn), round);
@@ -411,23 +432,31 @@ __global__ void __launch_bounds__(THREADS_MAX, 2) kernel(const __grid_constant__
                         kept[tid >> 5] = of;
                 }
                 TG *to = dz + lo;
-                if (reinterpret_cast<uintptr_t>(to) % (4 * sizeof(TG)) == 0) {
-#pragma unroll 4
-                    for (int i = tid; i < pieces4; i += thr) {
-                        float v[4];
-                        load4<TZ>(v, row + 4 * i);
+                auto dense = [&](auto is_far) {
+                    constexpr bool FAR = decltype(is_far)::value;
+                    constexpr int AHEAD = FAR ? 1 : 4;
+                    if (reinterpret_cast<uintptr_t>(to) % (4 * sizeof(TG)) == 0) {
+#pragma unroll AHEAD
+                        for (int i = tid; i < pieces4; i += thr) {
+                            float v[4];
+                            load4<TZ>(v, row + 4 * i);
 #pragma unroll
-                        for (int c = 0; c < 4; c++)
-                            v[c] = both(v[c]);
-                        store4<TG>(to + 4 * i, v);
+                            for (int c = 0; c < 4; c++)
+                                v[c] = both(FAR ? v[c] - base : v[c]);
+                            store4<TG>(to + 4 * i, v);
+                        }
+                    } else {
+#pragma unroll AHEAD
+                        for (int i = tid; i < hi - lo; i += thr)
+                            to[i] = from_f<TG>(both(to_f(row[i]) - (FAR ? base : 0.0f)));
                     }
-                } else {
-#pragma unroll 4
-                    for (int i = tid; i < hi - lo; i += thr)
-                        to[i] = from_f<TG>(both(to_f(row[i])));
-                }
+                };
+                if (far)
+                    dense(std::true_type());
+                else
+                    dense(std::false_type());
                 if (edge >= 0)
-                    dz[edge] = from_f<TG>(both(z_edge));
+                    dz[edge] = from_f<TG>(both(z_edge - base));
                 if (!defer) {
                     __syncthreads();
                     for (int k = tid; k <= K; k += thr) {

@@ -194,6 +194,41 @@ def test_distillation_at_temperatures_far_from_one(pkg, kind, V, tau):
     _distill_near(got[0], got[1:], want, grad, weight / tau, tau, 0.5, kind, V)
 
 
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("N,V,tau", [(9, 1000, 1.0), (9, 1000, 2.0), (9, 1003, 3.0), (9, 60001, 2.0), (700, 5001, 0.3)])
+def test_distillation_of_logits_far_from_zero(pkg, kind, N, V, tau):
+    """Rows of nothing but a type's lowest or largest value, masks of the lowest, logits about 1e4 and -3e6, in all three calls:
+    a constant on a row's logits changes nothing.  Tolerances of the test at ordinary logits."""
+    z, ids, top, targets, weight = _distill_data(N, V, 30, kind, seed=34)
+    low, high = torch.finfo(kind).min, torch.finfo(kind).max
+    half = V // 2
+    z[1] = low
+    z[2, half:] = low
+    ids[2], targets[2] = ids[2] % half, targets[2] % half
+    z[3] = (z[3].double() + 1e4).to(kind)
+    z[4] = (z[4].double() - 3e6).to(kind)
+    z[5] = high
+    top[6] = torch.finfo(torch.float32).min
+    top[7, ::2] = torch.finfo(torch.float32).min
+    z[8], z[8, 17] = low, 0.5
+    ids[8], targets[8] = 17, 17
+    got = _distill_calls(pkg, z, ids, top, targets, weight, tau, 0.5, kind)
+    want, grad = _distill_ref(z, ids, top, targets, weight, tau, 0.5)
+    _distill_near(got[0], got[1:], want, grad, weight, tau, 0.5, kind, V)
+
+
+@gpu
+def test_distillation_by_a_teacher_who_wants_a_masked_symbol(pkg):
+    """A finite mask's loss is finite: the logits' distance, to fp32's digits of it"""
+    z, ids, top, targets, weight = _distill_data(4, 500, 6, torch.float32, seed=35)
+    ids[1], top[1], ids[1, 0] = -1, 0.0, 7
+    z[1, 7], z[2, 9], targets[2] = -3e38, -3e38, 9
+    got = _distill_calls(pkg, z, ids, top, targets, weight, 1.0, 0.5, torch.float32)
+    want, grad = _distill_ref(z, ids, top, targets, weight, 1.0, 0.5)
+    _distill_near(got[0], got[1:], want, grad, weight, 1.0, 0.5, torch.float32, 500)
+
+
 # ---------------------------------------------------------------- the model's own path
 
 def _model(pkg, bf16, V=300):
