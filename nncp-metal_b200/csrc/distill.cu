@@ -15,6 +15,9 @@ static int distill_check(const nncu_distill_shape *s)
         !(s->teacher_share >= 0.0f && s->teacher_share <= 1.0f) || (s->ld_logits && s->ld_logits < s->n_symbols) ||
         (s->ld_dlogits && s->ld_dlogits < s->n_symbols))
         return nncu_fail(NNCU_ERR_INVALID, "distillation: bad shape");
+    // what the loss and the logits are multiplied by
+    if (s->teacher_share != 0.0f && !(isfinite(s->temperature * s->temperature) && isfinite(2.0f / s->temperature)))
+        return nncu_fail(NNCU_ERR_INVALID, "distillation: the temperature's square or inverse is no fp32 number");
     if (s->n_top > NNCU_DISTILL_TOP_MAX || s->n_symbols > INT_MAX / 2)
         return nncu_fail(NNCU_ERR_RANGE, "distillation: more than %d entries of the teacher, or too many symbols", NNCU_DISTILL_TOP_MAX);
     return NNCU_OK;

@@ -229,6 +229,16 @@ def test_distillation_by_a_teacher_who_wants_a_masked_symbol(pkg):
     _distill_near(got[0], got[1:], want, grad, weight, 1.0, 0.5, torch.float32, 500)
 
 
+def test_distillation_refuses_temperatures_that_overflow(pkg):
+    """tau^2 and 1 / tau are factors of the loss and of the logits"""
+    lib, one = pkg.library(), 4096
+    for tau, share, refused in ((1e20, 0.5, 1), (1e-39, 0.5, 1), (1e20, 0.0, 0), (1e-39, 0.0, 0), (1e19, 0.5, 0), (1e-37, 0.5, 0)):
+        shape = pkg.abi.DistillShape(n_rows=4, n_symbols=100, n_top=5, temperature=tau, teacher_share=share)
+        # an address that is no multiple of four is refused too, behind the shape: nothing is ever launched
+        assert lib.nncu_distill_gradient(C.byref(shape), one + 2, one, one, None, None, one, 2 * one, None) == pkg.abi.ERR_INVALID
+        assert (b"temperature" in lib.nncu_last_error()) == bool(refused), (tau, share)
+
+
 # ---------------------------------------------------------------- the model's own path
 
 def _model(pkg, bf16, V=300):
