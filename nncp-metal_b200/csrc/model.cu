@@ -25,7 +25,6 @@
 #include <string.h>
 
 #include <algorithm>
-#include <functional>
 #include <initializer_list>
 #include <string>
 #include <vector>
@@ -1892,8 +1891,43 @@ static bool sparse_embed_enabled()
     return on != 0;
 }
 
-// top: brings a teacher's entries to the device
-static int gradient_common(nncu_model *m, bool fused = false, const std::function<int(nncu_model *)> &top = nullptr)
+// a teacher's entries in host memory, n a row
+struct TopEntries {
+    const int32_t *ids;
+    const float *logits;
+    int n;
+    float share;
+};
+
+// Brings a teacher's entries to the device
+static int take_top(nncu_model *m, const TopEntries &top)
+{
+    const size_t n = (size_t)m->TB * top.n;
+    if (top.n != m->top_most || top.share != m->top_share) { // what a captured pass holds
+        CUDA_TRY(cudaStreamSynchronize(m->st));               // which nothing runs, and nothing reads the old entries
+        for (auto &g : m->graphs[GRAPH_BWD_TOP]) {
+            if (g.exec)
+                CUDA_TRY(cudaGraphExecDestroy(g.exec));
+            g = nncu_model::StepGraph{nullptr, 0, 0};
+        }
+        if (top.n != m->top_most) {
+            if (m->top_ids)
+                CUDA_TRY(cudaFree(m->top_ids));
+            m->top_ids = nullptr;
+            m->top_most = 0;
+            CUDA_TRY(cudaMalloc(&m->top_ids, n * (sizeof(int32_t) + sizeof(float))));
+        }
+        m->top_most = top.n;
+        m->top_share = top.share;
+    }
+    CUDA_TRY(cudaMemcpyAsync(m->top_ids, top.ids, n * sizeof(int32_t), cudaMemcpyHostToDevice, m->st));
+    CUDA_TRY(cudaMemcpyAsync(m->top_logits(), top.logits, n * sizeof(float), cudaMemcpyHostToDevice, m->st));
+    CUDA_TRY(cudaStreamSynchronize(m->st)); // the arrays are the caller's again
+    m->top_now = top.n;
+    return NNCU_OK;
+}
+
+static int gradient_common(nncu_model *m, bool fused = false, const TopEntries *top = nullptr)
 {
     if (!fused && m->master_stale)
         return nncu_fail(NNCU_ERR_STATE, "the optimizer state is sharded over the ranks: nncu_comm_gather_master first");
@@ -1924,7 +1958,7 @@ static int gradient_common(nncu_model *m, bool fused = false, const std::functio
         m->top_left = 0;
     }
     if (top) { // behind what has read the entries before them
-        NNCU_TRY(top(m));
+        NNCU_TRY(take_top(m, *top));
         m->top_left = m->top_now;
     }
     int rc = run_graphed(m, top ? GRAPH_BWD_TOP : fused ? GRAPH_BWD_UPD : GRAPH_BWD,
@@ -2006,31 +2040,8 @@ int nncu_eval_gradient_distill(nncu_model *m, const int32_t *expected_host, int 
     memcpy(m->tgt_pin, expected_host, sizeof(int32_t) * m->TB);
     CUDA_TRY(cudaMemcpyAsync(m->tgt_dev, m->tgt_pin, sizeof(int32_t) * m->TB, cudaMemcpyHostToDevice, m->st));
     CUDA_TRY(cudaEventRecord(m->ev_tgt, m->st));
-    const size_t n = (size_t)m->TB * n_top;
-    NNCU_TRY(gradient_common(m, false, [&](nncu_model *mm) -> int {
-        if (n_top != mm->top_most || teacher_share != mm->top_share) { // what a captured pass holds
-            CUDA_TRY(cudaStreamSynchronize(mm->st));                    // which nothing runs, and nothing reads the old entries
-            for (auto &g : mm->graphs[GRAPH_BWD_TOP]) {
-                if (g.exec)
-                    CUDA_TRY(cudaGraphExecDestroy(g.exec));
-                g = nncu_model::StepGraph{nullptr, 0, 0};
-            }
-            if (n_top != mm->top_most) {
-                if (mm->top_ids)
-                    CUDA_TRY(cudaFree(mm->top_ids));
-                mm->top_ids = nullptr;
-                mm->top_most = 0;
-                CUDA_TRY(cudaMalloc(&mm->top_ids, n * (sizeof(int32_t) + sizeof(float))));
-            }
-            mm->top_most = n_top;
-            mm->top_share = teacher_share;
-        }
-        CUDA_TRY(cudaMemcpyAsync(mm->top_ids, top_ids_host, n * sizeof(int32_t), cudaMemcpyHostToDevice, mm->st));
-        CUDA_TRY(cudaMemcpyAsync(mm->top_logits(), top_logits_host, n * sizeof(float), cudaMemcpyHostToDevice, mm->st));
-        CUDA_TRY(cudaStreamSynchronize(mm->st)); // the arrays are the caller's again
-        mm->top_now = n_top;
-        return NNCU_OK;
-    }));
+    const TopEntries top = {top_ids_host, top_logits_host, n_top, teacher_share};
+    NNCU_TRY(gradient_common(m, false, &top));
     NNCU_TRY(queue_loss(m));
     if (loss_out)
         return nncu_read_loss(m, loss_out);

@@ -282,6 +282,42 @@ def test_model_and_a_teacher_that_is_not_a_number(pkg, bf16):
     m.close()
 
 
+@gpu
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_model_and_teachers_of_other_sizes_and_shares(pkg, bf16):
+    """Entries and share change from step to step behind captured passes: 40 entries of which three are there are the bits of
+    three; a share's loss lies between the target's own and the teacher's by its weight (fp32 sums of 64 rows: 2^-24 * 64)"""
+    np = pytest.importorskip("numpy")
+    T, B, V = 16, 4, 300
+    rng = np.random.default_rng(11)
+    one, two = _model(pkg, bf16, V), _model(pkg, bf16, V)
+    for m in (one, two):
+        for n in m.info:
+            m.set_param(n, one.get_param(n))
+        m._ck(m.lib.nncu_own_stream(m.h))
+    for step in range(12):
+        ids_in, tg = (rng.integers(0, V, (T, B)).astype(np.int32) for _ in range(2))
+        ids = rng.integers(0, V, (T, B, 3)).astype(np.int32)
+        top = rng.normal(size=(T, B, 3)).astype(np.float32)
+        wide = np.full((T, B, 40), V, np.int32), np.full((T, B, 40), np.nan, np.float32)
+        wide[0][..., :3], wide[1][..., :3] = ids, top
+        share = (0.25, 0.25, 0.25, 0.75)[step % 4]
+        for m in (one, two):
+            m.eval(-1, ids_in, read=False)
+        want = one.eval_gradient_distill(tg, ids, top, share)
+        few = step % 3 == 0
+        assert two.eval_gradient_distill(tg, *((ids, top) if few else wide), share) == want
+        for n in one.info:
+            assert np.array_equal(one.get_grad(n), two.get_grad(n)), (step, n)
+        ends = [two.eval_gradient_distill(tg, ids, top, s) for s in (0.0, 1.0)]
+        assert abs(want - (1 - share) * ends[0] - share * ends[1]) <= 2.0 ** -24 * 64 * (abs(ends[0]) + abs(ends[1]))
+        for m in (one, two):
+            assert m.eval_gradient(tg) == ends[0]
+            m.update()
+    one.close()
+    two.close()
+
+
 # ---------------------------------------------------------------- waits that run out
 
 @pytest.fixture(scope="module")
