@@ -98,6 +98,39 @@ def test_linear_attention_rounds_a_bf16_result_once(pkg, case):
 
 
 @gpu
+@pytest.mark.parametrize("B,d_key,d_value,T", [(40, 64, 64, 64), (150, 64, 64, 200), (40, 32, 32, 130), (3, 128, 128, 130), (6, 64, 64, 1024), (2, 128, 128, 700),
+                                               (3, 40, 64, 333), (150, 32, 96, 90)])
+def test_linear_attention_states_are_fp32_sums_of_fp32_products(pkg, B, d_key, d_value, T):
+    """Each stream has one token that is not zero, in its last 60 (first 60 for the gradient): a state is that token's product times
+    a power of the decay.  Off by that power (two steps, and 2^-24 of its exponent), the decayed factor's rounding, three terms'
+    sums that are cut, a step for each chunk and part behind it: 16 steps of 2^-24.  Two terms of the factor would leave up to 2^-16."""
+    kind = torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(T + d_key)
+    stream = torch.arange(B, device="cuda")
+    live = T - 1 - (7 * stream + 3) % 60
+    one = lambda d: torch.randn(B, d, generator=g, device="cuda").to(kind)  # noqa: E731
+    k, v, q, dout = one(d_key), one(d_value), one(d_key), one(d_value)
+
+    def rows(x, at):
+        y = torch.zeros(T, B, x.shape[1], device="cuda", dtype=kind)
+        y[at, stream] = x
+        return y.view(T * B, -1)
+
+    decay = torch.tensor([0.97])
+    t = dict(q=rows(q, T - 1 - live), k=rows(k, live), v=rows(v, live), dout=rows(dout, T - 1 - live))
+    op = Linear(pkg, (B, 1, d_key, d_value, T), kind, t, decay, None, None, None)
+    _, state = op.forward()
+    dstate = op.backward()[3]
+    l = decay.cuda().double()
+    outer = lambda a, b: a.double()[:, :, None] * b.double()[:, None, :]  # noqa: E731
+    behind = (T - 1 - live)[:, None, None]
+    want = l ** behind * outer(k, v)
+    _near(state[:, 0], want, 16 * 2.0 ** -24 * want.abs(), "state")
+    want = d_key ** -0.5 * l ** (behind + 1) * outer(q, dout)
+    _near(dstate[:, 0], want, 16 * 2.0 ** -24 * want.abs(), "dstate")
+
+
+@gpu
 @pytest.mark.parametrize("d", [16, 64, 7])
 def test_linear_attention_decays_a_token_by_the_decay_given(pkg, d):
     """One token of nothing: the state times the decay, rounded once, forward and back: no bias that calls one after the other
