@@ -470,7 +470,7 @@ int nncu_qk_norm_rope_backward(const nncu_qk_norm_shape *s, const void *q, const
  * decoder's step, a state carried from call to call.  Steps and whole segments add in another order, so that
  * their last bits differ: what one codes the other does not decode.
  * Up to NNCU_LINEAR_ATTN_HEADS_MAX heads of up to NNCU_LINEAR_ATTN_DIM_MAX values (NNCU_ERR_RANGE beyond).  A value
- * that is not finite reaches rows of its stream from up to 63 tokens before it on.
+ * that is not finite reaches rows of its stream from up to 63 tokens before it on, as NaN where the formula gives infinity.
  * More than eight tokens of fp32 are multiplied in two parts of 11 bits: values from 3.40e38 on count as infinite,
  * those below 1e-34 may keep the first part only.
  */

@@ -24,8 +24,8 @@ static int distill_check(const nncu_distill_shape *s)
 }
 
 // An SM takes as many CTAs as rows fit its shared memory, each with a place or, where eight fit twice, more: one loads
-// while others compute (rows of 16384 fp32 logits, 2048 of them, loss and gradient: three CTAs of one place 55 us, one CTA of
-// three places 78).  Some 1024 threads an SM share them.
+// while others compute (rows of 16384 fp32 logits, 2048 of them, loss and gradient: three CTAs of one place 46 us, two 58, one
+// of three places 83).  Some 1024 threads an SM share them.
 template <typename TZ, typename TG, int WHAT, int HARD> static int distill_launch(distill::Args &a, cudaStream_t st)
 {
     const int entries = 2 * 3 * 4 * a.K4, fixed = entries + 4 * distill::PLACES + 2560; // static arrays and what a CTA costs

@@ -14,8 +14,9 @@
 // gradient.  (A row that is loaded, reduced twice and stored in turn leaves HBM idle most of the time: 2048 rows of 16384
 // logits, loss and gradient, took 69 us with a row in the registers of a CTA.)  What of a row does not lie in whole
 // 16-byte pieces, at its two ends, is a thread's each.  2048 rows of 16384 fp32 logits with a bf16 gradient, 64 entries a
-// row: 45 us, 201 MB at 4.5 TB/s; bound by the issue of instructions (25 for a logit, 11 of them in the three passes, the rest
-// a row's own) and by the barriers that a row's warps wait at for those with entries.
+// row: 46 us, 201 MB at 4.4 TB/s.  Nothing is full: instructions issue in 58 % of the cycles (25 for a logit, 11 of them in the
+// three passes, the rest a row's own: the wait for it, reductions, entries); a row of 64 KB leaves an SM three CTAs of one place
+// each, which wait for their copies and at barriers for the warps with entries.
 //
 // Exponentials are what an SM has least of, sixteen a cycle.  Where tau is 1 or 2, or one of the terms is not there, p
 // is 2^u or its square over their sum: one exponential a logit and pass instead of two.
@@ -140,8 +141,8 @@ struct Kept {
 // RING: rows through shared memory; otherwise rows too long for it are read from global memory each time, one to a CTA.
 //
 // LATE: what the entries' symbols get is computed while the next row is on its way, from what the warps have kept, and not
-// before the dense gradient: for CTAs of several rows (2048 of 16384 fp32 logits: 49.0 -> 46.2 us; at one row a CTA there is
-// nothing to wait for, 650 of 9208 bf16 logits, loss and gradient apart: 12.65 -> 13.0).
+// before the dense gradient: for CTAs of several rows (2048 of 16384 fp32 logits: 48.5 -> 46.3 us; at one row a CTA there is
+// nothing to wait for, 650 of 9208 bf16 logits, loss and gradient apart: 13.05 -> 13.65).
 //
 // Two barriers a row.  What one row leaves for behind a barrier -- the named entries over its dense gradient, its place in the
 // ring for the next copy -- is done behind the first one of the next row; entries and partial sums lie in two

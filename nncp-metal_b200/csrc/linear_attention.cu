@@ -27,7 +27,7 @@ static int lin_check(const nncu_linear_attn_shape *s)
 // In how many parts a stream's tokens are cut.  One part is one pass over the tokens; more parts read b and c
 // twice, and pay where one CTA for each (stream, head) would leave most SMs without work.  Parts of one chunk while there are
 // 16 at most, of two behind that, since each goes through the sums of all before it (1 x 2 pairs of 1000 tokens of 128, bf16,
-// in 4, 8 and 16 parts: 37, 26 and 23 us; one pair of 4096 of 64 in 16, 32 and 64: 19.5, 18.0 and 24.2).
+// in 4, 8 and 16 parts: 42, 27 and 24 us; one pair of 4096 of 64 in 16, 32 and 64: 21.5, 20.4 and 26.2).
 static void lin_parts(const nncu_linear_attn_shape *s, int roles, int *n_seg, int *seg)
 {
     const long long ctas = (long long)s->n_streams * s->n_head * roles;
@@ -37,7 +37,7 @@ static void lin_parts(const nncu_linear_attn_shape *s, int roles, int *n_seg, in
     const int n = (int)std::min<long long>(std::max<long long>(want / ctas, 1), std::max(std::min(chunks, 16), chunks / 2));
     int each = ceil_div(chunks, n);
     // a chunk of the first pass takes 0.6 of one of the second, both passes together a chunk more (two chunks of 64 tokens, 8
-    // pairs of 64: 6.4 us in one part, 7.2 in two; three 8.6 and 7.5)
+    // pairs of 64: 7.6 us in one part, 8.2 in two; three 9.8, in three parts 8.6)
     if (8ll * each + 5 > 5ll * chunks)
         each = chunks;
     *seg = each * chunk;
@@ -310,8 +310,8 @@ int nncu_linear_attention_backward(const nncu_linear_attn_shape *s, const void *
     rq.s_state = rq.s_pair = rk.s_pair = rv.s_pair = rk.s_in = rv.s_in = s->scale;
     rq.s_in = rk.s_state = rv.s_state = 1.0f;
     // bf16 rows in 16-byte pieces, head sizes from 33 to 64: dk beside dv, from the same tiles and the same state, where three
-    // CTAs for each (stream, head) are more than the two an SM that run in one round (128 pairs of 2048 tokens, backward 151 ->
-    // 128 us, 256 of 512 75 -> 67; 32 pairs of 1024 33 -> 52), and where different head sizes would make two launches
+    // CTAs for each (stream, head) are more than the two an SM that run in one round (128 pairs of 2048 tokens, backward 185 ->
+    // 155 us, 256 of 512 89 -> 80; 32 pairs of 1024 40 -> 62), and where different head sizes would make two launches
     const int least = std::min(s->d_key, s->d_value), most = std::max(s->d_key, s->d_value);
     if (s->dtype_bf16 && s->seg_len > lin::STEP_TOKENS && least > 32 && most <= 64 &&
         (3ll * s->n_streams * s->n_head * all.n_seg > 2 * SMS || s->d_key != s->d_value)) {

@@ -600,17 +600,18 @@ template <bool STATES> __global__ void __launch_bounds__(256) quad_kernel(const 
 // (and 16 (r + 4) .. of 128) in fp32 accumulators.  The results need all of the state: it goes through shared memory as two
 // bf16 terms, and so do the pair weights P.  What 16 bits leave out, 2^-16 of each, is far below a result's own rounding;
 // with one term each the errors against 64 bits were 2.35e-3 of the results instead of the 1.66e-3 of that rounding
-// (128 pairs of 2048 tokens of 64, forward: 62.7 us, now 76.6).  Products of a decayed b with c, which the state adds up, are
+// (128 pairs of 2048 tokens of 64, forward: 62.7 us, now 77).  Products of a decayed b with c, which the state adds up, are
 // kept to 24 bits by three bf16 terms of the decayed value, so that the state is an fp32 sum of fp32 products.  Pair weights
 // and terms are the same for the CG warps of the same rows: each computes every CG-th and they meet at a barrier of their own.
 //
 // Tiles come by TMA, 64 tokens x 64 (32) values of a head a copy, from a map of (value, head, stream, token): what lies beyond
-// a head's values or the sequence arrives as zeros.  One thread asks for the next chunk's under the present chunk; one
-// barrier a chunk hands over tiles and state.  In the reverse order a chunk's row i is the tile's row 63 - i.
+// a head's values or the sequence arrives as zeros.  One thread asks for the next chunk's under the present chunk; a
+// barrier hands over tiles and state, another one frees the state's place when all have read it (in the middle
+// of the chunk that one is no faster).  In the reverse order a chunk's row i is the tile's row 63 - i.
 //
 // Bound by the chain of a chunk's phases (weights, what the state gives, products with c, the state to the next chunk) in
-// too few warps to hide it: the tensor pipe is active 40 to 52 % of the time, shared memory 44 to 66, an instruction
-// issues in 35 to 45.  8 x 16 pairs of 2048 tokens of 64, forward and backward: 231 us, 50 GFLOP of the chunk form's
+// too few warps to hide it: the tensor pipe is active 40 to 55 % of the time (of single chunks 23), shared memory 33 to 46, an
+// instruction issues in 29 to 43.  8 x 16 pairs of 2048 tokens of 64, forward and backward: 231 us, 50 GFLOP of the chunk form's
 // products, in two or three terms but for the pair weights, 218 TFLOP/s of the 550 that this instruction reaches; the bytes
 // alone 41.5 us.  2 x 8 pairs of 4096 tokens of 128, forward, in eight parts: 77 us (both passes), bytes 10.5.
 
@@ -731,7 +732,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
         }
         __syncthreads();
     }
-    pdl_wait(); // no early trigger: successors resident beside these CTAs cost more than their launch (128 pairs of 2048 tokens 144 -> 97 us)
+    pdl_wait(); // no early trigger: successors resident beside these CTAs cost more than their launch (128 pairs of 2048 tokens 110 -> 78 us)
     const Rows rows(p, q, b);
     const size_t nn = (size_t)q.da * q.dc;
     if (STATES && !q.s_end && g == p.n_seg - 1) // nobody asks for the last part's sum
@@ -1075,7 +1076,7 @@ __global__ void __launch_bounds__(4 * DC, DA <= 64 && DC <= 64 ? 2 : 1) mma_kern
             }
         }
         row_barrier();
-        // the third term where a state is a result; 17 bits are more than the roundings behind them keep
+        // the third term where a state is a result; elsewhere the state is a factor, of which 16 bits are kept
         const bool third = follows && q.s_end;
         // what the chunk adds has sums of its own: products cut the sum they are added to, the state is rounded
         float add[MT][NT][4];
