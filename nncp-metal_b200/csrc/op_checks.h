@@ -2,9 +2,10 @@
 #pragma once
 #include <initializer_list>
 
+#include "attention_deal.h"
 #include "common.cuh"
 
-static const int SMS = 148;
+using attn::SMS;
 
 static inline bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
